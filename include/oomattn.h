@@ -53,7 +53,26 @@ typedef enum oomattn_status {
   OOMATTN_ERR_DEVICE_CHECK = 9  /* a kernel's own index check failed */
 } oomattn_status;
 
-enum { OOMATTN_DTYPE_F32 = 0, OOMATTN_DTYPE_BF16 = 1 };
+/* OOMATTN_DTYPE_Q4 is a cache type only (oomattn_config.kv_dtype); tensors
+ * that go in and out are f32 or bf16. */
+enum { OOMATTN_DTYPE_F32 = 0, OOMATTN_DTYPE_BF16 = 1, OOMATTN_DTYPE_Q4 = 2 };
+/* The 4-bit cache.  The 128 values of a (token, kv head) row of K or V are
+ * four groups of 32.  With x a group,
+ *   s = f16(bf16((max x - min x) / 15)), o = f16(min x + 8 s),
+ *   c = clamp(rint((x - o) / s) + 8, 0, 15)   (8 where s = 0)
+ * and the row stands for o + (c - 8) s: 80 bytes instead of 256 in bf16, each
+ * value off by at most 0.53 s + 2^-12 |o|.  Values saturate at +-60000; a
+ * group that holds a NaN reads back as NaN; groups whose values differ by less
+ * than about 1e-5 keep only their middle.
+ * A page of 16 tokens of one kv head is a chunk of OOMATTN_Q4_CHUNK bytes in
+ * the K pool and one in the V pool, chunk (layer, page, kv) at
+ * ((layer*(n_pages+1) + page)*n_kv + kv) * OOMATTN_Q4_CHUNK:
+ *   K: token r, dims 32w + 8t + n (w, t < 4, n < 8): nibble n of the 32-bit
+ *      word at 64r + 16t + 4w; f16 o[0..3], s[0..3] at 1024 + 16r.
+ *   V: token r = 8h + 2t + p (p < 2), dims 32w + 4g + n (g < 8, n < 4): nibble
+ *      n of the 16-bit piece at 512h + 64g + 16t + 4w + 2p; f16 s at
+ *      1024 + 64h + 16t + 4w + 2p, f16 o 128 bytes behind it. */
+#define OOMATTN_Q4_CHUNK 1280
 /* Floats per (row, q head) in the packed decode output: O in [0, 128), the
  * natural-log LSE at 128, 3 floats of padding (16-byte aligned rows). */
 #define OOMATTN_PACKED_STRIDE 132
@@ -76,7 +95,7 @@ typedef struct oomattn_config {
   int32_t max_seqs;     /* sequence slots (batch rows) */
   int32_t page_size;    /* must be 16 */
   int32_t n_pages;      /* pages per layer pool shared by all sequences */
-  int32_t kv_dtype;     /* OOMATTN_DTYPE_F32 or OOMATTN_DTYPE_BF16 */
+  int32_t kv_dtype;     /* OOMATTN_DTYPE_F32, OOMATTN_DTYPE_BF16 or OOMATTN_DTYPE_Q4 */
   int32_t rope_variant; /* OOMATTN_ROPE_* */
   float rope_theta;     /* 1e6 for Qwen2.5, 5e5 for Llama-3 */
   float softmax_scale;  /* <= 0 selects 1/sqrt(head_dim) (src/oomllama_turbo.rs:688) */
@@ -141,8 +160,8 @@ int oomattn_set_position_offset(oomattn_ctx* ctx, int32_t seq, int32_t offset);
 int oomattn_set_seq_len(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t len);
 
 /* Device addresses of the K and V pools: element (layer, page, kv, slot, d)
- * at (((layer*(n_pages+1) + page)*n_kv + kv)*16 + slot)*128 + d, in kv_dtype.
- * Page n_pages is the null page. */
+ * at (((layer*(n_pages+1) + page)*n_kv + kv)*16 + slot)*128 + d, in kv_dtype
+ * (4-bit: chunks, see OOMATTN_Q4_CHUNK).  Page n_pages is the null page. */
 int oomattn_kv_pool(const oomattn_ctx* ctx, void** k_pool, void** v_pool);
 
 /* LayerKVCache::append (src/oomllama_turbo.rs:41-55) of already-rotated rows:
@@ -151,8 +170,17 @@ int oomattn_kv_write(oomattn_ctx* ctx, int32_t layer, int32_t seq, const void* k
                      int32_t src_dtype);
 
 /* LayerKVCache::get (src/oomllama_turbo.rs:57-63): copies the layer's cache of
- * `seq` to host k_out, v_out [n_kv][len][128] in kv_dtype (synchronises). */
+ * `seq` to host k_out, v_out [n_kv][len][128] in kv_dtype, the values of a
+ * 4-bit cache in f32 (synchronises). */
 int oomattn_kv_read(oomattn_ctx* ctx, int32_t layer, int32_t seq, void* k_out /* host */, void* v_out /* host */);
+
+/* The same on the device: the values of n cached rows of each sequence, from
+ * slot starts[i] (NULL: 0), to k_out, v_out [n_seqs * n][n_kv][128] (device,
+ * 16-byte aligned) in out_dtype.  Every slot must be below the sequence's
+ * length; a sequence may appear more than once. */
+int oomattn_kv_gather(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids /* host */,
+                      const int32_t* starts /* host, may be NULL */, int32_t n, int32_t out_dtype, void* k_out,
+                      void* v_out);
 
 /* Host copy of the f32 RoPE table rows [pos0, pos0+n) as cos, sin
  * [n][64] (compute_rope_freqs, src/oomllama_turbo.rs:376-396). */
@@ -176,6 +204,28 @@ int oomattn_rope_append(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const i
                         int32_t n_new, const void* q, const void* k, const void* v, int32_t in_dtype,
                         const float* bq, const float* bk, const float* bv, void* q_out, int32_t q_out_dtype);
 
+/* Weights of a norm of every q and k head between bias and RoPE: y / sqrt(mean
+ * of y^2 over the head's 128 values + eps) * weight, in f32.  Device f32 [128],
+ * 16-byte aligned, one for all heads; a NULL weight leaves that side as it is. */
+typedef struct oomattn_qk_norm {
+  const float* q;
+  const float* k;
+  float eps; /* finite, >= 0 */
+} oomattn_qk_norm;
+
+/* oomattn_rope_append with a norm of the q and k heads in the same pass (norm
+ * NULL: none) and, where starts (host) is not NULL, the sequences' first new
+ * slots: starts[i] <= the sequence's length in `layer`; the rows behind it are
+ * given up and its length becomes starts[i] + n_new (drafted tokens that were
+ * not accepted).  No counterpart in the reference, whose models have neither.
+ * The append into a 4-bit cache is this entry point's too: K and V rows are
+ * quantised as they are written. */
+int oomattn_rope_append_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids /* host */,
+                                const int32_t* starts /* host, may be NULL */, int32_t n_new, const void* q,
+                                const void* k, const void* v, int32_t in_dtype, const float* bq, const float* bk,
+                                const float* bv, const oomattn_qk_norm* norm /* host struct, may be NULL */,
+                                void* q_out, int32_t q_out_dtype);
+
 /* The q half of the RoPE step (TurboEngine::apply_rope, src/oomllama_turbo.rs:
  * 737-786, and apply_rope :402-438, by the context's variant) at explicit
  * positions, with nothing appended: q rows [n_rows][n_heads][128] in in_dtype
@@ -184,6 +234,11 @@ int oomattn_rope_append(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const i
  * they attend with the same rotated query as the rank that appends it. */
 int oomattn_rope_q(oomattn_ctx* ctx, int32_t n_rows, const int32_t* positions /* host */, const void* q,
                    int32_t in_dtype, const float* bq, void* q_out, int32_t q_out_dtype);
+
+/* oomattn_rope_q with the norm of the q heads (norm->k is not used). */
+int oomattn_rope_q_qk_norm(oomattn_ctx* ctx, int32_t n_rows, const int32_t* positions /* host */, const void* q,
+                           int32_t in_dtype, const float* bq, const oomattn_qk_norm* norm /* host struct, may be NULL */,
+                           void* q_out, int32_t q_out_dtype);
 
 /* Fused QKV projection + bias + RoPE + append (src/oomllama_turbo.rs:638-681).
  *   x: f32 [T][hidden]; wq [n_heads*128][hidden], wk/wv [n_kv*128][hidden] in
@@ -194,6 +249,15 @@ int oomattn_qkv_rope_append(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, con
                             int32_t n_new, const float* x, const void* wq, const void* wk, const void* wv,
                             int32_t w_dtype, const float* bq, const float* bk, const float* bv, void* q_out,
                             int32_t q_out_dtype);
+
+/* The same with a norm of the q and k heads.  With a norm, or into a 4-bit
+ * cache, the projections are their own kernels at every T (the append needs
+ * whole heads). */
+int oomattn_qkv_rope_append_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids /* host */,
+                                    int32_t n_new, const float* x, const void* wq, const void* wk, const void* wv,
+                                    int32_t w_dtype, const float* bq, const float* bk, const float* bv,
+                                    const oomattn_qk_norm* norm /* host struct, may be NULL */, void* q_out,
+                                    int32_t q_out_dtype);
 
 /* ---------------------------------------------------------------- K-B */
 
@@ -233,8 +297,9 @@ int oomattn_merge_packed(oomattn_ctx* ctx, int32_t n_parts, int32_t n_rows, cons
  * fixed 8.1 MiB array inside the library's device image (every GPU that loads
  * the library holds one copy until the process exits).
  *   device, stream: the GPU and cudaStream_t to run on
- *   kv_dtype: OOMATTN_DTYPE_BF16 or OOMATTN_DTYPE_F32
- *   k_pool, v_pool: [n_pool_pages][n_kv_heads][16][128] in kv_dtype, 16-byte aligned
+ *   kv_dtype: OOMATTN_DTYPE_BF16, OOMATTN_DTYPE_F32 or OOMATTN_DTYPE_Q4
+ *   k_pool, v_pool: [n_pool_pages][n_kv_heads][16][128] in kv_dtype (4-bit:
+ *     chunks [n_pool_pages][n_kv_heads][OOMATTN_Q4_CHUNK]), 16-byte aligned
  *   block_table: device int32 [n_block_rows][max_pages_per_seq]
  *   q, out: f32 [n_rows][n_heads][128]; lse: f32 [n_rows][n_heads] or NULL
  *   seq_ids, lens (host): row z attends to the first lens[z] slots of block-table row seq_ids[z]
@@ -246,7 +311,8 @@ int oomattn_merge_packed(oomattn_ctx* ctx, int32_t n_parts, int32_t n_rows, cons
  *     the pool's last page and reported by oomattn_decode_static_scratch_status,
  *     so the pool should end with a zeroed page that no sequence uses;
  *   - slots past lens[z] in a row's last page hold finite values (they are
- *     weighted by zero, and 0 x inf or 0 x NaN would reach the output).
+ *     weighted by zero, and 0 x inf or 0 x NaN would reach the output); in a
+ *     4-bit cache they may hold anything.
  * Limits: n_rows <= 128, n_kv_heads <= 64, n_heads / n_kv_heads <= 8; larger
  * requests return OOMATTN_ERR_OUT_OF_RANGE.  The split count is capped so
  * that n_rows * n_heads * splits <= 16384.  The first call on a device looks
@@ -272,8 +338,9 @@ int oomattn_decode_static_scratch_status(int device, void* stream, int32_t* flag
 
 /* ---------------------------------------------------------------- K-C */
 
-/* Causal prefill of the n_new newest tokens of `seq` (bf16 cache only):
- * query i (absolute slot len-n_new+i) attends to slots 0..len-n_new+i.
+/* Causal prefill of the n_new newest tokens of `seq` (bf16 or 4-bit cache; a
+ * 4-bit one's rows are taken as bf16 where there are more than 16 queries or
+ * the output is f32, exactly otherwise): query i (absolute slot len-n_new+i) attends to slots 0..len-n_new+i.
  *   q: bf16 [n_new][n_heads][128] rotated; out: [n_new][n_heads][128] in
  *   out_dtype; lse: f32 [n_new][n_heads] or NULL. */
 int oomattn_prefill(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_new, const void* q, void* out,
@@ -316,6 +383,13 @@ int oomattn_attention_forward_with_bias(oomattn_ctx* ctx, int32_t layer, int32_t
                                         const float* x, const float* wq, const float* wk, const float* wv,
                                         const float* wo, int32_t o_out, const float* bq, const float* bk,
                                         const float* bv, float* out);
+
+/* The same with a norm of the q and k heads between bias and RoPE. */
+int oomattn_attention_forward_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t batch, int32_t seq_len,
+                                      const float* x, const float* wq, const float* wk, const float* wv,
+                                      const float* wo, int32_t o_out, const float* bq, const float* bk,
+                                      const float* bv, const oomattn_qk_norm* norm /* host struct, may be NULL */,
+                                      float* out);
 
 /* ------------------------------------------- K-E: GPU-resident Q8 weights */
 
@@ -401,6 +475,11 @@ typedef struct oomattn_q8_layer {
 int oomattn_decoder_layer_q8(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids /* host */,
                              const float* x, const oomattn_q8_layer* w /* host struct */, float* out);
 
+/* The same with a norm of the q and k heads between bias and RoPE. */
+int oomattn_decoder_layer_q8_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids /* host */,
+                                     const float* x, const oomattn_q8_layer* w /* host struct */,
+                                     const oomattn_qk_norm* norm /* host struct, may be NULL */, float* out);
+
 /* ------------------------------------------------------------------ .oom files */
 
 /* One tensor of an .oom file: OomTensorMeta (src/quant.rs:307-312) plus where
@@ -481,11 +560,22 @@ int oomattn_decode_step_q8(oomattn_ctx* ctx, const oomattn_q8_model* m /* host s
  * appends their K/V to its cache (K-A), attends causally over each sequence
  * (K-C) and runs its projections and MLP on the tensor cores (Q8 weights); the
  * final RMSNorm, LM head and argmax of each sequence's last prompt token give
- * next[b] (device; logits [n_seqs][vocab] or NULL).  Needs a bf16 cache; the
+ * next[b] (device; logits [n_seqs][vocab] or NULL).  Needs a bf16 or 4-bit cache; the
  * sequences' lengths grow by n_new in every layer. */
 int oomattn_prefill_step_q8(oomattn_ctx* ctx, const oomattn_q8_model* m /* host struct */, int32_t n_seqs,
                             const int32_t* seq_ids /* host */, int32_t n_new, const int32_t* tokens, int32_t* next,
                             float* logits);
+
+/* Both steps of a model whose q and k heads are normed: norms is a host array
+ * [m->n_layers], or NULL. */
+int oomattn_decode_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q8_model* m /* host struct */,
+                                   const oomattn_qk_norm* norms /* host, may be NULL */, int32_t n_seqs,
+                                   const int32_t* seq_ids /* host */, const int32_t* tokens, int32_t* next,
+                                   float* logits);
+int oomattn_prefill_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q8_model* m /* host struct */,
+                                    const oomattn_qk_norm* norms /* host, may be NULL */, int32_t n_seqs,
+                                    const int32_t* seq_ids /* host */, int32_t n_new, const int32_t* tokens,
+                                    int32_t* next, float* logits);
 
 
 #ifdef __cplusplus

@@ -16,7 +16,8 @@ STATUS_NAMES = {
     0: "OK", 1: "INVALID_ARG", 2: "BAD_CONFIG", 3: "OUT_OF_RANGE", 4: "CUDA", 5: "NCCL", 6: "TIMEOUT",
     7: "NO_MEMORY", 8: "UNSUPPORTED", 9: "DEVICE_CHECK",
 }
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_Q4 = 0, 1, 2   # Q4: a cache type only
+Q4_CHUNK = 1280                     # bytes of a page of one kv head in a 4-bit K or V pool
 PACKED_STRIDE = 132                 # floats per (row, q head) of a packed decode output: O[128], lse, pad
 TEST_DROP_DECODE_COPIES = 1         # oomattn_set_test_flags: the bf16 decode's producer issues no copies
 TEST_DROP_LINEAR_COPIES = 2         # oomattn_set_test_flags: the Q8 tensor-core pass's producer issues no copies
@@ -34,6 +35,9 @@ EXPORTS = (
     "oomattn_set_wait_limit", "oomattn_set_test_flags", "oomattn_rope_q", "oomattn_decode_packed",
     "oomattn_merge_packed", "oomattn_decode_static_scratch_status", "oomattn_prefill_blocks",
     "oomattn_linear", "oomattn_prefill_step_q8",
+    "oomattn_kv_gather", "oomattn_rope_append_qk_norm", "oomattn_rope_q_qk_norm", "oomattn_qkv_rope_append_qk_norm",
+    "oomattn_attention_forward_qk_norm", "oomattn_decoder_layer_q8_qk_norm", "oomattn_decode_step_q8_qk_norm",
+    "oomattn_prefill_step_q8_qk_norm",
 )
 
 
@@ -82,6 +86,11 @@ class Q8Model(ctypes.Structure):
                 ("lm_head", Q8Matrix), ("final_norm", ctypes.c_void_p), ("eps", ctypes.c_float)]
 
 
+class QkNorm(ctypes.Structure):
+    """oomattn_qk_norm: weights [128] and eps of a norm of every q and k head."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("eps", ctypes.c_float)]
+
+
 _lib = None
 
 
@@ -95,6 +104,7 @@ def load():
     L = ctypes.CDLL(LIB_PATH)
     P, I, F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_float
     IP = ctypes.POINTER(ctypes.c_int32)
+    NP = ctypes.POINTER(QkNorm)
     sig = {
         "oomattn_version": ([], ctypes.c_char_p),
         "oomattn_create": ([ctypes.POINTER(Config), ctypes.c_int, P, ctypes.POINTER(P)], ctypes.c_int),
@@ -141,6 +151,14 @@ def load():
         "oomattn_prefill_blocks": ([P, I, I, I, P, P, I, P, I, IP], ctypes.c_int),
         "oomattn_linear": ([P, P, P, I, I, I, I, P, P], ctypes.c_int),
         "oomattn_prefill_step_q8": ([P, ctypes.POINTER(Q8Model), I, IP, I, P, P, P], ctypes.c_int),
+        "oomattn_kv_gather": ([P, I, I, IP, IP, I, I, P, P], ctypes.c_int),
+        "oomattn_rope_append_qk_norm": ([P, I, I, IP, IP, I, P, P, P, I, P, P, P, NP, P, I], ctypes.c_int),
+        "oomattn_rope_q_qk_norm": ([P, I, IP, P, I, P, NP, P, I], ctypes.c_int),
+        "oomattn_qkv_rope_append_qk_norm": ([P, I, I, IP, I, P, P, P, P, I, P, P, P, NP, P, I], ctypes.c_int),
+        "oomattn_attention_forward_qk_norm": ([P, I, I, I, P, P, P, P, P, I, P, P, P, NP, P], ctypes.c_int),
+        "oomattn_decoder_layer_q8_qk_norm": ([P, I, I, IP, P, ctypes.POINTER(Q8Layer), NP, P], ctypes.c_int),
+        "oomattn_decode_step_q8_qk_norm": ([P, ctypes.POINTER(Q8Model), NP, I, IP, P, P, P], ctypes.c_int),
+        "oomattn_prefill_step_q8_qk_norm": ([P, ctypes.POINTER(Q8Model), NP, I, IP, I, P, P, P], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)

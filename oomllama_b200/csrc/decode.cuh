@@ -50,6 +50,16 @@ struct MergeSmem {
 
 __device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
+// Four dims of a finished output row, as f32 or (OUT16) rounded to bf16.
+template <bool OUT16>
+__device__ __forceinline__ void store_out4(const DecodeArgs& a, size_t zh, int d, float x0, float x1, float x2, float x3) {
+  if (OUT16)
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + zh * a.o_stride + d) =
+        make_uint2(pack_bf16(x0, x1), pack_bf16(x2, x3));
+  else
+    *reinterpret_cast<float4*>(a.out + zh * a.o_stride + d) = make_float4(x0, x1, x2, x3);
+}
+
 // The last CTA's merge when it has a shared-memory area to stage into (the
 // bf16 kernel's page ring, free by then): every (q head, split) partial O row
 // of the (row, kv head) is copied in by cp.async (one warp per row, one lane
@@ -64,6 +74,7 @@ __device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, 128;"
 // instead of 2.2-4 us at 6-32 splits; the decode of a 16-row, 67 MB layer
 // 18.3 -> 16.6 us.  The sums still run in split order, so the result is the
 // same to the bit.
+template <bool OUT16>
 __device__ __forceinline__ void merge_splits_staged(const DecodeArgs& a, int z, int g, int nsplit, int tid,
                                                     float* stage, int stage_floats, float* s_w) {
   const int j = tid >> 4, da = (tid & 15) * 4, db = da + kHeadDim / 2;
@@ -128,9 +139,9 @@ __device__ __forceinline__ void merge_splits_staged(const DecodeArgs& a, int z, 
   if (active) {
     const int h = g * a.group + j;
     const float inv = 1.f / wsum;
-    float* orow = a.out + ((size_t)z * a.n_heads + h) * a.o_stride;
-    *reinterpret_cast<float4*>(orow + da) = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
-    *reinterpret_cast<float4*>(orow + db) = make_float4(acc[4] * inv, acc[5] * inv, acc[6] * inv, acc[7] * inv);
+    const size_t zh = (size_t)z * a.n_heads + h;
+    store_out4<OUT16>(a, zh, da, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    store_out4<OUT16>(a, zh, db, acc[4] * inv, acc[5] * inv, acc[6] * inv, acc[7] * inv);
     if (a.lse && (tid & 15) == 0)
       a.lse[((size_t)z * a.n_heads + h) * a.lse_stride] = (M + log2f(wsum)) * 0.69314718055994531f;
   }
@@ -145,6 +156,7 @@ __device__ __forceinline__ void merge_splits_staged(const DecodeArgs& a, int z, 
 // (`stage`, and `s_w` for the weights) the merge is merge_splits_staged;
 // without one (the f32 kernel, which holds no shared ring) the partials are
 // loaded into registers.
+template <bool OUT16 = false>
 __device__ __forceinline__ void combine_and_store(const MergeSmem& ms, const DecodeArgs& a, int z, int g, int split,
                                                   int nsplit, int n_kv, int tid, int* s_last, float* stage,
                                                   int stage_floats, float* s_w) {
@@ -177,9 +189,9 @@ __device__ __forceinline__ void combine_and_store(const MergeSmem& ms, const Dec
     for (int i = 0; i < 8; ++i) acc[i] *= inv;
     lse2 = M + log2f(lsum);
     if (nsplit == 1) {
-      float* orow = a.out + ((size_t)z * a.n_heads + h) * a.o_stride;
-      *reinterpret_cast<float4*>(orow + da) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      *reinterpret_cast<float4*>(orow + db) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      const size_t zh = (size_t)z * a.n_heads + h;
+      store_out4<OUT16>(a, zh, da, acc[0], acc[1], acc[2], acc[3]);
+      store_out4<OUT16>(a, zh, db, acc[4], acc[5], acc[6], acc[7]);
       if (a.lse && (tid & 15) == 0)
         a.lse[((size_t)z * a.n_heads + h) * a.lse_stride] = lse2 * 0.69314718055994531f;
     } else {
@@ -199,7 +211,7 @@ __device__ __forceinline__ void combine_and_store(const MergeSmem& ms, const Dec
   consumer_bar();
   if (!*s_last) return;
   if (stage != nullptr) {
-    merge_splits_staged(a, z, g, nsplit, tid, stage, stage_floats, s_w);
+    merge_splits_staged<OUT16>(a, z, g, nsplit, tid, stage, stage_floats, s_w);
     if (tid == 0) a.counters[(size_t)z * n_kv + g] = 0u;
     return;
   }

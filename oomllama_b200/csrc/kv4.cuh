@@ -1,0 +1,211 @@
+// The 4-bit KV cache: its format, the quantiser, and the kernel that reads
+// cached rows back as values (of any cache type).
+//
+// A page of 16 tokens of one kv head is one 1280-byte chunk in the K pool and
+// one in the V pool.  The 128 values of a token are four groups of 32; with x
+// the group,
+//   s = f16(bf16((max x - min x) / 15))      (f32 division; 8 significant bits)
+//   o = f16(min x + 8 s)
+//   c = clamp(rint((x - o) / s) + 8, 0, 15)  (8 where s = 0)
+// and the group stands for o + (c - 8) s.  The roundings: a code is off by at
+// most half a step s; s rounded to 8 bits moves the end of a group's range by
+// at most 15 s 2^-9 < 0.03 s; o is off by at most 2^-12 |o|.  s has 8 bits so
+// that (c - 8) s, a 4-bit number times an 8-bit one, is exact in f16.  A group
+// that holds a NaN reads back as NaN; values saturate at +-60000, which keeps
+// s <= 8000 and (c - 8) s <= 64000 finite in f16.  5 bits per value, against
+// 16: 160 bytes instead of 512 for a token's K and V of one kv head.
+//
+// The codes lie in the order in which the decode kernel's lanes want them as
+// tensor-core operands, so that a lane's 128-bit load is its operand and no
+// shuffle is needed (lane = 4 g + t, g = lane / 4 = 0..7, t = lane % 4):
+//   K: token r (0..15), dims 32 w + 8 t + n (w = group, n = 0..7): nibble n of
+//      the 32-bit word at r * 64 + t * 16 + w * 4;
+//      then at 1024 + r * 16 the token's f16 o[0..3], s[0..3].
+//   V: token r = 8 h + 2 t + p (p = 0, 1), dims 32 w + 4 g + n (n = 0..3):
+//      nibble n of the 16-bit piece at h * 512 + g * 64 + t * 16 + w * 4 + p * 2;
+//      then f16 s at 1024 and o at 1152, each at + h * 64 + t * 16 + w * 4 + p * 2.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "params.cuh"
+
+namespace oomattn {
+
+constexpr int kQ4Chunk = 1280;        // bytes of a (page, kv head) chunk of K or of V
+constexpr int kQ4Meta = 1024;         // its scales and offsets
+constexpr int kQ4VOffsets = 1152;     // V: the offsets, behind the scales
+constexpr float kQ4Sat = 60000.f;
+static_assert(kPageSize == 16 && kHeadDim == 128, "the chunk layout");
+
+enum : int { kKvF32 = 0, kKvBf16 = 1, kKvQ4 = 2 };  // cache types, as OOMATTN_DTYPE_*
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// Scale and offset of a group from its least and greatest value (NaN in both
+// where the group holds one).
+__device__ __forceinline__ void q4_params(float lo, float hi, __half& s, __half& o) {
+  if (!(lo <= hi)) {  // a NaN
+    s = __ushort_as_half(0);
+    o = __ushort_as_half(0x7fff);
+    return;
+  }
+  lo = fminf(fmaxf(lo, -kQ4Sat), kQ4Sat);
+  hi = fminf(fmaxf(hi, -kQ4Sat), kQ4Sat);
+  s = __float2half_rn(__bfloat162float(__float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f))));
+  o = __float2half_rn(__fadd_rn(lo, __fmul_rn(8.f, __half2float(s))));
+}
+
+__device__ __forceinline__ uint32_t q4_code(float x, float s, float o) {
+  if (!(s > 0.f)) return 8u;
+  // rint, then clamped: an infinite x gives an end of the range
+  const float c = rintf(__fdiv_rn(__fsub_rn(x, o), s));
+  return (uint32_t)(int)(fminf(fmaxf(c, -8.f), 7.f) + 8.f);
+}
+
+__device__ __forceinline__ float q4_value(uint32_t code, float s, float o) {
+  return __fadd_rn(o, __fmul_rn((float)((int)code - 8), s));
+}
+
+// Chunk of (layer, page, kv head) in a 4-bit pool.
+__device__ __forceinline__ size_t q4_chunk_off(const KVPool& pool, int layer, int page, int g) {
+  return ((size_t)((size_t)layer * pool.n_pool_pages + page) * pool.n_kv + g) * kQ4Chunk;
+}
+
+// Byte offsets inside a chunk.
+__host__ __device__ __forceinline__ int q4_k_word(int tok, int block) {  // the 8 dims [8 block, 8 block + 8)
+  return tok * 64 + (block & 3) * 16 + (block >> 2) * 4;
+}
+__host__ __device__ __forceinline__ int q4_v_pair(int tok, int g) {  // the 16 bytes of tok's pair (tok & ~1, tok | 1), piece g
+  return (tok >> 3) * 512 + g * 64 + ((tok >> 1) & 3) * 16;
+}
+__host__ __device__ __forceinline__ int q4_v_meta(int tok) {  // the pair's 4 x 2 scales (or, at kQ4VOffsets, offsets)
+  return (tok >> 3) * 64 + ((tok >> 1) & 3) * 16;
+}
+
+// ---------------------------------------------------------------- rows read back
+struct GatherArgs {
+  void* k_out;
+  void* v_out;
+  int layer;
+  int n;          // tokens per row: slots sb.len[z] .. sb.len[z] + n - 1
+  int pages;      // pages a row's range can touch
+  int paged;      // 1: out as pool pages [page][n_kv][16][128] from slot 0, zeros at and past slot n
+  int* status;
+};
+
+template <bool BF16>
+__device__ __forceinline__ void store4(void* p, size_t i, const float* x) {
+  if (BF16) {
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+  } else {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = make_float4(x[0], x[1], x[2], x[3]);
+  }
+}
+
+// LayerKVCache::get (oomllama_turbo.rs:57-63) on the device: the cached rows as
+// values.  One CTA of 128 threads per (row, page, kv head): 64 threads read the
+// K chunk, 64 the V chunk; a thread's 128-bit load is 32 codes (4-bit cache).
+// Bound by bytes: a 4-bit page is 2.5 KB read for 8 KB (bf16) written.
+template <int KV, bool OUT_BF16>
+__global__ void __launch_bounds__(128)
+    kv_gather_kernel(const GatherArgs a, const KVPool pool, const __grid_constant__ SeqBatch sb) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int g = blockIdx.x % pool.n_kv;
+  const int rest = blockIdx.x / pool.n_kv;
+  const int z = rest / a.pages;
+  const int first = sb.len[z], last = first + a.n;  // slots wanted
+  const int lp = first / kPageSize + (rest - z * a.pages);
+  const int s0 = lp * kPageSize;
+  if (!a.paged && s0 >= last) return;
+  const bool held = s0 < last;
+  int page = pool.n_pool_pages - 1;
+  if (held) {
+    const int id = lp < pool.max_pages_per_seq ? __ldg(pool.block_table + (size_t)sb.seq[z] * pool.max_pages_per_seq + lp) : -1;
+    if ((unsigned)id < (unsigned)pool.n_pool_pages)
+      page = id;
+    else if (threadIdx.x == 0)
+      report_error(a.status, kDevErrBounds);
+  }
+  const int u = threadIdx.x & 63;
+  const bool is_v = threadIdx.x >= 64;
+  void* out = is_v ? a.v_out : a.k_out;
+  // element offset of (slot, dim) in the output
+  auto at = [&](int slot, int d) -> size_t {
+    return a.paged ? (((size_t)lp * pool.n_kv + g) * kPageSize + (slot - s0)) * kHeadDim + d
+                   : (((size_t)z * a.n + (slot - first)) * pool.n_kv + g) * kHeadDim + d;
+  };
+  auto wanted = [&](int slot) { return slot >= first && slot < last; };
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+  if (KV == kKvQ4) {
+    const uint8_t* c = static_cast<const uint8_t*>(is_v ? pool.v : pool.k) + q4_chunk_off(pool, a.layer, page, g);
+    const uint4 w4 = *reinterpret_cast<const uint4*>(c + u * 16);
+    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+    if (!is_v) {
+      const int tok = u >> 2, t = u & 3, slot = s0 + tok;
+      const uint4 m4 = *reinterpret_cast<const uint4*>(c + kQ4Meta + tok * 16);
+      const uint32_t m[4] = {m4.x, m4.y, m4.z, m4.w};  // o01 o23 s01 s23
+      if (!wanted(slot) && !a.paged) return;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float o = __half2float(__ushort_as_half((uint16_t)(m[q >> 1] >> (16 * (q & 1)))));
+        const float s = __half2float(__ushort_as_half((uint16_t)(m[2 + (q >> 1)] >> (16 * (q & 1)))));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = q4_value((w[q] >> (16 * e + 4 * i)) & 15u, s, o);
+          store4<OUT_BF16>(out, at(slot, 32 * q + 8 * t + 4 * e), wanted(slot) ? x : zero);
+        }
+      }
+    } else {
+      const int h = u >> 5, gg = (u >> 2) & 7, t = u & 3;
+      const uint4 s4 = *reinterpret_cast<const uint4*>(c + kQ4Meta + h * 64 + t * 16);
+      const uint4 o4 = *reinterpret_cast<const uint4*>(c + kQ4VOffsets + h * 64 + t * 16);
+      const uint32_t sw[4] = {s4.x, s4.y, s4.z, s4.w}, ow[4] = {o4.x, o4.y, o4.z, o4.w};
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int slot = s0 + 8 * h + 2 * t + p;
+        if (!wanted(slot) && !a.paged) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float o = __half2float(__ushort_as_half((uint16_t)(ow[q] >> (16 * p))));
+          const float s = __half2float(__ushort_as_half((uint16_t)(sw[q] >> (16 * p))));
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = q4_value((w[q] >> (16 * p + 4 * i)) & 15u, s, o);
+          store4<OUT_BF16>(out, at(slot, 32 * q + 4 * gg), wanted(slot) ? x : zero);
+        }
+      }
+    }
+  } else {
+    constexpr int es = KV == kKvBf16 ? 2 : 4;
+    const uint8_t* c = static_cast<const uint8_t*>(is_v ? pool.v : pool.k) +
+                       (((size_t)a.layer * pool.n_pool_pages + page) * pool.n_kv + g) * (size_t)(kPageSize * kHeadDim * es);
+    for (int i = u; i < kPageSize * kHeadDim / 4; i += 64) {
+      const int slot = s0 + i / (kHeadDim / 4), d = (i % (kHeadDim / 4)) * 4;
+      if (!wanted(slot)) continue;
+      float x[4];
+      if (KV == kKvBf16) {
+        const uint2 v = *reinterpret_cast<const uint2*>(c + (size_t)i * 8);
+        x[0] = bf16_lo_f32(v.x); x[1] = bf16_hi_f32(v.x); x[2] = bf16_lo_f32(v.y); x[3] = bf16_hi_f32(v.y);
+      } else {
+        const float4 v = *reinterpret_cast<const float4*>(c + (size_t)i * 16);
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+      }
+      store4<OUT_BF16>(out, at(slot, d), x);
+    }
+  }
+}
+
+}  // namespace oomattn

@@ -18,9 +18,12 @@
 #include "../../include/oomattn.h"
 #include "common.cuh"
 #include "decode.cuh"
+#include "decode_q4.cuh"
 #include "gemm.cuh"
+#include "kv4.cuh"
 #include "params.cuh"
 #include "prefill.cuh"
+#include "qk_norm.cuh"
 #include "q8_linear.cuh"
 #include "q8_tc.cuh"
 #include "rope_append.cuh"
@@ -29,7 +32,11 @@ using namespace oomattn;
 
 namespace {
 
-int split_cap(int kv_dtype) { return kv_dtype == OOMATTN_DTYPE_BF16 ? kMaxSplitsBf16 : kMaxSplits; }
+static_assert((int)kKvF32 == OOMATTN_DTYPE_F32 && (int)kKvBf16 == OOMATTN_DTYPE_BF16 && (int)kKvQ4 == OOMATTN_DTYPE_Q4, "cache types");
+
+int split_cap(int kv_dtype) { return kv_dtype == OOMATTN_DTYPE_F32 ? kMaxSplits : kMaxSplitsBf16; }
+// Resident decode CTAs per SM, and the fixed cost of one in pages (plan_decode), by cache type.
+int decode_slots(int kv_dtype) { return kv_dtype == OOMATTN_DTYPE_Q4 ? kQ4CtasPerSm : kDecCtasPerSm; }
 static_assert(kMaxGroup * kMaxSplits <= kDecWarps * kMaxGroup * kMergeStride,
               "the f32 decode merge stages [group][splits] lse values over the per-warp O area");
 constexpr unsigned long long kDefaultTimeoutNs = 2000000000ull;  // bounded device waits: 2 s
@@ -94,6 +101,13 @@ struct oomattn_ctx {
   // key-split prefill: the chunks' partial O and lse
   uint8_t* d_pf_part = nullptr;
   size_t pf_part_bytes = 0;
+  // prefill over a 4-bit cache: one sequence's rows of one layer as bf16 pages
+  // [exp_pages + 1][n_kv][16][128] of K, then of V (the last page zero), and the
+  // block table that names them in order
+  std::vector<void*> exp_blocks;
+  uint8_t* d_exp = nullptr;
+  int exp_pages = 0;
+  int* d_exp_table = nullptr;
   // Q8 linear: activation splits and split-K partials, and per-row-tile
   // arrival counters (zero between launches)
   uint8_t* d_q8_scratch = nullptr;
@@ -177,10 +191,10 @@ void build_rope_table(float theta, int n_pos, std::vector<float>& c, std::vector
   }
 }
 
-int encode_pool_map(oomattn_ctx* ctx, void* base, CUtensorMap* map) {
+int encode_pool_map(oomattn_ctx* ctx, void* base, uint64_t n_pages, CUtensorMap* map) {
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) return fail(ctx, OOMATTN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  const uint64_t rows = (uint64_t)ctx->cfg.n_layers * ctx->n_pool_pages * ctx->cfg.n_kv_heads * kPageSize;
+  const uint64_t rows = n_pages * ctx->cfg.n_kv_heads * kPageSize;
   cuuint64_t dims[2] = {(cuuint64_t)kHeadDim, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)kHeadDim * 2};
   cuuint32_t box[2] = {64, (cuuint32_t)kPageSize};
@@ -429,7 +443,9 @@ int f32_gemv(oomattn_ctx* ctx, const float* x, const float* w, int T, int n, int
 }
 
 // Fills the SeqBatch of an append over rows [r0, r0+n) and advances the host lengths.
-int plan_append(oomattn_ctx* ctx, int layer, int n, const int32_t* seq_ids, int n_new, SeqBatch& sb) {
+// starts (null: each sequence's length): the slot of each sequence's first new token, at most its length.
+int plan_append(oomattn_ctx* ctx, int layer, int n, const int32_t* seq_ids, int n_new, SeqBatch& sb,
+                const int32_t* starts = nullptr) {
   sb.n = n;
   for (int z = 0; z < n; ++z) {
     const int seq = seq_ids[z];
@@ -437,11 +453,14 @@ int plan_append(oomattn_ctx* ctx, int layer, int n, const int32_t* seq_ids, int 
     if (rc) return rc;
     for (int w = 0; w < z; ++w)
       if (sb.seq[w] == seq) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "sequence %d appears twice in one append", seq);
-    const int len = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq];
+    const int cur = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq];
+    const int len = starts ? starts[z] : cur;
+    if (len < 0 || len > cur)
+      return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "sequence %d: start %d outside [0, %d]", seq, len, cur);
+    if ((long long)ctx->h_pos_off[seq] + len + n_new > ctx->cfg.max_seq_len)
+      return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "sequence %d: positions up to %lld exceed max_seq_len %d", seq,
+                  (long long)ctx->h_pos_off[seq] + len + n_new - 1, ctx->cfg.max_seq_len);
     const int pos = ctx->h_pos_off[seq] + len;
-    if (pos + n_new > ctx->cfg.max_seq_len)
-      return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "sequence %d: positions up to %d exceed max_seq_len %d", seq,
-                  pos + n_new - 1, ctx->cfg.max_seq_len);
     rc = check_slots(ctx, seq, len, len + n_new);
     if (rc) return rc;
     sb.seq[z] = seq;
@@ -452,7 +471,7 @@ int plan_append(oomattn_ctx* ctx, int layer, int n, const int32_t* seq_ids, int 
 }
 
 void commit_append(oomattn_ctx* ctx, int layer, const SeqBatch& sb, int n_new) {
-  for (int z = 0; z < sb.n; ++z) ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + sb.seq[z]] += n_new;
+  for (int z = 0; z < sb.n; ++z) ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + sb.seq[z]] = sb.len[z] + n_new;
 }
 
 AppendArgs base_append_args(oomattn_ctx* ctx, int layer, int n_new) {
@@ -522,6 +541,127 @@ int launch_rope_append(oomattn_ctx* ctx, const AppendArgs& ap, const SeqBatch& s
   return OOMATTN_OK;
 }
 
+// The append with a norm of the q and k heads and / or into a 4-bit cache: one
+// warp per four heads of a token (qk_norm.cuh).
+int launch_qk_norm_append(oomattn_ctx* ctx, const AppendArgs& ap, const NormArgs& na, const SeqBatch& sb, int T) {
+  const void* ptrs[] = {ap.q, ap.k, ap.v, ap.q_out, ap.bq, ap.bk, ap.bv, na.qw, na.kw};
+  for (const void* p : ptrs)
+    if (p && !aligned16(p))
+      return fail(ctx, OOMATTN_ERR_INVALID_ARG, "tensors, biases and norm weights must be 16-byte aligned");
+  const int hq = ctx->cfg.n_heads, hkv = ctx->cfg.n_kv_heads, kv = ctx->cfg.kv_dtype;
+  const long long qw = ap.q ? (hq + 3) / 4 : 0, kw = ap.k ? (hkv + 3) / 4 : 0;
+  const long long v_units = kv == OOMATTN_DTYPE_Q4 ? (long long)sb.n * (ap.n_new / 2 + 1) : T;
+  const long long tasks = T * (qw + kw) + v_units * kw;
+  if (tasks >= (1ll << 26)) return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "%d tokens in one append call", T);
+  const int grid = (int)std::max<long long>(1, std::min<long long>((tasks + 7) / 8, (long long)ctx->num_sms * kQkNormCtasPerSm));
+  const KVPool pool = make_pool(ctx);
+  cudaError_t le = cudaSuccess;
+#define OOMATTN_QN(I, Q, K) \
+  le = launch_pdl(qk_norm_append_kernel<I, Q, K>, dim3(grid), dim3(256), 0, ctx->stream, ap, na, pool, sb, T)
+#define OOMATTN_QN_IO(K)                                                   \
+  do {                                                                     \
+    if (ap.in_bf16 && ap.q_out_bf16) OOMATTN_QN(true, true, K);            \
+    else if (ap.in_bf16) OOMATTN_QN(true, false, K);                       \
+    else if (ap.q_out_bf16) OOMATTN_QN(false, true, K);                    \
+    else OOMATTN_QN(false, false, K);                                      \
+  } while (0)
+  if (kv == OOMATTN_DTYPE_Q4) OOMATTN_QN_IO(kKvQ4);
+  else if (kv == OOMATTN_DTYPE_BF16) OOMATTN_QN_IO(kKvBf16);
+  else OOMATTN_QN_IO(kKvF32);
+#undef OOMATTN_QN_IO
+#undef OOMATTN_QN
+  if (le != cudaSuccess) return fail(ctx, OOMATTN_ERR_CUDA, "append launch: %s", cudaGetErrorString(le));
+  return OOMATTN_OK;
+}
+
+// Rows of an append (or of q alone) by the kernel that their cache and norm need.
+int launch_append(oomattn_ctx* ctx, const AppendArgs& ap, const oomattn_qk_norm* norm, const SeqBatch& sb, int T) {
+  const NormArgs na{norm ? norm->q : nullptr, norm ? norm->k : nullptr, norm ? norm->eps : 0.f};
+  if (na.qw || na.kw || (ap.k && ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4))
+    return launch_qk_norm_append(ctx, ap, na, sb, T);
+  return launch_rope_append(ctx, ap, sb, T);
+}
+
+int check_norm(oomattn_ctx* ctx, const oomattn_qk_norm* norm) {
+  if (norm && !(norm->eps >= 0.f && norm->eps <= 3.4e38f))
+    return fail(ctx, OOMATTN_ERR_INVALID_ARG, "the norm's eps must be a finite number >= 0");
+  return OOMATTN_OK;
+}
+
+int rope_append_impl(oomattn_ctx* ctx, int layer, int n_seqs, const int32_t* seq_ids, const int32_t* starts,
+                     int n_new, const void* q, const void* k, const void* v, int in_dtype, const float* bq,
+                     const float* bk, const float* bv, const oomattn_qk_norm* norm, void* q_out, int q_out_dtype) {
+  if (!ctx) return OOMATTN_ERR_INVALID_ARG;
+  if (!seq_ids || !q || !k || !v || !q_out || n_seqs <= 0 || n_new <= 0)
+    return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad rope_append arguments");
+  int rc = check_layer(ctx, layer);
+  if (!rc) rc = validate_dtype(ctx, in_dtype, "rope_append input");
+  if (!rc) rc = validate_dtype(ctx, q_out_dtype, "rope_append q_out");
+  if (!rc) rc = check_norm(ctx, norm);
+  if (rc) return rc;
+  DeviceGuard dg(ctx->device);
+  const int in_es = in_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4, out_es = q_out_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4;
+  for (int r0 = 0; r0 < n_seqs; r0 += kMaxBatch) {
+    const int n = std::min(kMaxBatch, n_seqs - r0);
+    SeqBatch sb;
+    rc = plan_append(ctx, layer, n, seq_ids + r0, n_new, sb, starts ? starts + r0 : nullptr);
+    if (rc) return rc;
+    const size_t t0 = (size_t)r0 * n_new;
+    AppendArgs ap = base_append_args(ctx, layer, n_new);
+    ap.q = (const uint8_t*)q + t0 * ctx->cfg.n_heads * kHeadDim * in_es;
+    ap.k = (const uint8_t*)k + t0 * ctx->cfg.n_kv_heads * kHeadDim * in_es;
+    ap.v = (const uint8_t*)v + t0 * ctx->cfg.n_kv_heads * kHeadDim * in_es;
+    ap.in_bf16 = in_dtype == OOMATTN_DTYPE_BF16;
+    ap.q_out = (uint8_t*)q_out + t0 * ctx->cfg.n_heads * kHeadDim * out_es;
+    ap.q_out_bf16 = q_out_dtype == OOMATTN_DTYPE_BF16;
+    ap.bq = bq;
+    ap.bk = bk;
+    ap.bv = bv;
+    rc = launch_append(ctx, ap, norm, sb, n * n_new);
+    if (rc) return rc;
+    CKLAUNCH();
+    commit_append(ctx, layer, sb, n_new);
+  }
+  return OOMATTN_OK;
+}
+
+int rope_q_impl(oomattn_ctx* ctx, int n_rows, const int32_t* positions, const void* q, int in_dtype, const float* bq,
+                const oomattn_qk_norm* norm, void* q_out, int q_out_dtype) {
+  if (!ctx) return OOMATTN_ERR_INVALID_ARG;
+  if (!positions || !q || !q_out || n_rows <= 0) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad rope_q arguments");
+  int rc = validate_dtype(ctx, in_dtype, "rope_q input");
+  if (!rc) rc = validate_dtype(ctx, q_out_dtype, "rope_q q_out");
+  if (!rc) rc = check_norm(ctx, norm);
+  if (rc) return rc;
+  DeviceGuard dg(ctx->device);
+  const int in_es = in_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4, out_es = q_out_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4;
+  for (int r0 = 0; r0 < n_rows; r0 += kMaxBatch) {
+    const int n = std::min(kMaxBatch, n_rows - r0);
+    SeqBatch sb;
+    sb.n = n;
+    for (int z = 0; z < n; ++z) {
+      const int pos = positions[r0 + z];
+      if (pos < 0 || pos >= ctx->cfg.max_seq_len)
+        return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "row %d: position %d outside [0, %d)", r0 + z, pos,
+                    ctx->cfg.max_seq_len);
+      sb.seq[z] = 0;
+      sb.len[z] = 0;
+      sb.pos[z] = pos;
+    }
+    AppendArgs ap = base_append_args(ctx, 0, 1);
+    ap.q = (const uint8_t*)q + (size_t)r0 * ctx->cfg.n_heads * kHeadDim * in_es;
+    ap.k = nullptr;  // q rows only: nothing is appended
+    ap.v = nullptr;
+    ap.in_bf16 = in_dtype == OOMATTN_DTYPE_BF16;
+    ap.q_out = (uint8_t*)q_out + (size_t)r0 * ctx->cfg.n_heads * kHeadDim * out_es;
+    ap.q_out_bf16 = q_out_dtype == OOMATTN_DTYPE_BF16;
+    ap.bq = bq;
+    rc = launch_append(ctx, ap, norm, sb, n);
+    if (rc) return rc;
+  }
+  return OOMATTN_OK;
+}
+
 // Split-KV decode schedule.  Row z's pages are split into ns_z = ceil(pages_z
 // / t) near-equal ranges (at most max_splits) for each kv head, and the rows
 // are ordered by range size, longest first, so that the block scheduler's
@@ -532,6 +672,11 @@ int launch_rope_append(oomattn_ctx* ctx, const AppendArgs& ap, const SeqBatch& s
 // (pipeline fill and merge).  Returns the number of items (the grid size).
 constexpr int kDecodeFillPages = 12;     // bf16 cache
 constexpr int kDecodeFillPagesF32 = 12;  // f32 cache (measured insensitive: 4 to 200 chose the same plans on C1)
+constexpr int kDecodeFillPagesQ4 = 12;   // 4-bit cache
+int decode_fill(int kv_dtype) {
+  return kv_dtype == OOMATTN_DTYPE_BF16 ? kDecodeFillPages
+                                        : (kv_dtype == OOMATTN_DTYPE_F32 ? kDecodeFillPagesF32 : kDecodeFillPagesQ4);
+}
 constexpr int kDecodeMaxSimSlots = 2048;
 
 long long lpt_makespan(const int* size, const int* count, int groups, int slots, int fill, long long* heap) {
@@ -629,16 +774,17 @@ int plan_decode(const SeqBatch& sb, int n_kv, int slots, int max_splits, int fil
   return items;
 }
 
+// io16: q and out are bf16 (4-bit cache only).
 int launch_decode_rows(oomattn_ctx* ctx, int layer, const SeqBatch& sb, const float* q, float* out, float* lse,
-                       int o_stride, int lse_stride) {
+                       int o_stride, int lse_stride, bool io16 = false) {
   const int n_kv = ctx->cfg.n_kv_heads;
-  const int slots = ctx->num_sms * (ctx->cfg.kv_dtype == OOMATTN_DTYPE_BF16 ? kDecCtasPerSm : 3);
+  const int slots = ctx->num_sms * decode_slots(ctx->cfg.kv_dtype);
   int key[kMaxBatch + 1];
   key[0] = sb.n;
   for (int z = 0; z < sb.n; ++z) key[z + 1] = sb.len[z] > 0 ? (sb.len[z] + kPageSize - 1) / kPageSize : 0;
   if (ctx->sched_key.size() != (size_t)sb.n + 1 || !std::equal(key, key + sb.n + 1, ctx->sched_key.begin())) {
     ctx->sched_items = plan_decode(sb, n_kv, slots, split_cap(ctx->cfg.kv_dtype),
-                                   ctx->cfg.kv_dtype == OOMATTN_DTYPE_BF16 ? kDecodeFillPages : kDecodeFillPagesF32,
+                                   decode_fill(ctx->cfg.kv_dtype),
                                    ctx->sched);
     ctx->sched_key.assign(key, key + sb.n + 1);
   }
@@ -677,6 +823,10 @@ int launch_decode_rows(oomattn_ctx* ctx, int layer, const SeqBatch& sb, const fl
     cfg.blockDim = dim3((kDecWarps + 1) * 32);
     cfg.dynamicSmemBytes = kDecSmemBytes;
     le = cudaLaunchKernelEx(&cfg, decode_bf16_kernel, ctx->kmap, ctx->vmap, pool, a, sb, sched);
+  } else if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4) {
+    cfg.blockDim = dim3(kDecWarps * 32);
+    cfg.dynamicSmemBytes = kQ4SmemBytes;
+    le = cudaLaunchKernelEx(&cfg, io16 ? decode_q4_kernel<true> : decode_q4_kernel<false>, pool, a, sb, sched);
   } else {
     cfg.blockDim = dim3(kDecWarps * 32);
     le = cudaLaunchKernelEx(&cfg, decode_f32_kernel, pool, a, sb, sched);
@@ -692,7 +842,7 @@ namespace {
 // Decode rows in launches of at most kMaxBatch rows; (row, head) outputs at
 // out + (row * n_heads + head) * o_stride and lse + (row * n_heads + head) * lse_stride.
 int decode_rows_impl(oomattn_ctx* ctx, int layer, int n_rows, const int32_t* seq_ids, const int32_t* lens,
-                     const float* q, float* out, float* lse, int o_stride, int lse_stride) {
+                     const float* q, float* out, float* lse, int o_stride, int lse_stride, bool io16 = false) {
   int rc = check_layer(ctx, layer);
   if (rc) return rc;
   DeviceGuard dg(ctx->device);
@@ -713,8 +863,10 @@ int decode_rows_impl(oomattn_ctx* ctx, int layer, int n_rows, const int32_t* seq
       sb.len[z] = len;
       sb.pos[z] = 0;
     }
-    rc = launch_decode_rows(ctx, layer, sb, q + (size_t)r0 * hq * kHeadDim, out + (size_t)r0 * hq * o_stride,
-                            lse ? lse + (size_t)r0 * hq * lse_stride : nullptr, o_stride, lse_stride);
+    const size_t es = io16 ? 2 : 4;  // bytes of a q and an out element
+    rc = launch_decode_rows(ctx, layer, sb, (const float*)((const uint8_t*)q + (size_t)r0 * hq * kHeadDim * es),
+                            (float*)((uint8_t*)out + (size_t)r0 * hq * o_stride * es),
+                            lse ? lse + (size_t)r0 * hq * lse_stride : nullptr, o_stride, lse_stride, io16);
     if (rc) return rc;
   }
   return OOMATTN_OK;
@@ -735,6 +887,122 @@ cudaError_t launch_gemv(const GemvArgs& ga, const KVPool& pool, const SeqBatch& 
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, qkv_gemv_rope_append_kernel<T, WBF16>, ga, pool, sb);
 }
+
+int launch_gather(oomattn_ctx* ctx, const GatherArgs& a, const SeqBatch& sb, int out_dtype) {
+  const long long grid = (long long)sb.n * a.pages * ctx->cfg.n_kv_heads;
+  if (grid >= (1ll << 31)) return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "%d tokens in one gather", a.n);
+  const KVPool pool = make_pool(ctx);
+  const bool b = out_dtype == OOMATTN_DTYPE_BF16;
+  cudaError_t le;
+#define OOMATTN_KG(K)                                                                                      \
+  (b ? launch_pdl(kv_gather_kernel<K, true>, dim3((unsigned)grid), dim3(128), 0, ctx->stream, a, pool, sb) \
+     : launch_pdl(kv_gather_kernel<K, false>, dim3((unsigned)grid), dim3(128), 0, ctx->stream, a, pool, sb))
+  switch (ctx->cfg.kv_dtype) {
+    case OOMATTN_DTYPE_Q4: le = OOMATTN_KG(kKvQ4); break;
+    case OOMATTN_DTYPE_BF16: le = OOMATTN_KG(kKvBf16); break;
+    default: le = OOMATTN_KG(kKvF32); break;
+  }
+#undef OOMATTN_KG
+  if (le != cudaSuccess) return fail(ctx, OOMATTN_ERR_CUDA, "gather launch: %s", cudaGetErrorString(le));
+  return OOMATTN_OK;
+}
+
+// The q, k and v rows of an append are projected by themselves, not inside the fused GEMV (whose CTAs own
+// parts of a head), where its epilogue needs whole heads: their norm, or the 32-value groups of a 4-bit cache.
+bool rows_apart(const oomattn_ctx* ctx, const oomattn_qk_norm* norm) {
+  return ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4 || (norm && (norm->q || norm->k));
+}
+
+// x [T][k] times each job's weights: GEMVs up to 16 tokens with f32 weights, else the tensor-core linear.
+int project(oomattn_ctx* ctx, const float* x, int T, int k, const KfJob* jobs, int n_jobs) {
+  if (T > kGemvMaxT || jobs[0].w_bf16) return kf_linear_f32(ctx, x, T, k, jobs, n_jobs);
+  for (int j = 0; j < n_jobs; ++j) {
+    const int rc = f32_gemv(ctx, x, static_cast<const float*>(jobs[j].w), T, jobs[j].n, k, jobs[j].bias,
+                            jobs[j].residual, jobs[j].out);
+    if (rc) return rc;
+  }
+  return OOMATTN_OK;
+}
+
+// Prefill over a 4-bit cache, many tokens: the sequence's rows of one layer as
+// bf16 pages, in order, which the tensor-core prefill then reads as its pool.
+// It reads 160 and writes 512 bytes per token and kv head once, for the 4 * 128
+// * group * n_new products that each of those tokens takes part in.
+int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtensorMap* kmap, CUtensorMap* vmap) {
+  const int n_kv = ctx->cfg.n_kv_heads;
+  const int pages = ((L + kPageSize - 1) / kPageSize + 7) / 8 * 8;  // the prefill's 128-key tiles: zeros past L
+  const size_t page_bytes = (size_t)n_kv * kPageSize * kHeadDim * 2;
+  if (pages > ctx->exp_pages) {
+    const int cap = pages + pages / 2;  // a growing sequence does not reallocate at every chunk
+    if ((long long)(cap + 1) * n_kv * kPageSize >= (1ll << 31))
+      return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "prefill over %d tokens of a 4-bit cache", L);
+    cudaStreamCaptureStatus cap_st = cudaStreamCaptureStatusNone;
+    CK(cudaStreamIsCapturing(ctx->stream, &cap_st));
+    if (cap_st != cudaStreamCaptureStatusNone)
+      return fail(ctx, OOMATTN_ERR_UNSUPPORTED,
+                  "the prefill's scratch has to grow: run a prefill of this length once before the capture");
+    // K pages, V pages, table.  An earlier, smaller block stays until the context
+    // is destroyed: a captured graph may still name it.
+    const size_t half_bytes = (size_t)(cap + 1) * page_bytes, bytes = 2 * half_bytes + (size_t)cap * sizeof(int);
+    void* p = nullptr;
+    if (cudaMalloc(&p, bytes) != cudaSuccess) {
+      cudaGetLastError();
+      return fail(ctx, OOMATTN_ERR_NO_MEMORY, "prefill scratch of %zu bytes failed", bytes);
+    }
+    ctx->exp_blocks.push_back(p);
+    uint8_t* b = static_cast<uint8_t*>(p);
+    std::vector<int> table(cap);
+    for (int i = 0; i < cap; ++i) table[i] = i;
+    CK(cudaMemsetAsync(b + half_bytes - page_bytes, 0, page_bytes, ctx->stream));  // the null pages
+    CK(cudaMemsetAsync(b + 2 * half_bytes - page_bytes, 0, page_bytes, ctx->stream));
+    CK(cudaMemcpyAsync(b + 2 * half_bytes, table.data(), (size_t)cap * sizeof(int), cudaMemcpyHostToDevice, ctx->stream));
+    CK(cudaStreamSynchronize(ctx->stream));  // the host table ends here
+    ctx->d_exp = b;
+    ctx->d_exp_table = reinterpret_cast<int*>(b + 2 * half_bytes);
+    ctx->exp_pages = cap;
+  }
+  const size_t half = (size_t)(ctx->exp_pages + 1) * page_bytes;
+  SeqBatch sb;
+  sb.n = 1;
+  sb.seq[0] = seq;
+  sb.len[0] = 0;
+  sb.pos[0] = 0;
+  GatherArgs a;
+  a.k_out = ctx->d_exp;
+  a.v_out = ctx->d_exp + half;
+  a.layer = layer;
+  a.n = L;
+  a.pages = pages;
+  a.paged = 1;
+  a.status = ctx->d_status;
+  int rc = launch_gather(ctx, a, sb, OOMATTN_DTYPE_BF16);
+  if (!rc) rc = encode_pool_map(ctx, ctx->d_exp, (uint64_t)ctx->exp_pages + 1, kmap);
+  if (!rc) rc = encode_pool_map(ctx, ctx->d_exp + half, (uint64_t)ctx->exp_pages + 1, vmap);
+  pool->k = ctx->d_exp;
+  pool->v = ctx->d_exp + half;
+  pool->block_table = ctx->d_exp_table;
+  pool->max_pages_per_seq = pages;
+  pool->n_pool_pages = ctx->exp_pages + 1;
+  pool->kv_bf16 = 1;
+  return rc;
+}
+
+// Prefill over a 4-bit cache, few tokens (drafts to verify, a short tail of a
+// prompt): each as one decode row that sees the slots up to its own.
+constexpr int kQ4PrefillRows = 16;
+int q4_prefill_rows(oomattn_ctx* ctx, int layer, int seq, int n_new, const void* q, void* out, float* lse) {
+  if (!q || !out) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad prefill arguments");
+  int rc = check_layer(ctx, layer);
+  if (!rc) rc = check_seq(ctx, seq);
+  if (rc) return rc;
+  if (!aligned16(q) || !aligned16(out)) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
+  const int L = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq];
+  if (n_new > L) return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "n_new %d exceeds the cached length %d", n_new, L);
+  std::vector<int32_t> rows(n_new, seq), lens(n_new);
+  for (int i = 0; i < n_new; ++i) lens[i] = L - n_new + i + 1;
+  return decode_rows_impl(ctx, layer, n_new, rows.data(), lens.data(), static_cast<const float*>(q),
+                          static_cast<float*>(out), lse, kHeadDim, 1, true);
+}
 }  // namespace
 
 extern "C" {
@@ -750,7 +1018,7 @@ int oomattn_create(const oomattn_config* cfg, int device, void* stream, oomattn_
   if (c.head_dim != kHeadDim || c.page_size != kPageSize || c.n_heads <= 0 || c.n_kv_heads <= 0 ||
       c.n_heads % c.n_kv_heads != 0 || c.n_heads / c.n_kv_heads > kMaxGroup || c.n_layers <= 0 ||
       c.max_seq_len <= 0 || c.max_seqs <= 0 || c.n_pages <= 0 || c.hidden_size < 0 || !(c.rope_theta > 0.f) ||
-      (c.kv_dtype != OOMATTN_DTYPE_F32 && c.kv_dtype != OOMATTN_DTYPE_BF16) ||
+      (c.kv_dtype != OOMATTN_DTYPE_F32 && c.kv_dtype != OOMATTN_DTYPE_BF16 && c.kv_dtype != OOMATTN_DTYPE_Q4) ||
       (c.rope_variant != OOMATTN_ROPE_SPLIT_HALF && c.rope_variant != OOMATTN_ROPE_INTERLEAVED))
     return OOMATTN_ERR_BAD_CONFIG;
   const long long rows = (long long)c.n_layers * (c.n_pages + 1) * c.n_kv_heads * kPageSize;
@@ -763,7 +1031,7 @@ int oomattn_create(const oomattn_config* cfg, int device, void* stream, oomattn_
   ctx->group = c.n_heads / c.n_kv_heads;
   ctx->max_pages_per_seq = (c.max_seq_len + kPageSize - 1) / kPageSize;
   ctx->n_pool_pages = c.n_pages + 1;
-  ctx->esize = c.kv_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4;
+  ctx->esize = c.kv_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4;  // f32 and bf16 caches only
   ctx->scale = c.softmax_scale > 0.f ? c.softmax_scale : 1.0f / sqrtf((float)kHeadDim);
   DeviceGuard dg(device);
   auto bail = [&](int code) {
@@ -772,7 +1040,8 @@ int oomattn_create(const oomattn_config* cfg, int device, void* stream, oomattn_
   };
   if (cudaSetDevice(device) != cudaSuccess) return bail(OOMATTN_ERR_CUDA);
   cudaDeviceGetAttribute(&ctx->num_sms, cudaDevAttrMultiProcessorCount, device);
-  const size_t pool_bytes = (size_t)rows * kHeadDim * ctx->esize;
+  const size_t pool_bytes = c.kv_dtype == OOMATTN_DTYPE_Q4 ? (size_t)(rows / kPageSize) * kQ4Chunk
+                                                           : (size_t)rows * kHeadDim * ctx->esize;
   if (cudaMalloc(&ctx->kpool, pool_bytes) != cudaSuccess || cudaMalloc(&ctx->vpool, pool_bytes) != cudaSuccess)
     return bail(OOMATTN_ERR_NO_MEMORY);
   if (cudaMemset(ctx->kpool, 0, pool_bytes) != cudaSuccess || cudaMemset(ctx->vpool, 0, pool_bytes) != cudaSuccess)
@@ -802,11 +1071,16 @@ int oomattn_create(const oomattn_config* cfg, int device, void* stream, oomattn_
       cudaMemset(ctx->d_status, 0, sizeof(int)) != cudaSuccess)
     return bail(OOMATTN_ERR_CUDA);
   if (c.kv_dtype == OOMATTN_DTYPE_BF16) {
-    if (encode_pool_map(ctx, ctx->kpool, &ctx->kmap) || encode_pool_map(ctx, ctx->vpool, &ctx->vmap))
+    const uint64_t pages = (uint64_t)c.n_layers * ctx->n_pool_pages;
+    if (encode_pool_map(ctx, ctx->kpool, pages, &ctx->kmap) || encode_pool_map(ctx, ctx->vpool, pages, &ctx->vmap))
       return bail(OOMATTN_ERR_CUDA);
     ctx->have_maps = true;
   }
   if (cudaFuncSetAttribute(decode_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmemBytes) !=
+          cudaSuccess ||
+      cudaFuncSetAttribute(decode_q4_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4SmemBytes) !=
+          cudaSuccess ||
+      cudaFuncSetAttribute(decode_q4_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4SmemBytes) !=
           cudaSuccess ||
       cudaFuncSetAttribute(prefill_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPfSmemBytes) !=
           cudaSuccess ||
@@ -846,6 +1120,7 @@ int oomattn_destroy(oomattn_ctx* ctx) {
                   ctx->d_argmax_part, ctx->d_kf, ctx->d_pf_part};
   for (void* p : ptrs)
     if (p) cudaFree(p);
+  for (void* p : ctx->exp_blocks) cudaFree(p);
   delete ctx;
   return OOMATTN_OK;
 }
@@ -955,7 +1230,7 @@ int oomattn_kv_write(oomattn_ctx* ctx, int32_t layer, int32_t seq, const void* k
   ap.in_bf16 = src_dtype == OOMATTN_DTYPE_BF16;
   ap.rope_k = 0;  // K is stored as given: no rotation
   DeviceGuard dg(ctx->device);
-  rc = launch_rope_append(ctx, ap, sb, n);
+  rc = launch_append(ctx, ap, nullptr, sb, n);
   if (rc) return rc;
   CKLAUNCH();
   commit_append(ctx, layer, sb, n);
@@ -971,6 +1246,43 @@ int oomattn_kv_read(oomattn_ctx* ctx, int32_t layer, int32_t seq, void* k_out, v
   CK(cudaStreamSynchronize(ctx->stream));
   const int L = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq];
   const int n_kv = ctx->cfg.n_kv_heads;
+  if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4) {
+    std::vector<uint8_t> chunk(kQ4Chunk);
+    auto half_at = [&](int off) {
+      __half h;
+      memcpy(&h, chunk.data() + off, 2);
+      return __half2float(h);
+    };
+    for (int lp = 0; lp * kPageSize < L; ++lp) {
+      const int pg = ctx->h_block_table[(size_t)seq * ctx->max_pages_per_seq + lp];
+      const int nt = std::min(kPageSize, L - lp * kPageSize);
+      for (int g = 0; g < n_kv; ++g)
+        for (int which = 0; which < 2; ++which) {
+          const size_t off = (((size_t)layer * ctx->n_pool_pages + pg) * n_kv + g) * kQ4Chunk;
+          CK(cudaMemcpy(chunk.data(), (const uint8_t*)(which ? ctx->vpool : ctx->kpool) + off, kQ4Chunk,
+                        cudaMemcpyDeviceToHost));
+          float* dst = (float*)(which ? v_out : k_out) + ((size_t)g * L + (size_t)lp * kPageSize) * kHeadDim;
+          for (int r = 0; r < nt; ++r)
+            for (int d = 0; d < kHeadDim; ++d) {
+              const int w = d >> 5;
+              int code;
+              float s, o;
+              if (which == 0) {
+                code = chunk[q4_k_word(r, d >> 3) + ((d & 7) >> 1)] >> (4 * (d & 1)) & 15;
+                o = half_at(kQ4Meta + r * 16 + 2 * w);
+                s = half_at(kQ4Meta + r * 16 + 8 + 2 * w);
+              } else {
+                code = chunk[q4_v_pair(r, (d & 31) >> 2) + 4 * w + 2 * (r & 1) + ((d & 3) >> 1)] >> (4 * (d & 1)) & 15;
+                s = half_at(kQ4Meta + q4_v_meta(r) + 4 * w + 2 * (r & 1));
+                o = half_at(kQ4VOffsets + q4_v_meta(r) + 4 * w + 2 * (r & 1));
+              }
+              const volatile float cs = (float)(code - 8) * s;  // rounded by itself, as on the device
+              dst[(size_t)r * kHeadDim + d] = o + cs;
+            }
+        }
+    }
+    return OOMATTN_OK;
+  }
   const size_t es = ctx->esize;
   std::vector<uint8_t> page(kPageSize * kHeadDim * es);
   for (int lp = 0; lp * kPageSize < L; ++lp) {
@@ -985,6 +1297,49 @@ int oomattn_kv_read(oomattn_ctx* ctx, int32_t layer, int32_t seq, void* k_out, v
         memcpy(dst, page.data(), (size_t)nt * kHeadDim * es);
       }
     }
+  }
+  return OOMATTN_OK;
+}
+
+int oomattn_kv_gather(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const int32_t* starts,
+                      int32_t n, int32_t out_dtype, void* k_out, void* v_out) {
+  if (!ctx) return OOMATTN_ERR_INVALID_ARG;
+  if (!seq_ids || n_seqs <= 0 || n < 0 || (n > 0 && (!k_out || !v_out)))
+    return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad kv_gather arguments");
+  int rc = check_layer(ctx, layer);
+  if (!rc) rc = validate_dtype(ctx, out_dtype, "kv_gather");
+  if (rc) return rc;
+  if (!aligned16(k_out) || !aligned16(v_out))
+    return fail(ctx, OOMATTN_ERR_INVALID_ARG, "k_out and v_out must be 16-byte aligned");
+  for (int i = 0; i < n_seqs; ++i) {
+    rc = check_seq(ctx, seq_ids[i]);
+    if (rc) return rc;
+    const int cur = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq_ids[i]], from = starts ? starts[i] : 0;
+    if (from < 0 || (long long)from + n > cur)
+      return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "sequence %d: slots [%d, %lld) outside its %d cached tokens",
+                  seq_ids[i], from, (long long)from + n, cur);
+  }
+  if (n == 0) return OOMATTN_OK;
+  DeviceGuard dg(ctx->device);
+  const size_t row = (size_t)n * ctx->cfg.n_kv_heads * kHeadDim * (out_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4);
+  for (int r0 = 0; r0 < n_seqs; r0 += kMaxBatch) {
+    SeqBatch sb;
+    sb.n = std::min(kMaxBatch, n_seqs - r0);
+    for (int z = 0; z < sb.n; ++z) {
+      sb.seq[z] = seq_ids[r0 + z];
+      sb.len[z] = starts ? starts[r0 + z] : 0;
+      sb.pos[z] = 0;
+    }
+    GatherArgs a;
+    a.k_out = (uint8_t*)k_out + r0 * row;
+    a.v_out = (uint8_t*)v_out + r0 * row;
+    a.layer = layer;
+    a.n = n;
+    a.pages = (n + kPageSize - 2) / kPageSize + 1;  // the most that n slots can touch
+    a.paged = 0;
+    a.status = ctx->d_status;
+    rc = launch_gather(ctx, a, sb, out_dtype);
+    if (rc) return rc;
   }
   return OOMATTN_OK;
 }
@@ -1011,91 +1366,54 @@ int oomattn_compute_rope_table(float theta, int32_t head_dim, int32_t pos0, int3
 int oomattn_rope_append(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, int32_t n_new,
                         const void* q, const void* k, const void* v, int32_t in_dtype, const float* bq,
                         const float* bk, const float* bv, void* q_out, int32_t q_out_dtype) {
-  if (!ctx) return OOMATTN_ERR_INVALID_ARG;
-  if (!seq_ids || !q || !k || !v || !q_out || n_seqs <= 0 || n_new <= 0)
-    return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad rope_append arguments");
-  int rc = check_layer(ctx, layer);
-  if (!rc) rc = validate_dtype(ctx, in_dtype, "rope_append input");
-  if (!rc) rc = validate_dtype(ctx, q_out_dtype, "rope_append q_out");
-  if (rc) return rc;
-  DeviceGuard dg(ctx->device);
-  const int in_es = in_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4, out_es = q_out_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4;
-  for (int r0 = 0; r0 < n_seqs; r0 += kMaxBatch) {
-    const int n = std::min(kMaxBatch, n_seqs - r0);
-    SeqBatch sb;
-    rc = plan_append(ctx, layer, n, seq_ids + r0, n_new, sb);
-    if (rc) return rc;
-    const size_t t0 = (size_t)r0 * n_new;
-    AppendArgs ap = base_append_args(ctx, layer, n_new);
-    ap.q = (const uint8_t*)q + t0 * ctx->cfg.n_heads * kHeadDim * in_es;
-    ap.k = (const uint8_t*)k + t0 * ctx->cfg.n_kv_heads * kHeadDim * in_es;
-    ap.v = (const uint8_t*)v + t0 * ctx->cfg.n_kv_heads * kHeadDim * in_es;
-    ap.in_bf16 = in_dtype == OOMATTN_DTYPE_BF16;
-    ap.q_out = (uint8_t*)q_out + t0 * ctx->cfg.n_heads * kHeadDim * out_es;
-    ap.q_out_bf16 = q_out_dtype == OOMATTN_DTYPE_BF16;
-    ap.bq = bq;
-    ap.bk = bk;
-    ap.bv = bv;
-    rc = launch_rope_append(ctx, ap, sb, n * n_new);
-    if (rc) return rc;
-    CKLAUNCH();
-    commit_append(ctx, layer, sb, n_new);
-  }
-  return OOMATTN_OK;
+  return rope_append_impl(ctx, layer, n_seqs, seq_ids, nullptr, n_new, q, k, v, in_dtype, bq, bk, bv, nullptr, q_out,
+                          q_out_dtype);
+}
+
+int oomattn_rope_append_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids,
+                                const int32_t* starts, int32_t n_new, const void* q, const void* k, const void* v,
+                                int32_t in_dtype, const float* bq, const float* bk, const float* bv,
+                                const oomattn_qk_norm* norm, void* q_out, int32_t q_out_dtype) {
+  return rope_append_impl(ctx, layer, n_seqs, seq_ids, starts, n_new, q, k, v, in_dtype, bq, bk, bv, norm, q_out,
+                          q_out_dtype);
 }
 
 int oomattn_rope_q(oomattn_ctx* ctx, int32_t n_rows, const int32_t* positions, const void* q, int32_t in_dtype,
                    const float* bq, void* q_out, int32_t q_out_dtype) {
-  if (!ctx) return OOMATTN_ERR_INVALID_ARG;
-  if (!positions || !q || !q_out || n_rows <= 0) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad rope_q arguments");
-  int rc = validate_dtype(ctx, in_dtype, "rope_q input");
-  if (!rc) rc = validate_dtype(ctx, q_out_dtype, "rope_q q_out");
-  if (rc) return rc;
-  DeviceGuard dg(ctx->device);
-  const int in_es = in_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4, out_es = q_out_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4;
-  for (int r0 = 0; r0 < n_rows; r0 += kMaxBatch) {
-    const int n = std::min(kMaxBatch, n_rows - r0);
-    SeqBatch sb;
-    sb.n = n;
-    for (int z = 0; z < n; ++z) {
-      const int pos = positions[r0 + z];
-      if (pos < 0 || pos >= ctx->cfg.max_seq_len)
-        return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "row %d: position %d outside [0, %d)", r0 + z, pos,
-                    ctx->cfg.max_seq_len);
-      sb.seq[z] = 0;
-      sb.len[z] = 0;
-      sb.pos[z] = pos;
-    }
-    AppendArgs ap = base_append_args(ctx, 0, 1);
-    ap.q = (const uint8_t*)q + (size_t)r0 * ctx->cfg.n_heads * kHeadDim * in_es;
-    ap.k = nullptr;  // q rows only: nothing is appended
-    ap.v = nullptr;
-    ap.in_bf16 = in_dtype == OOMATTN_DTYPE_BF16;
-    ap.q_out = (uint8_t*)q_out + (size_t)r0 * ctx->cfg.n_heads * kHeadDim * out_es;
-    ap.q_out_bf16 = q_out_dtype == OOMATTN_DTYPE_BF16;
-    ap.bq = bq;
-    rc = launch_rope_append(ctx, ap, sb, n);
-    if (rc) return rc;
-  }
-  return OOMATTN_OK;
+  return rope_q_impl(ctx, n_rows, positions, q, in_dtype, bq, nullptr, q_out, q_out_dtype);
+}
+
+int oomattn_rope_q_qk_norm(oomattn_ctx* ctx, int32_t n_rows, const int32_t* positions, const void* q,
+                           int32_t in_dtype, const float* bq, const oomattn_qk_norm* norm, void* q_out,
+                           int32_t q_out_dtype) {
+  return rope_q_impl(ctx, n_rows, positions, q, in_dtype, bq, norm, q_out, q_out_dtype);
 }
 
 int oomattn_qkv_rope_append(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, int32_t n_new,
                             const float* x, const void* wq, const void* wk, const void* wv, int32_t w_dtype,
                             const float* bq, const float* bk, const float* bv, void* q_out, int32_t q_out_dtype) {
+  return oomattn_qkv_rope_append_qk_norm(ctx, layer, n_seqs, seq_ids, n_new, x, wq, wk, wv, w_dtype, bq, bk, bv,
+                                         nullptr, q_out, q_out_dtype);
+}
+
+int oomattn_qkv_rope_append_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids,
+                                    int32_t n_new, const float* x, const void* wq, const void* wk, const void* wv,
+                                    int32_t w_dtype, const float* bq, const float* bk, const float* bv,
+                                    const oomattn_qk_norm* norm, void* q_out, int32_t q_out_dtype) {
   if (!ctx) return OOMATTN_ERR_INVALID_ARG;
   if (!seq_ids || !x || !wq || !wk || !wv || !q_out || n_seqs <= 0 || n_new <= 0)
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad qkv_rope_append arguments");
   int rc = check_layer(ctx, layer);
   if (!rc) rc = validate_dtype(ctx, w_dtype, "weights");
   if (!rc) rc = validate_dtype(ctx, q_out_dtype, "q_out");
+  if (!rc) rc = check_norm(ctx, norm);
   if (rc) return rc;
   const int H = ctx->cfg.hidden_size;
   if (H <= 0 || H % 8 != 0) return fail(ctx, OOMATTN_ERR_BAD_CONFIG, "hidden_size %d must be a positive multiple of 8", H);
   DeviceGuard dg(ctx->device);
   const long long T = (long long)n_seqs * n_new;
   const int nq = ctx->cfg.n_heads * kHeadDim, nk = ctx->cfg.n_kv_heads * kHeadDim;
-  if (T <= kGemvMaxT) {
+  if (T <= kGemvMaxT && !rows_apart(ctx, norm)) {
     SeqBatch sb;
     rc = plan_append(ctx, layer, n_seqs, seq_ids, n_new, sb);
     if (rc) return rc;
@@ -1144,7 +1462,8 @@ int oomattn_qkv_rope_append(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, con
     commit_append(ctx, layer, sb, n_new);
     return OOMATTN_OK;
   }
-  // Larger T: tensor-core projections (K-F) into scratch, then the K-A epilogue kernel.
+  // Larger T: tensor-core projections (K-F) into scratch, then the K-A epilogue kernel; so too where that kernel
+  // needs whole heads (GEMVs up to 16 tokens).
   const int wb = w_dtype == OOMATTN_DTYPE_BF16;
   const size_t proj_bytes = (size_t)T * (nq + 2 * nk) * sizeof(float);
   rc = ensure_scratch(ctx, proj_bytes);
@@ -1154,10 +1473,10 @@ int oomattn_qkv_rope_append(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, con
   float* sv = sk + (size_t)T * nk;
   const KfJob jobs[3] = {{wq, wb, nq, nullptr, nullptr, sq}, {wk, wb, nk, nullptr, nullptr, sk},
                          {wv, wb, nk, nullptr, nullptr, sv}};
-  rc = kf_linear_f32(ctx, x, (int)T, H, jobs, 3);
+  rc = project(ctx, x, (int)T, H, jobs, 3);
   if (rc) return rc;
-  return oomattn_rope_append(ctx, layer, n_seqs, seq_ids, n_new, sq, sk, sv, OOMATTN_DTYPE_F32, bq, bk, bv, q_out,
-                             q_out_dtype);
+  return rope_append_impl(ctx, layer, n_seqs, seq_ids, nullptr, n_new, sq, sk, sv, OOMATTN_DTYPE_F32, bq, bk, bv, norm,
+                          q_out, q_out_dtype);
 }
 
 int oomattn_linear(oomattn_ctx* ctx, const float* x, const void* w, int32_t w_dtype, int32_t n_tokens, int32_t rows,
@@ -1236,6 +1555,8 @@ int oomattn_prefill(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_new,
                     int32_t out_dtype, float* lse) {
   if (!ctx) return OOMATTN_ERR_INVALID_ARG;
   if (n_new <= 0) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad prefill arguments");
+  if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4 && out_dtype == OOMATTN_DTYPE_BF16 && n_new <= kQ4PrefillRows)
+    return q4_prefill_rows(ctx, layer, seq, n_new, q, out, lse);
   const int32_t all[2] = {0, (n_new + 255) / 256};
   return oomattn_prefill_blocks(ctx, layer, seq, n_new, q, out, out_dtype, lse, 1, all);
 }
@@ -1249,8 +1570,8 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
   if (!rc) rc = check_seq(ctx, seq);
   if (!rc) rc = validate_dtype(ctx, out_dtype, "prefill out");
   if (rc) return rc;
-  if (ctx->cfg.kv_dtype != OOMATTN_DTYPE_BF16)
-    return fail(ctx, OOMATTN_ERR_UNSUPPORTED, "the tensor-core prefill needs a bf16 cache");
+  if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_F32)
+    return fail(ctx, OOMATTN_ERR_UNSUPPORTED, "the tensor-core prefill needs a bf16 or 4-bit cache");
   // The kernel's register split (setmaxnreg) balances only at this launch count.
   if (ctx->prefill_regs != kPfLaunchRegs)
     return fail(ctx, OOMATTN_ERR_UNSUPPORTED, "prefill kernel compiled with %d registers per thread, expected %d",
@@ -1332,8 +1653,16 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
   a.lse = lse;
   a.n_new = n_new;
   a.prefix = L - n_new;
+  KVPool pool = make_pool(ctx);
+  CUtensorMap kmap = ctx->kmap, vmap = ctx->vmap;
   a.seq = seq;
   a.layer = layer;
+  if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4) {
+    rc = q4_expand(ctx, layer, seq, L, &pool, &kmap, &vmap);
+    if (rc) return rc;
+    a.seq = 0;
+    a.layer = 0;
+  }
   a.n_heads = ctx->cfg.n_heads;
   a.group = ctx->group;
   a.n_pairs = n_pairs;
@@ -1341,7 +1670,7 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
   a.status = ctx->d_status;
   a.timeout_ns = ctx->timeout_ns;
   prefill_bf16_kernel<<<dim3((unsigned)(blocks * a.n_heads), n_chunks), kPfThreads, kPfSmemBytes, ctx->stream>>>(
-      qmap, ctx->kmap, ctx->vmap, omap, pmap, make_pool(ctx), a);
+      qmap, kmap, vmap, omap, pmap, pool, a);
   CKLAUNCH();
   if (n_chunks > 1) {
     const long long warps = (long long)n_new * a.n_heads;
@@ -1355,22 +1684,32 @@ int oomattn_attention_forward_with_bias(oomattn_ctx* ctx, int32_t layer, int32_t
                                         const float* x, const float* wq, const float* wk, const float* wv,
                                         const float* wo, int32_t o_out, const float* bq, const float* bk,
                                         const float* bv, float* out) {
+  return oomattn_attention_forward_qk_norm(ctx, layer, batch, seq_len, x, wq, wk, wv, wo, o_out, bq, bk, bv, nullptr,
+                                           out);
+}
+
+int oomattn_attention_forward_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t batch, int32_t seq_len,
+                                      const float* x, const float* wq, const float* wk, const float* wv,
+                                      const float* wo, int32_t o_out, const float* bq, const float* bk,
+                                      const float* bv, const oomattn_qk_norm* norm, float* out) {
   if (!ctx) return OOMATTN_ERR_INVALID_ARG;
   if (!x || !wq || !wk || !wv || !wo || !out || batch <= 0 || seq_len <= 0 || o_out <= 0)
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad attention_forward_with_bias arguments");
   if (batch > ctx->cfg.max_seqs)
     return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "batch %d exceeds max_seqs %d", batch, ctx->cfg.max_seqs);
   int rc = check_layer(ctx, layer);
+  if (!rc) rc = check_norm(ctx, norm);
   if (rc) return rc;
   DeviceGuard dg(ctx->device);
   const long long T = (long long)batch * seq_len;
   const int hq = ctx->cfg.n_heads, qo = hq * kHeadDim;
-  const bool use_prefill = ctx->cfg.kv_dtype == OOMATTN_DTYPE_BF16 && seq_len > 16;
+  const bool use_prefill = ctx->cfg.kv_dtype != OOMATTN_DTYPE_F32 && seq_len > 16;
+  const bool apart = T > kGemvMaxT || rows_apart(ctx, norm);
   // scratch: q (f32) | attention out (f32) | q bf16 for the prefill path
   const size_t q_bytes = (size_t)T * qo * sizeof(float);
   const size_t need = 2 * q_bytes + (use_prefill ? (size_t)T * qo * 2 : 0);
   // projection scratch is separate from the q/attention buffers; allocate both in one block
-  const size_t proj = T > kGemvMaxT ? (size_t)T * (qo + 2 * ctx->cfg.n_kv_heads * kHeadDim) * sizeof(float) : 0;
+  const size_t proj = apart ? (size_t)T * (qo + 2 * ctx->cfg.n_kv_heads * kHeadDim) * sizeof(float) : 0;
   rc = ensure_scratch(ctx, need + proj + 256);
   if (rc) return rc;
   float* qbuf = (float*)((uint8_t*)ctx->d_scratch + proj);
@@ -1381,7 +1720,7 @@ int oomattn_attention_forward_with_bias(oomattn_ctx* ctx, int32_t layer, int32_t
   std::vector<int> plen(batch);
   for (int b = 0; b < batch; ++b) plen[b] = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + b];
   // K-A (the cuBLAS branch writes its projections at the start of the scratch block)
-  if (T <= kGemvMaxT) {
+  if (!apart) {
     rc = oomattn_qkv_rope_append(ctx, layer, batch, seqs.data(), seq_len, x, wq, wk, wv, OOMATTN_DTYPE_F32, bq, bk,
                                  bv, use_prefill ? qb16 : (void*)qbuf,
                                  use_prefill ? OOMATTN_DTYPE_BF16 : OOMATTN_DTYPE_F32);
@@ -1393,10 +1732,10 @@ int oomattn_attention_forward_with_bias(oomattn_ctx* ctx, int32_t layer, int32_t
     const int H = ctx->cfg.hidden_size;
     const KfJob jobs[3] = {{wq, 0, qo, nullptr, nullptr, sq}, {wk, 0, nk, nullptr, nullptr, sk},
                            {wv, 0, nk, nullptr, nullptr, sv}};
-    rc = kf_linear_f32(ctx, x, (int)T, H, jobs, 3);
+    rc = project(ctx, x, (int)T, H, jobs, 3);
     if (rc) return rc;
-    rc = oomattn_rope_append(ctx, layer, batch, seqs.data(), seq_len, sq, sk, sv, OOMATTN_DTYPE_F32, bq, bk, bv,
-                             use_prefill ? qb16 : (void*)qbuf, use_prefill ? OOMATTN_DTYPE_BF16 : OOMATTN_DTYPE_F32);
+    rc = rope_append_impl(ctx, layer, batch, seqs.data(), nullptr, seq_len, sq, sk, sv, OOMATTN_DTYPE_F32, bq, bk, bv,
+                          norm, use_prefill ? qb16 : (void*)qbuf, use_prefill ? OOMATTN_DTYPE_BF16 : OOMATTN_DTYPE_F32);
   }
   if (rc) return rc;
   // attention
@@ -1484,7 +1823,7 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
   if (errbuf && errbuf_len > 0) errbuf[0] = '\0';
   if (!k_pool || !v_pool || !block_table || !seq_ids || !lens || !q || !out)
     return static_fail(errbuf, errbuf_len, OOMATTN_ERR_INVALID_ARG, "null pointer argument");
-  if (kv_dtype != OOMATTN_DTYPE_F32 && kv_dtype != OOMATTN_DTYPE_BF16)
+  if (kv_dtype != OOMATTN_DTYPE_F32 && kv_dtype != OOMATTN_DTYPE_BF16 && kv_dtype != OOMATTN_DTYPE_Q4)
     return static_fail(errbuf, errbuf_len, OOMATTN_ERR_INVALID_ARG, "unknown kv dtype %d", kv_dtype);
   if (device < 0 || device >= kStaticMaxDevices)
     return static_fail(errbuf, errbuf_len, OOMATTN_ERR_OUT_OF_RANGE, "device %d outside [0, %d)", device,
@@ -1504,6 +1843,8 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
     return static_fail(errbuf, errbuf_len, OOMATTN_ERR_OUT_OF_RANGE, "pool of %d pages unsupported", n_pool_pages);
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u)
     return static_fail(errbuf, errbuf_len, OOMATTN_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
+  if (kv_dtype == OOMATTN_DTYPE_Q4 && ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15u))
+    return static_fail(errbuf, errbuf_len, OOMATTN_ERR_INVALID_ARG, "the pools must be 16-byte aligned");
   SeqBatch sb;
   sb.n = n_rows;
   for (int z = 0; z < n_rows; ++z) {
@@ -1532,6 +1873,8 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
       if (e != cudaSuccess || !p)
         return static_fail(errbuf, errbuf_len, OOMATTN_ERR_CUDA, "cudaGetSymbolAddress: %s", cudaGetErrorString(e));
       e = cudaFuncSetAttribute(decode_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmemBytes);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(decode_q4_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4SmemBytes);
       if (e != cudaSuccess)
         return static_fail(errbuf, errbuf_len, OOMATTN_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       g_static_scratch[device] = p;
@@ -1550,8 +1893,8 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
   // partial fits the static array: nsplit <= slots / (rows * heads).
   const int cap_splits = std::max(1, std::min(split_cap(kv_dtype), kStaticPartSlots / (n_rows * n_heads)));
   DecodeSched sched;
-  const int n_items = plan_decode(sb, n_kv_heads, num_sms * (kv_dtype == OOMATTN_DTYPE_BF16 ? kDecCtasPerSm : 3), cap_splits,
-                                  kv_dtype == OOMATTN_DTYPE_BF16 ? kDecodeFillPages : kDecodeFillPagesF32, sched);
+  const int n_items = plan_decode(sb, n_kv_heads, num_sms * decode_slots(kv_dtype), cap_splits,
+                                  decode_fill(kv_dtype), sched);
   if (n_items == 0) return OOMATTN_OK;
 
   // The counters must start at zero; a previous call that ended early could
@@ -1604,6 +1947,8 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
                            "pool pointer rejected by cuTensorMapEncodeTiled (%d): it must be 16-byte aligned", (int)r);
     }
     decode_bf16_kernel<<<n_items, (kDecWarps + 1) * 32, kDecSmemBytes, st>>>(maps[0], maps[1], pool, a, sb, sched);
+  } else if (kv_dtype == OOMATTN_DTYPE_Q4) {
+    decode_q4_kernel<false><<<n_items, kDecWarps * 32, kQ4SmemBytes, st>>>(pool, a, sb, sched);
   } else {
     decode_f32_kernel<<<n_items, kDecWarps * 32, 0, st>>>(pool, a, sb, sched);
   }
@@ -2182,6 +2527,12 @@ extern "C" int oomattn_q8_mlp(oomattn_ctx* ctx, const oomattn_q8_matrix* gate, c
 
 extern "C" int oomattn_decoder_layer_q8(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids,
                                         const float* x, const oomattn_q8_layer* w, float* out) {
+  return oomattn_decoder_layer_q8_qk_norm(ctx, layer, n_seqs, seq_ids, x, w, nullptr, out);
+}
+
+extern "C" int oomattn_decoder_layer_q8_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs,
+                                                const int32_t* seq_ids, const float* x, const oomattn_q8_layer* w,
+                                                const oomattn_qk_norm* norm, float* out) {
   if (!ctx) return OOMATTN_ERR_INVALID_ARG;
   if (!seq_ids || !x || !w || !out || n_seqs <= 0)
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad decoder_layer_q8 arguments");
@@ -2218,8 +2569,8 @@ extern "C" int oomattn_decoder_layer_q8(oomattn_ctx* ctx, int32_t layer, int32_t
   const Q8Job qkv[3] = {{&w->q, w->bq, nullptr, q}, {&w->k, w->bk, nullptr, k}, {&w->v, w->bv, nullptr, v}};
   rc = q8_run(ctx, qkv, 3, x, nullptr, n_seqs, w->input_norm, w->eps);
   if (rc) return rc;
-  rc = oomattn_rope_append(ctx, layer, n_seqs, seq_ids, 1, q, k, v, OOMATTN_DTYPE_F32, nullptr, nullptr, nullptr, qr,
-                           OOMATTN_DTYPE_F32);
+  rc = rope_append_impl(ctx, layer, n_seqs, seq_ids, nullptr, 1, q, k, v, OOMATTN_DTYPE_F32, nullptr, nullptr, nullptr,
+                        norm, qr, OOMATTN_DTYPE_F32);
   if (rc) return rc;
   rc = oomattn_decode(ctx, layer, n_seqs, seq_ids, nullptr, qr, att, nullptr);
   if (rc) return rc;
@@ -2280,6 +2631,12 @@ extern "C" int oomattn_argmax(oomattn_ctx* ctx, const float* logits, int32_t n_r
 
 extern "C" int oomattn_decode_step_q8(oomattn_ctx* ctx, const oomattn_q8_model* m, int32_t n_seqs,
                                       const int32_t* seq_ids, const int32_t* tokens, int32_t* next, float* logits) {
+  return oomattn_decode_step_q8_qk_norm(ctx, m, nullptr, n_seqs, seq_ids, tokens, next, logits);
+}
+
+extern "C" int oomattn_decode_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q8_model* m,
+                                              const oomattn_qk_norm* norms, int32_t n_seqs, const int32_t* seq_ids,
+                                              const int32_t* tokens, int32_t* next, float* logits) {
   if (!ctx) return OOMATTN_ERR_INVALID_ARG;
   if (!m || !m->layers || !seq_ids || !tokens || !next || n_seqs <= 0)
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad decode_step_q8 arguments");
@@ -2311,7 +2668,7 @@ extern "C" int oomattn_decode_step_q8(oomattn_ctx* ctx, const oomattn_q8_model* 
   int rc = oomattn_embed_q8(ctx, &m->embed, tokens, n_seqs, xa);
   if (rc) return rc;
   for (int l = 0; l < m->n_layers; ++l) {
-    rc = oomattn_decoder_layer_q8(ctx, l, n_seqs, seq_ids, xa, &m->layers[l], xb);
+    rc = oomattn_decoder_layer_q8_qk_norm(ctx, l, n_seqs, seq_ids, xa, &m->layers[l], norms ? norms + l : nullptr, xb);
     if (rc) return rc;
     std::swap(xa, xb);
   }
@@ -2324,13 +2681,20 @@ extern "C" int oomattn_decode_step_q8(oomattn_ctx* ctx, const oomattn_q8_model* 
 extern "C" int oomattn_prefill_step_q8(oomattn_ctx* ctx, const oomattn_q8_model* m, int32_t n_seqs,
                                        const int32_t* seq_ids, int32_t n_new, const int32_t* tokens, int32_t* next,
                                        float* logits) {
+  return oomattn_prefill_step_q8_qk_norm(ctx, m, nullptr, n_seqs, seq_ids, n_new, tokens, next, logits);
+}
+
+extern "C" int oomattn_prefill_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q8_model* m,
+                                               const oomattn_qk_norm* norms, int32_t n_seqs, const int32_t* seq_ids,
+                                               int32_t n_new, const int32_t* tokens, int32_t* next, float* logits) {
   if (!ctx) return OOMATTN_ERR_INVALID_ARG;
   if (!m || !m->layers || !seq_ids || !tokens || !next || n_seqs <= 0 || n_new <= 0)
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad prefill_step_q8 arguments");
   if (m->n_layers <= 0 || m->n_layers > ctx->cfg.n_layers)
     return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "model has %d layers, the context %d", m->n_layers, ctx->cfg.n_layers);
-  if (ctx->cfg.kv_dtype != OOMATTN_DTYPE_BF16)
-    return fail(ctx, OOMATTN_ERR_UNSUPPORTED, "the model prefill runs the tensor-core attention: bf16 cache needed");
+  if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_F32)
+    return fail(ctx, OOMATTN_ERR_UNSUPPORTED,
+                "the model prefill runs the tensor-core attention: bf16 or 4-bit cache needed");
   const int H = ctx->cfg.hidden_size, hq = ctx->cfg.n_heads, hkv = ctx->cfg.n_kv_heads;
   const int nq = hq * kHeadDim, nkv = hkv * kHeadDim;
   if (m->embed.cols != H || m->lm_head.cols != H || !m->final_norm)
@@ -2342,6 +2706,10 @@ extern "C" int oomattn_prefill_step_q8(oomattn_ctx* ctx, const oomattn_q8_model*
         w->up.rows != w->gate.rows || w->down.rows != H || w->down.cols != w->gate.rows || !w->input_norm ||
         !w->post_norm)
       return fail(ctx, OOMATTN_ERR_INVALID_ARG, "layer %d: weight shapes do not match the configuration", l);
+    if (norms) {
+      const int nrc = check_norm(ctx, norms + l);
+      if (nrc) return nrc;
+    }
   }
   DeviceGuard dg(ctx->device);
   const size_t T = (size_t)n_seqs * n_new, B = (size_t)n_seqs, vocab = (size_t)m->lm_head.rows;
@@ -2392,8 +2760,8 @@ extern "C" int oomattn_prefill_step_q8(oomattn_ctx* ctx, const oomattn_q8_model*
     const Q8Job qkv[3] = {{&w->q, w->bq, nullptr, q}, {&w->k, w->bk, nullptr, k}, {&w->v, w->bv, nullptr, v}};
     rc = q8_run(ctx, qkv, 3, xa, nullptr, (int)T, w->input_norm, w->eps);
     if (rc) return rc;
-    rc = oomattn_rope_append(ctx, l, n_seqs, seq_ids, n_new, q, k, v, OOMATTN_DTYPE_F32, nullptr, nullptr, nullptr,
-                             qr, OOMATTN_DTYPE_BF16);
+    rc = rope_append_impl(ctx, l, n_seqs, seq_ids, nullptr, n_new, q, k, v, OOMATTN_DTYPE_F32, nullptr, nullptr,
+                          nullptr, norms ? norms + l : nullptr, qr, OOMATTN_DTYPE_BF16);
     if (rc) return rc;
     for (int b = 0; b < n_seqs; ++b) {
       rc = oomattn_prefill(ctx, l, seq_ids[b], n_new, qr + (size_t)b * n_new * nq, att + (size_t)b * n_new * nq,

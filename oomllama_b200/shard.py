@@ -260,23 +260,27 @@ class ShardedDecodeStep:
             a, _ = plan.slice_of(L, plan.slice_index)
             engine.set_position_offset(s, a)  # this slice's slot 0 sits at global position a
 
-    def __call__(self, q, k, v, bq=None, bk=None, bv=None):
-        """q [B, Hq_local*128], k, v [B, Hkv_local*128] projected (before bias and RoPE) for the new token
-        of each sequence -> attention output [B, Hq_local, 128] over the whole global context."""
+    def __call__(self, q, k, v, bq=None, bk=None, bv=None, q_norm=None, k_norm=None, eps=1e-6):
+        """q [B, Hq_local*128], k, v [B, Hkv_local*128] projected (before bias, the heads' norm if the model
+        has one, and RoPE) for the new token of each sequence -> attention output [B, Hq_local, 128] over the
+        whole global context."""
         import torch
         B = len(self.seq_ids)
         mine = [self.plan.appends_here(L, g) for L, g in zip(self.prompt_lens, self.global_lens)]
         hq = self.engine.config.n_heads
+        # only where the model norms its heads: an engine without them needs no such argument
+        q_args = {} if q_norm is None else {"q_norm": q_norm, "eps": eps}
+        k_args = {} if q_norm is None and k_norm is None else {"q_norm": q_norm, "k_norm": k_norm, "eps": eps}
         if all(mine):
-            qr = self.engine.rope_append(self.layer, self.seq_ids, q, k, v, bq, bk, bv)
+            qr = self.engine.rope_append(self.layer, self.seq_ids, q, k, v, bq, bk, bv, **k_args)
         else:
-            qr = self.engine.rope_q(self.global_lens, q, bq)
+            qr = self.engine.rope_q(self.global_lens, q, bq, **q_args)
             idx = [i for i, m in enumerate(mine) if m]
             if idx:  # the sequences whose new slot lies in this rank's slice
                 sel = torch.tensor(idx, device=q.device)
                 self.engine.rope_append(self.layer, [self.seq_ids[i] for i in idx], q.index_select(0, sel).contiguous(),
                                         k.index_select(0, sel).contiguous(), v.index_select(0, sel).contiguous(),
-                                        bq, bk, bv)
+                                        bq, bk, bv, **k_args)
         self.global_lens = [g + 1 for g in self.global_lens]
         return self.decoder(self.layer, self.seq_ids, qr.view(B, hq, 128))
 

@@ -25,7 +25,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import _lib
-from ._lib import DTYPE_BF16, DTYPE_F32, ROPE_INTERLEAVED, ROPE_SPLIT_HALF, check, int_array
+from ._lib import DTYPE_BF16, DTYPE_F32, DTYPE_Q4, ROPE_INTERLEAVED, ROPE_SPLIT_HALF, check, int_array
 
 PAGE_SIZE = 16
 HEAD_DIM = 128
@@ -41,6 +41,11 @@ def _dtype_code(t: torch.Tensor) -> int:
 
 def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+def _same_count(values, seq_ids, name: str):
+    if values is not None and len(values) != len(seq_ids):
+        raise ValueError(f"{name} has {len(values)} entries for {len(seq_ids)} sequences")
 
 
 def _dev(t: torch.Tensor, name: str, device: int, dtype=None, numel=None):
@@ -78,7 +83,7 @@ class TurboConfig:
     # new settings
     max_seqs: int = 1
     n_pages: int | None = None          # default: every sequence can reach max_seq_len
-    kv_dtype: str = "f32"               # "f32" or "bf16"
+    kv_dtype: str = "f32"               # "f32", "bf16" or "q4" (4 bits a value, groups of 32; include/oomattn.h)
     rope_variant: str = "interleaved"   # "interleaved" (apply_rope) or "split_half" (apply_rope_llama)
     rope_theta: float = 1e6
     softmax_scale: float | None = None  # None: 1/sqrt(head_dim)
@@ -94,7 +99,7 @@ class TurboConfig:
 
     def to_c(self) -> _lib.Config:
         n_pages = self.n_pages if self.n_pages is not None else self.max_seqs * self.pages_per_seq()
-        kv = {"f32": DTYPE_F32, "bf16": DTYPE_BF16}[self.kv_dtype]
+        kv = {"f32": DTYPE_F32, "bf16": DTYPE_BF16, "q4": DTYPE_Q4}[self.kv_dtype]
         rv = {"split_half": ROPE_SPLIT_HALF, "interleaved": ROPE_INTERLEAVED}[self.rope_variant]
         return _lib.Config(self.n_layers, self.hidden_size, self.n_heads, self.n_kv_heads, self.head_dim,
                            self.max_seq_len, self.max_seqs, PAGE_SIZE, n_pages, kv, rv, float(self.rope_theta),
@@ -187,10 +192,15 @@ class TurboEngine:
         check(self._ctx, self._L.oomattn_set_seq_len(self._ctx, layer, seq, length))
 
     def kv_pool(self):
-        """(k_pool, v_pool) device tensors [n_layers, n_pages+1, n_kv, 16, 128] aliasing the pools."""
+        """(k_pool, v_pool) device tensors [n_layers, n_pages+1, n_kv, 16, 128] aliasing the pools; of a 4-bit cache
+        uint8 [n_layers, n_pages+1, n_kv, Q4_CHUNK] in the layout that include/oomattn.h gives."""
         kp, vp = ctypes.c_void_p(), ctypes.c_void_p()
         check(self._ctx, self._L.oomattn_kv_pool(self._ctx, ctypes.byref(kp), ctypes.byref(vp)))
         c = self.config
+        if c.kv_dtype == "q4":
+            shape = (c.n_layers, self._n_pages + 1, c.n_kv_heads, _lib.Q4_CHUNK)
+            return (_alias(kp.value, shape, torch.uint8, self.device),
+                    _alias(vp.value, shape, torch.uint8, self.device))
         shape = (c.n_layers, self._n_pages + 1, c.n_kv_heads, PAGE_SIZE, HEAD_DIM)
         dt = torch.bfloat16 if c.kv_dtype == "bf16" else torch.float32
         return _alias(kp.value, shape, dt, self.device), _alias(vp.value, shape, dt, self.device)
@@ -205,7 +215,7 @@ class TurboEngine:
         check(self._ctx, self._L.oomattn_kv_write(self._ctx, layer, seq, _ptr(k), _ptr(v), n, _dtype_code(k)))
 
     def kv_read(self, layer: int, seq: int):
-        """LayerKVCache::get (src/oomllama_turbo.rs:57-63): host tensors [n_kv, L, 128]."""
+        """LayerKVCache::get (src/oomllama_turbo.rs:57-63): host tensors [n_kv, L, 128] (4-bit cache: its values, f32)."""
         L_ = self.seq_len(layer, seq)
         dt = torch.bfloat16 if self.config.kv_dtype == "bf16" else torch.float32
         k = torch.empty(self.config.n_kv_heads, L_, HEAD_DIM, dtype=dt)
@@ -214,13 +224,51 @@ class TurboEngine:
         check(self._ctx, self._L.oomattn_kv_read(self._ctx, layer, seq, _ptr(k), _ptr(v)))
         return k, v
 
-    # ------------------------------------------------------------ K-A
-    def rope_append(self, layer: int, seq_ids, q, k, v, bq=None, bk=None, bv=None, q_out_dtype=torch.float32):
-        """Bias + RoPE + append for projected rows; q [T, Hq*128], k/v [T, Hkv*128]
-        with T = len(seq_ids) * n_new.  Returns the rotated q [T, Hq, 128]."""
+    def kv_gather(self, layer: int, seq_ids, starts=None, n: int | None = None, out_dtype=torch.float32, k_out=None,
+                  v_out=None):
+        """LayerKVCache::get (src/oomllama_turbo.rs:57-63) on the device: the values of n cached rows of each
+        sequence from slot starts[i] (None: 0; n None: the first sequence's whole length).
+        Returns k, v [len(seq_ids) * n, n_kv, 128] in out_dtype."""
         seq_ids = list(seq_ids)
+        starts = None if starts is None else list(starts)
+        _same_count(starts, seq_ids, "starts")
+        if n is None:
+            n = self.seq_len(layer, seq_ids[0]) - (starts[0] if starts else 0)
+        shape = (len(seq_ids) * n, self.config.n_kv_heads, HEAD_DIM)
+        if k_out is None:
+            k_out = torch.empty(shape, dtype=out_dtype, device=self.device)
+        if v_out is None:
+            v_out = torch.empty(shape, dtype=out_dtype, device=self.device)
+        for name, t in (("k_out", k_out), ("v_out", v_out)):
+            _dev(t, name, self.device, dtype=out_dtype, numel=shape[0] * shape[1] * HEAD_DIM)
+        self._bind_stream()
+        check(self._ctx, self._L.oomattn_kv_gather(
+            self._ctx, layer, len(seq_ids), int_array(seq_ids), None if starts is None else int_array(starts), n,
+            _DT[out_dtype], _ptr(k_out), _ptr(v_out)))
+        return k_out, v_out
+
+    # ------------------------------------------------------------ K-A
+    def _qk_norm(self, q_norm, k_norm, eps):
+        """The oomattn_qk_norm of two weights [128] f32 (either may be None), or None without any."""
+        if q_norm is None and k_norm is None:
+            return None
+        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if w is not None:
+                _dev(w, name, self.device, dtype=torch.float32, numel=HEAD_DIM)
+        return _lib.QkNorm(None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
+                           float(eps))
+
+    def rope_append(self, layer: int, seq_ids, q, k, v, bq=None, bk=None, bv=None, q_out_dtype=torch.float32,
+                    q_norm=None, k_norm=None, eps: float = 1e-6, starts=None, q_out=None):
+        """Bias + RoPE + append for projected rows; q [T, Hq*128], k/v [T, Hkv*128]
+        with T = len(seq_ids) * n_new.  Returns the rotated q [T, Hq, 128].
+        q_norm, k_norm [128] f32: weights of an RMS norm of every q and k head between bias and RoPE.
+        starts: the first new slot of each sequence, at most its length (default); the rows behind it are given up."""
+        seq_ids = list(seq_ids)
+        starts = None if starts is None else list(starts)
+        _same_count(starts, seq_ids, "starts")
         T = q.shape[0]
-        if T % len(seq_ids):
+        if not seq_ids or T % len(seq_ids):
             raise ValueError("token count is not a multiple of the number of sequences")
         n_new = T // len(seq_ids)
         c = self.config
@@ -230,16 +278,22 @@ class TurboEngine:
         for b, n in ((bq, c.n_heads), (bk, c.n_kv_heads), (bv, c.n_kv_heads)):
             if b is not None:
                 _dev(b, "bias", self.device, dtype=torch.float32, numel=n * HEAD_DIM)
-        q_out = torch.empty(T, c.n_heads, HEAD_DIM, dtype=q_out_dtype, device=q.device)
+        if q_out is None:
+            q_out = torch.empty(T, c.n_heads, HEAD_DIM, dtype=q_out_dtype, device=q.device)
+        else:
+            _dev(q_out, "q_out", self.device, dtype=q_out_dtype, numel=T * c.n_heads * HEAD_DIM)
+        norm = self._qk_norm(q_norm, k_norm, eps)
         self._bind_stream()
-        check(self._ctx, self._L.oomattn_rope_append(
-            self._ctx, layer, len(seq_ids), int_array(seq_ids), n_new, _ptr(q), _ptr(k), _ptr(v), _dtype_code(q),
-            _ptr(bq), _ptr(bk), _ptr(bv), _ptr(q_out), _DT[q_out_dtype]))
+        check(self._ctx, self._L.oomattn_rope_append_qk_norm(
+            self._ctx, layer, len(seq_ids), int_array(seq_ids), None if starts is None else int_array(starts), n_new,
+            _ptr(q), _ptr(k), _ptr(v), _dtype_code(q), _ptr(bq), _ptr(bk), _ptr(bv), norm, _ptr(q_out),
+            _DT[q_out_dtype]))
         return q_out
 
-    def rope_q(self, positions, q, bq=None, q_out_dtype=torch.float32, out=None):
+    def rope_q(self, positions, q, bq=None, q_out_dtype=torch.float32, out=None, q_norm=None, eps: float = 1e-6):
         """RoPE of q rows [R, Hq*128] at explicit positions, nothing appended (the q half of
-        TurboEngine::apply_rope, src/oomllama_turbo.rs:737-786).  Returns [R, Hq, 128]."""
+        TurboEngine::apply_rope, src/oomllama_turbo.rs:737-786), behind a norm of every head where q_norm [128] is
+        given.  Returns [R, Hq, 128]."""
         positions = list(positions)
         R = len(positions)
         c = self.config
@@ -248,13 +302,14 @@ class TurboEngine:
             _dev(bq, "bq", self.device, dtype=torch.float32, numel=c.n_heads * HEAD_DIM)
         if out is None:
             out = torch.empty(R, c.n_heads, HEAD_DIM, dtype=q_out_dtype, device=q.device)
+        norm = self._qk_norm(q_norm, None, eps)
         self._bind_stream()
-        check(self._ctx, self._L.oomattn_rope_q(self._ctx, R, int_array(positions), _ptr(q), _dtype_code(q), _ptr(bq),
-                                                _ptr(out), _DT[out.dtype]))
+        check(self._ctx, self._L.oomattn_rope_q_qk_norm(self._ctx, R, int_array(positions), _ptr(q), _dtype_code(q),
+                                                        _ptr(bq), norm, _ptr(out), _DT[out.dtype]))
         return out
 
     def qkv_rope_append(self, layer: int, seq_ids, x, wq, wk, wv, bq=None, bk=None, bv=None,
-                        q_out_dtype=torch.float32):
+                        q_out_dtype=torch.float32, q_norm=None, k_norm=None, eps: float = 1e-6):
         """QKV projection + bias + RoPE + append (src/oomllama_turbo.rs:638-681).
         x [T, hidden] f32; weights [out, hidden] f32 or bf16."""
         seq_ids = list(seq_ids)
@@ -267,10 +322,11 @@ class TurboEngine:
         _dev(wk, "wk", self.device, dtype=wq.dtype, numel=c.n_kv_heads * HEAD_DIM * H)
         _dev(wv, "wv", self.device, dtype=wq.dtype, numel=c.n_kv_heads * HEAD_DIM * H)
         q_out = torch.empty(T, c.n_heads, HEAD_DIM, dtype=q_out_dtype, device=x.device)
+        norm = self._qk_norm(q_norm, k_norm, eps)
         self._bind_stream()
-        check(self._ctx, self._L.oomattn_qkv_rope_append(
+        check(self._ctx, self._L.oomattn_qkv_rope_append_qk_norm(
             self._ctx, layer, len(seq_ids), int_array(seq_ids), n_new, _ptr(x), _ptr(wq), _ptr(wk), _ptr(wv),
-            _dtype_code(wq), _ptr(bq), _ptr(bk), _ptr(bv), _ptr(q_out), _DT[q_out_dtype]))
+            _dtype_code(wq), _ptr(bq), _ptr(bk), _ptr(bv), norm, _ptr(q_out), _DT[q_out_dtype]))
         return q_out
 
     # ------------------------------------------------------------ K-B / K-C
@@ -320,7 +376,7 @@ class TurboEngine:
 
     def prefill(self, layer: int, seq: int, q, out_dtype=torch.float32, with_lse: bool = False, out=None,
                 blocks=None):
-        """Causal attention of the n_new newest tokens of `seq` (bf16 cache).
+        """Causal attention of the n_new newest tokens of `seq` (bf16 or 4-bit cache).
         q [n_new, Hq, 128] bf16 (rotated) -> out [n_new, Hq, 128].  `blocks`: optional list of
         (lo, hi) ranges of 256-row query blocks to compute (the others' rows are not written)."""
         c = self.config
@@ -353,7 +409,8 @@ class TurboEngine:
         return out, lse
 
     # ------------------------------------------------------------ the layer step
-    def attention_forward_with_bias(self, layer_idx: int, x, wq, wk, wv, wo, bq=None, bk=None, bv=None):
+    def attention_forward_with_bias(self, layer_idx: int, x, wq, wk, wv, wo, bq=None, bk=None, bv=None, q_norm=None,
+                                    k_norm=None, eps: float = 1e-6):
         """TurboEngine::attention_forward_with_bias (src/oomllama_turbo.rs:618-723).
         x [B, S, hidden] f32, weights [out, in] f32 -> [B, S, o_out] f32."""
         c = self.config
@@ -369,10 +426,11 @@ class TurboEngine:
             if b is not None:
                 _dev(b, name, self.device, dtype=torch.float32, numel=n * HEAD_DIM)
         out = torch.empty(B, S, o_out, dtype=torch.float32, device=x.device)
+        norm = self._qk_norm(q_norm, k_norm, eps)
         self._bind_stream()
-        check(self._ctx, self._L.oomattn_attention_forward_with_bias(
+        check(self._ctx, self._L.oomattn_attention_forward_qk_norm(
             self._ctx, layer_idx, B, S, _ptr(x), _ptr(wq), _ptr(wk), _ptr(wv), _ptr(wo), o_out, _ptr(bq), _ptr(bk),
-            _ptr(bv), _ptr(out)))
+            _ptr(bv), norm, _ptr(out)))
         return out
 
 
@@ -445,8 +503,9 @@ class TurboEngine:
         out = torch.empty_like(x) if out is None else _dev(out, "out", self.device, dtype=torch.float32, numel=B * H)
         self._bind_stream()
         ids = int_array(seq_ids)
-        check(self._ctx, self._L.oomattn_decoder_layer_q8(self._ctx, layer, B, ids, _ptr(x),
-                                                          ctypes.byref(w.c_struct()), _ptr(out)))
+        norm = self._qk_norm(w.q_norm, w.k_norm, w.eps)
+        check(self._ctx, self._L.oomattn_decoder_layer_q8_qk_norm(self._ctx, layer, B, ids, _ptr(x),
+                                                                  ctypes.byref(w.c_struct()), norm, _ptr(out)))
         return out
 
     def q8_repack(self, blocks: torch.Tensor, n_values: int, rows: int = None, cols: int = None):
@@ -496,15 +555,15 @@ class TurboEngine:
             _dev(logits, "logits", self.device, dtype=torch.float32, numel=B * model.lm_head.rows)
         self._bind_stream()
         ids = int_array(seq_ids)
-        check(self._ctx, self._L.oomattn_decode_step_q8(self._ctx, ctypes.byref(model.c_struct()), B, ids,
-                                                        _ptr(tokens), _ptr(nxt),
-                                                        None if logits is None else _ptr(logits)))
+        check(self._ctx, self._L.oomattn_decode_step_q8_qk_norm(self._ctx, ctypes.byref(model.c_struct()),
+                                                                model.c_norms(self), B, ids, _ptr(tokens), _ptr(nxt),
+                                                                None if logits is None else _ptr(logits)))
         return nxt
 
     def prefill_step_q8(self, model: "Q8Model", seq_ids, tokens: torch.Tensor, next_tokens=None, logits=None):
         """The prompt through the whole model (OomLlamaModel::forward_turbo over every prompt token,
         src/oomllama.rs:504-553, 969-970): int32 tokens [B, n_new] -> int32 next [B], the greedy pick after each
-        sequence's last prompt token.  Every layer's cache grows by n_new tokens per sequence (bf16 cache)."""
+        sequence's last prompt token.  Every layer's cache grows by n_new tokens per sequence (bf16 or 4-bit cache)."""
         B, n_new = tokens.shape
         _dev(tokens, "tokens", self.device, dtype=torch.int32)
         nxt = (torch.empty(B, dtype=torch.int32, device=self.device) if next_tokens is None
@@ -512,9 +571,10 @@ class TurboEngine:
         if logits is not None:
             _dev(logits, "logits", self.device, dtype=torch.float32, numel=B * model.lm_head.rows)
         self._bind_stream()
-        check(self._ctx, self._L.oomattn_prefill_step_q8(self._ctx, ctypes.byref(model.c_struct()), B,
-                                                         int_array(seq_ids), n_new, _ptr(tokens), _ptr(nxt),
-                                                         None if logits is None else _ptr(logits)))
+        check(self._ctx, self._L.oomattn_prefill_step_q8_qk_norm(self._ctx, ctypes.byref(model.c_struct()),
+                                                                 model.c_norms(self), B, int_array(seq_ids), n_new,
+                                                                 _ptr(tokens), _ptr(nxt),
+                                                                 None if logits is None else _ptr(logits)))
         return nxt
 
 
@@ -644,7 +704,7 @@ def _alias(ptr: int, shape, dtype, device: int) -> torch.Tensor:
 @dataclass
 class Q8DecoderLayer:
     """One decoder layer's resident weights (GhostDecoderLayer, src/oomllama.rs:366-402): Q8 projections and MLP,
-    f32 attention biases (or None) and RMSNorm weights."""
+    f32 attention biases (or None) and RMSNorm weights; q_norm and k_norm [128] where the model norms its heads."""
     q: Q8Matrix
     k: Q8Matrix
     v: Q8Matrix
@@ -658,6 +718,8 @@ class Q8DecoderLayer:
     bq: torch.Tensor = None
     bk: torch.Tensor = None
     bv: torch.Tensor = None
+    q_norm: torch.Tensor = None
+    k_norm: torch.Tensor = None
 
     def c_struct(self) -> _lib.Q8Layer:
         p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
@@ -697,7 +759,8 @@ class Q8Model:
                 gate=m("mlp.gate_proj.weight", inter, H), up=m("mlp.up_proj.weight", inter, H),
                 down=m("mlp.down_proj.weight", H, inter), input_norm=f32(p + "input_layernorm.weight"),
                 post_norm=f32(p + "post_attention_layernorm.weight"), eps=eps, bq=f32(p + "self_attn.q_proj.bias"),
-                bk=f32(p + "self_attn.k_proj.bias"), bv=f32(p + "self_attn.v_proj.bias")))
+                bk=f32(p + "self_attn.k_proj.bias"), bv=f32(p + "self_attn.v_proj.bias"),
+                q_norm=f32(p + "self_attn.q_norm.weight"), k_norm=f32(p + "self_attn.k_norm.weight")))
         embed = oom.q8_matrix(engine, "model.embed_tokens.weight", vocab, H)
         head = oom.q8_matrix(engine, "lm_head.weight", vocab, H) if "lm_head.weight" in oom.tensors else embed
         return cls(layers=layers, embed=embed, lm_head=head, final_norm=f32("model.norm.weight"), eps=eps)
@@ -708,3 +771,10 @@ class Q8Model:
                          self.lm_head.c_struct(), self.final_norm.data_ptr(), self.eps)
         m._keep = arr  # the layer array lives as long as the struct
         return m
+
+    def c_norms(self, engine: "TurboEngine"):
+        """The layers' oomattn_qk_norm array, or None where no layer norms its heads."""
+        norms = [engine._qk_norm(l.q_norm, l.k_norm, l.eps) for l in self.layers]
+        if not any(norms):
+            return None
+        return (_lib.QkNorm * len(norms))(*[n or _lib.QkNorm(None, None, 0.0) for n in norms])
