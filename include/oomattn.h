@@ -64,9 +64,9 @@ enum { OOMATTN_DTYPE_F32 = 0, OOMATTN_DTYPE_BF16 = 1, OOMATTN_DTYPE_Q4 = 2 };
  * value off by at most 0.53 s + 2^-12 |o|.  Values saturate at +-60000; a
  * group that holds a NaN reads back as NaN; groups whose values differ by less
  * than about 1e-5 keep only their middle.
- * A page of 16 tokens of one kv head is a chunk of OOMATTN_Q4_CHUNK bytes in
- * the K pool and one in the V pool, chunk (layer, page, kv) at
- * ((layer*(n_pages+1) + page)*n_kv + kv) * OOMATTN_Q4_CHUNK:
+ * A page of 16 tokens of one kv head is a chunk of OOMATTN_Q4_CHUNK bytes of K
+ * and, right behind it, one of V: one pool, whose chunk of K (layer, page, kv)
+ * lies at ((layer*(n_pages+1) + page)*n_kv + kv) * 2 * OOMATTN_Q4_CHUNK.
  *   K: token r, dims 32w + 8t + n (w, t < 4, n < 8): nibble n of the 32-bit
  *      word at 64r + 16t + 4w; f16 o[0..3], s[0..3] at 1024 + 16r.
  *   V: token r = 8h + 2t + p (p < 2), dims 32w + 4g + n (g < 8, n < 4): nibble
@@ -161,7 +161,8 @@ int oomattn_set_seq_len(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t le
 
 /* Device addresses of the K and V pools: element (layer, page, kv, slot, d)
  * at (((layer*(n_pages+1) + page)*n_kv + kv)*16 + slot)*128 + d, in kv_dtype
- * (4-bit: chunks, see OOMATTN_Q4_CHUNK).  Page n_pages is the null page. */
+ * (4-bit: K and V chunks in turn, see OOMATTN_Q4_CHUNK; *v_pool is *k_pool +
+ * OOMATTN_Q4_CHUNK).  Page n_pages is the null page. */
 int oomattn_kv_pool(const oomattn_ctx* ctx, void** k_pool, void** v_pool);
 
 /* LayerKVCache::append (src/oomllama_turbo.rs:41-55) of already-rotated rows:
@@ -299,7 +300,7 @@ int oomattn_merge_packed(oomattn_ctx* ctx, int32_t n_parts, int32_t n_rows, cons
  *   device, stream: the GPU and cudaStream_t to run on
  *   kv_dtype: OOMATTN_DTYPE_BF16, OOMATTN_DTYPE_F32 or OOMATTN_DTYPE_Q4
  *   k_pool, v_pool: [n_pool_pages][n_kv_heads][16][128] in kv_dtype (4-bit:
- *     chunks [n_pool_pages][n_kv_heads][OOMATTN_Q4_CHUNK]), 16-byte aligned
+ *     one pool, v_pool = k_pool + OOMATTN_Q4_CHUNK), 16-byte aligned
  *   block_table: device int32 [n_block_rows][max_pages_per_seq]
  *   q, out: f32 [n_rows][n_heads][128]; lse: f32 [n_rows][n_heads] or NULL
  *   seq_ids, lens (host): row z attends to the first lens[z] slots of block-table row seq_ids[z]

@@ -17,7 +17,7 @@ STATUS_NAMES = {
     7: "NO_MEMORY", 8: "UNSUPPORTED", 9: "DEVICE_CHECK",
 }
 DTYPE_F32, DTYPE_BF16, DTYPE_Q4 = 0, 1, 2   # Q4: a cache type only
-Q4_CHUNK = 1280                     # bytes of a page of one kv head in a 4-bit K or V pool
+Q4_CHUNK = 1280                     # bytes of K, and of V, of a page of one kv head in a 4-bit pool
 PACKED_STRIDE = 132                 # floats per (row, q head) of a packed decode output: O[128], lse, pad
 TEST_DROP_DECODE_COPIES = 1         # oomattn_set_test_flags: the bf16 decode's producer issues no copies
 TEST_DROP_LINEAR_COPIES = 2         # oomattn_set_test_flags: the Q8 tensor-core pass's producer issues no copies

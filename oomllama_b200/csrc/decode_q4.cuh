@@ -23,7 +23,7 @@
 // when it accumulates, which over a long context would shrink O.
 //
 // Each warp works alone: its own ring of tiles in shared memory, filled by
-// bulk copies (two 1280-byte chunks per page) that one of its lanes issues, its
+// bulk copies (one of 2560 bytes per page: K, then V) that one of its lanes issues, its
 // own running maximum and sum; the four warps of a CTA join at the end.
 #pragma once
 #include "common.cuh"
@@ -36,7 +36,7 @@ namespace oomattn {
 
 constexpr int kQ4Pages = 2;                              // pages per tile
 constexpr int kQ4Tile = kQ4Pages * kPageSize;            // tokens per tile
-constexpr int kQ4TileBytes = kQ4Pages * 2 * kQ4Chunk;    // 5 KB
+constexpr int kQ4TileBytes = kQ4Pages * kQ4Pair;         // 5 KB
 constexpr int kQ4Stages = 3;
 constexpr int kQ4CtasPerSm = 3;
 constexpr int kQ4RingBytes = kDecWarps * kQ4Stages * kQ4TileBytes;
@@ -55,11 +55,18 @@ __device__ __forceinline__ void mma_f16_16816(float* d, const uint32_t* a, uint3
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_f16_1688(float* d, uint32_t a0, uint32_t a1, uint32_t b0) {
+// The same from zero: the accumulator's registers need no clearing.
+__device__ __forceinline__ void mma_f16_16816_z(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm(
-      "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(b0));
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_f16_1688_z(float* d, uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm(
+      "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -76,6 +83,12 @@ __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
+// (x & mask) | magic in one instruction (with both as immediates it takes two).
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t magic) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(mask), "r"(magic));
+  return d;
+}
 __device__ __forceinline__ float h_lo(uint32_t v) { return __half2float(__ushort_as_half((uint16_t)v)); }
 __device__ __forceinline__ float h_hi(uint32_t v) { return __half2float(__ushort_as_half((uint16_t)(v >> 16))); }
 // (a, b) as f16 pairs hi + lo: lo = x - hi is exact in f32 and rounded once.
@@ -89,13 +102,13 @@ __device__ __forceinline__ void q4_prefetch_then_wait(const KVPool& pool, const 
                                                       int pe) {
   const int np = min(pe - pb, kDecPrefetchPages);
   if (np > 0) {
-    constexpr int lines = kQ4Chunk / 128;
+    constexpr int lines = kQ4Pair / 128;
     const int* bt = pool.block_table + (size_t)seq * pool.max_pages_per_seq;
-    for (int i = threadIdx.x; i < np * 2 * lines; i += blockDim.x) {
-      const int page = __ldg(bt + pb + i / (2 * lines)), r = i % (2 * lines);
+    for (int i = threadIdx.x; i < np * lines; i += blockDim.x) {
+      const int page = __ldg(bt + pb + i / lines), r = i % lines;
       if ((unsigned)page >= (unsigned)pool.n_pool_pages) continue;  // reported by the main loop
-      const char* base = static_cast<const char*>(r < lines ? pool.k : pool.v) + q4_chunk_off(pool, a.layer, page, g);
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(base + (size_t)(r % lines) * 128));
+      const char* base = static_cast<const char*>(pool.k) + q4_chunk_off(pool, a.layer, page, g);
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(base + (size_t)r * 128));
     }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -127,7 +140,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
   uint8_t* ring = smem_q4 + warp * (kQ4Stages * kQ4TileBytes);
   uint64_t* full = bars + warp * kQ4Stages;
   if (lane == 0)
-    for (int s = 0; s < kQ4Stages; ++s) mbar_init(&full[s], 1);
+    for (int s = 0; s < kQ4Stages; ++s) mbar_init(&full[s], kQ4Pages);
   fence_mbar_init();
   __syncwarp();
 
@@ -152,8 +165,10 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
   int ids = load_id(lane), ids_next = load_id(lane + 32);
   int issued = 0;
   bool gave_up = false;
-  const uint8_t* kbase = static_cast<const uint8_t*>(pool.k);
-  const uint8_t* vbase = static_cast<const uint8_t*>(pool.v);
+  // lane i copies K and V of a tile's page i: one chunk of the pool
+  const uint8_t* base = static_cast<const uint8_t*>(pool.k) + q4_chunk_off(pool, a.layer, 0, g_kv);
+  const uint32_t page_bytes = (uint32_t)pool.n_kv * kQ4Pair;
+  uint8_t* dst0 = ring + (lane & 1) * kQ4Pair;
   const bool drop = (a.test_flags & kTestDropDecodeCopies) != 0;
   auto issue = [&](int k) {  // all lanes; copies of local tile k into its stage
     const int j = (k * kQ4Pages) & 31;
@@ -161,15 +176,14 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
       ids = ids_next;
       ids_next = load_id(k * kQ4Pages + 32 + lane);
     }
-    const int id = __shfl_sync(0xffffffffu, ids, j + (lane >> 1 & 1));
-    const int id1 = __shfl_sync(0xffffffffu, ids, j + 1);
+    const int id = __shfl_sync(0xffffffffu, ids, j + (lane & 1));
     if (drop) return;
     const int s = k % kQ4Stages;
-    if (lane == 0) mbar_arrive_expect_tx(&full[s], id1 >= 0 ? 4 * kQ4Chunk : 2 * kQ4Chunk);
-    __syncwarp();
-    if (lane < 4 && id >= 0)  // lane 0: K of page 0, 1: V of page 0, 2, 3: page 1
-      bulk_load(ring + s * kQ4TileBytes + lane * kQ4Chunk,
-                ((lane & 1) ? vbase : kbase) + q4_chunk_off(pool, a.layer, id, g_kv), kQ4Chunk, &full[s]);
+    // each of the two lanes arrives for its own page (a missing second one: no bytes)
+    if (lane < kQ4Pages) {
+      mbar_arrive_expect_tx(&full[s], id >= 0 ? kQ4Pair : 0);
+      if (id >= 0) bulk_load(dst0 + s * kQ4TileBytes, base + (size_t)(uint32_t)id * page_bytes, kQ4Pair, &full[s]);
+    }
     issued = k + 1;
   };
   for (int k = 0; k < min(kQ4Stages, n_tiles); ++k) issue(k);
@@ -232,6 +246,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
   uint64_t oo = 0;   // sum p * offset of groups 2 (t & 1), 2 (t & 1) + 1
   float m = -INFINITY, l = 0.f;
   const int tok_end = min(pe * kPageSize, L);
+  uint32_t magic;  // 1024.0 in both halves, in a register
+  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
   const uint64_t kMetaUnit = f2_pack(1.f / 4096.f, 1.f / 4096.f);  // 2^-24 / 2^-12
 
   for (int k = 0; k < n_tiles; ++k) {
@@ -249,7 +265,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
       // become -inf below.  (No copy follows into this stage.)
       const int tok = lane;
       if (tok >= lim) {
-        uint8_t* mp = st + (tok >> 4) * (2 * kQ4Chunk) + kQ4Chunk + kQ4Meta + q4_v_meta(tok & 15) + 2 * (tok & 1);
+        uint8_t* mp = st + (tok >> 4) * kQ4Pair + kQ4Chunk + kQ4Meta + q4_v_meta(tok & 15) + 2 * (tok & 1);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           *reinterpret_cast<uint16_t*>(mp + 4 * w) = 0;
@@ -262,22 +278,22 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
     float sc[8];
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt) {
-      const uint8_t* kc = st + (nt >> 1) * (2 * kQ4Chunk);
+      const uint8_t* kc = st + (nt >> 1) * kQ4Pair;
       const int h = nt & 1;
       const uint4 w4 = *reinterpret_cast<const uint4*>(kc + h * 512 + lane * 16);
       const uint32_t bm = *reinterpret_cast<const uint32_t*>(kc + kQ4Meta + (8 * h + g) * 16 + t * 4);
       const uint2 s0 = *reinterpret_cast<const uint2*>(kc + kQ4Meta + (8 * h + 2 * t) * 16 + 8);
       const uint2 s1 = *reinterpret_cast<const uint2*>(kc + kQ4Meta + (8 * h + 2 * t + 1) * 16 + 8);
       const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-      float d[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_f16_1688(d, am[0], am[1], bm);
+      float d[4];
+      mma_f16_1688_z(d, am[0], am[1], bm);
       uint64_t acc = f2_fma(f2_pack(d[0], d[1]), kMetaUnit, 0);
       acc = f2_fma(f2_pack(d[2], d[3]), kMetaUnit, acc);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const uint32_t x = w[q], y = w[q] >> 8;
-        float e[4] = {0.f, 0.f, 0.f, 0.f};
-        mma_f16_16816(e, qa[2 * q], x & 0x000f000fu, x & 0x00f000f0u);
+        float e[4];
+        mma_f16_16816_z(e, qa[2 * q], x & 0x000f000fu, x & 0x00f000f0u);
         mma_f16_16816(e, qa[2 * q + 1], y & 0x000f000fu, y & 0x00f000f0u);
         const uint32_t a0 = q < 2 ? s0.x : s0.y, a1 = q < 2 ? s1.x : s1.y;
         const uint64_t sp = (q & 1) ? f2_pack(h_hi(a0), h_hi(a1)) : f2_pack(h_lo(a0), h_lo(a1));
@@ -297,10 +313,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
     mt = max3f(mt, sc[6], sc[7]);
     mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
     mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-    const float mn = fmaxf(m, mt);
-    const float alpha = ex2_ftz((m - mn) * f2);
-    m = mn;
-    const float mf = mn * f2;
+    // m is the running maximum as a base-2 logit, rounded: the same number in
+    // every weight, so its rounding cancels
+    const float mf = fmaxf(m, mt * f2);
+    const float alpha = ex2_ftz(m - mf);
+    m = mf;
     float ps = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -317,25 +334,25 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
     // ---- O = O * alpha + P V
     const uint64_t al2 = f2_pack(alpha, alpha);
     uint4 vw[4], vs[4];  // [page, half]: the four groups' codes and scales of the lane's token pair
-    float d[4] = {0.f, 0.f, 0.f, 0.f};
+    float d[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint8_t* vc = st + (i >> 1) * (2 * kQ4Chunk) + kQ4Chunk;
+      const uint8_t* vc = st + (i >> 1) * kQ4Pair + kQ4Chunk;
       vw[i] = *reinterpret_cast<const uint4*>(vc + (i & 1) * 512 + lane * 16);
       vs[i] = *reinterpret_cast<const uint4*>(vc + kQ4Meta + (i & 1) * 64 + t * 16);
     }
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) {
-      const uint8_t* vo = st + pg * (2 * kQ4Chunk) + kQ4Chunk + kQ4VOffsets + t * 16 + (g & 3) * 4;
-      mma_f16_16816(d, pa[pg], *reinterpret_cast<const uint32_t*>(vo), *reinterpret_cast<const uint32_t*>(vo + 64));
+      const uint8_t* vo = st + pg * kQ4Pair + kQ4Chunk + kQ4VOffsets + t * 16 + (g & 3) * 4;
+      const uint32_t b0 = *reinterpret_cast<const uint32_t*>(vo), b1 = *reinterpret_cast<const uint32_t*>(vo + 64);
+      if (pg == 0) mma_f16_16816_z(d, pa[pg], b0, b1);
+      else mma_f16_16816(d, pa[pg], b0, b1);
     }
     oo = f2_fma(oo, al2, f2_pack(d[0], d[1]));
     oo = f2_add(oo, f2_pack(d[2], d[3]));
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       float e[4][4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) e[n][0] = e[n][1] = e[n][2] = e[n][3] = 0.f;
 #pragma unroll
       for (int pg = 0; pg < 2; ++pg) {
         uint32_t b[2][4];  // [half][n]
@@ -347,13 +364,16 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
           const uint32_t s2 = w == 0 ? s4.x : (w == 1 ? s4.y : (w == 2 ? s4.z : s4.w));
           const uint32_t y = x >> 8;
           // 1024 + c, or 1024 + 16 c, to c - 8, times s: every step exact
-          b[h][0] = h2_mul(h2_add((x & 0x000f000fu) | 0x64006400u, 0xe408e408u), s2);
-          b[h][1] = h2_mul(h2_fma((x & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u), s2);
-          b[h][2] = h2_mul(h2_add((y & 0x000f000fu) | 0x64006400u, 0xe408e408u), s2);
-          b[h][3] = h2_mul(h2_fma((y & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u), s2);
+          b[h][0] = h2_mul(h2_add(and_or(x, 0x000f000fu, magic), 0xe408e408u), s2);
+          b[h][1] = h2_mul(h2_fma(and_or(x, 0x00f000f0u, magic), 0x2c002c00u, 0xd480d480u), s2);
+          b[h][2] = h2_mul(h2_add(and_or(y, 0x000f000fu, magic), 0xe408e408u), s2);
+          b[h][3] = h2_mul(h2_fma(and_or(y, 0x00f000f0u, magic), 0x2c002c00u, 0xd480d480u), s2);
         }
 #pragma unroll
-        for (int n = 0; n < 4; ++n) mma_f16_16816(e[n], pa[pg], b[0][n], b[1][n]);
+        for (int n = 0; n < 4; ++n) {
+          if (pg == 0) mma_f16_16816_z(e[n], pa[pg], b[0][n], b[1][n]);
+          else mma_f16_16816(e[n], pa[pg], b[0][n], b[1][n]);
+        }
       }
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
@@ -374,7 +394,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
   consumer_bar();  // every warp is done with its ring
   MergeSmem& ms = *reinterpret_cast<MergeSmem*>(smem_q4);
   if (t == 0) {
-    ms.m[warp][g] = m == -INFINITY ? -INFINITY : m * f2;
+    ms.m[warp][g] = m;
     ms.l[warp][g] = l;
   }
 #pragma unroll

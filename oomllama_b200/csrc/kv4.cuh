@@ -1,8 +1,8 @@
 // The 4-bit KV cache: its format, the quantiser, and the kernel that reads
 // cached rows back as values (of any cache type).
 //
-// A page of 16 tokens of one kv head is one 1280-byte chunk in the K pool and
-// one in the V pool.  The 128 values of a token are four groups of 32; with x
+// A page of 16 tokens of one kv head is a chunk of 1280 bytes of K and, right
+// behind it (one copy brings both), one of V.  The 128 values of a token are four groups of 32; with x
 // the group,
 //   s = f16(bf16((max x - min x) / 15))      (f32 division; 8 significant bits)
 //   o = f16(min x + 8 s)
@@ -33,6 +33,7 @@
 namespace oomattn {
 
 constexpr int kQ4Chunk = 1280;        // bytes of a (page, kv head) chunk of K or of V
+constexpr int kQ4Pair = 2 * kQ4Chunk; // K and V: the step from one (page, kv head) to the next
 constexpr int kQ4Meta = 1024;         // its scales and offsets
 constexpr int kQ4VOffsets = 1152;     // V: the offsets, behind the scales
 constexpr float kQ4Sat = 60000.f;
@@ -76,9 +77,9 @@ __device__ __forceinline__ float q4_value(uint32_t code, float s, float o) {
   return __fadd_rn(o, __fmul_rn((float)((int)code - 8), s));
 }
 
-// Chunk of (layer, page, kv head) in a 4-bit pool.
+// Chunk of (layer, page, kv head) in a 4-bit pool, from pool.k or pool.v.
 __device__ __forceinline__ size_t q4_chunk_off(const KVPool& pool, int layer, int page, int g) {
-  return ((size_t)((size_t)layer * pool.n_pool_pages + page) * pool.n_kv + g) * kQ4Chunk;
+  return ((size_t)((size_t)layer * pool.n_pool_pages + page) * pool.n_kv + g) * kQ4Pair;
 }
 
 // Byte offsets inside a chunk.

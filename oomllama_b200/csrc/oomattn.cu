@@ -241,7 +241,7 @@ int encode_out_map(oomattn_ctx* ctx, void* out, int n_new, bool bf16, CUtensorMa
 KVPool make_pool(const oomattn_ctx* ctx) {
   KVPool p;
   p.k = ctx->kpool;
-  p.v = ctx->vpool;
+  p.v = ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4 ? static_cast<uint8_t*>(ctx->kpool) + kQ4Chunk : ctx->vpool;
   p.block_table = ctx->d_block_table;
   p.max_pages_per_seq = ctx->max_pages_per_seq;
   p.n_pool_pages = ctx->n_pool_pages;
@@ -1040,12 +1040,17 @@ int oomattn_create(const oomattn_config* cfg, int device, void* stream, oomattn_
   };
   if (cudaSetDevice(device) != cudaSuccess) return bail(OOMATTN_ERR_CUDA);
   cudaDeviceGetAttribute(&ctx->num_sms, cudaDevAttrMultiProcessorCount, device);
-  const size_t pool_bytes = c.kv_dtype == OOMATTN_DTYPE_Q4 ? (size_t)(rows / kPageSize) * kQ4Chunk
-                                                           : (size_t)rows * kHeadDim * ctx->esize;
-  if (cudaMalloc(&ctx->kpool, pool_bytes) != cudaSuccess || cudaMalloc(&ctx->vpool, pool_bytes) != cudaSuccess)
-    return bail(OOMATTN_ERR_NO_MEMORY);
-  if (cudaMemset(ctx->kpool, 0, pool_bytes) != cudaSuccess || cudaMemset(ctx->vpool, 0, pool_bytes) != cudaSuccess)
-    return bail(OOMATTN_ERR_CUDA);
+  if (c.kv_dtype == OOMATTN_DTYPE_Q4) {  // one pool, K and V chunks in turn
+    const size_t pool_bytes = (size_t)(rows / kPageSize) * kQ4Pair;
+    if (cudaMalloc(&ctx->kpool, pool_bytes) != cudaSuccess) return bail(OOMATTN_ERR_NO_MEMORY);
+    if (cudaMemset(ctx->kpool, 0, pool_bytes) != cudaSuccess) return bail(OOMATTN_ERR_CUDA);
+  } else {
+    const size_t pool_bytes = (size_t)rows * kHeadDim * ctx->esize;
+    if (cudaMalloc(&ctx->kpool, pool_bytes) != cudaSuccess || cudaMalloc(&ctx->vpool, pool_bytes) != cudaSuccess)
+      return bail(OOMATTN_ERR_NO_MEMORY);
+    if (cudaMemset(ctx->kpool, 0, pool_bytes) != cudaSuccess || cudaMemset(ctx->vpool, 0, pool_bytes) != cudaSuccess)
+      return bail(OOMATTN_ERR_CUDA);
+  }
   const size_t bt_n = (size_t)c.max_seqs * ctx->max_pages_per_seq;
   ctx->h_block_table.assign(bt_n, ctx->n_pool_pages - 1);
   ctx->h_len.assign((size_t)c.n_layers * c.max_seqs, 0);
@@ -1207,8 +1212,9 @@ int oomattn_set_seq_len(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t le
 
 int oomattn_kv_pool(const oomattn_ctx* ctx, void** k_pool, void** v_pool) {
   if (!ctx || !k_pool || !v_pool) return OOMATTN_ERR_INVALID_ARG;
-  *k_pool = ctx->kpool;
-  *v_pool = ctx->vpool;
+  const KVPool pool = make_pool(ctx);
+  *k_pool = pool.k;
+  *v_pool = pool.v;
   return OOMATTN_OK;
 }
 
@@ -1258,9 +1264,8 @@ int oomattn_kv_read(oomattn_ctx* ctx, int32_t layer, int32_t seq, void* k_out, v
       const int nt = std::min(kPageSize, L - lp * kPageSize);
       for (int g = 0; g < n_kv; ++g)
         for (int which = 0; which < 2; ++which) {
-          const size_t off = (((size_t)layer * ctx->n_pool_pages + pg) * n_kv + g) * kQ4Chunk;
-          CK(cudaMemcpy(chunk.data(), (const uint8_t*)(which ? ctx->vpool : ctx->kpool) + off, kQ4Chunk,
-                        cudaMemcpyDeviceToHost));
+          const size_t off = (((size_t)layer * ctx->n_pool_pages + pg) * n_kv + g) * kQ4Pair + which * kQ4Chunk;
+          CK(cudaMemcpy(chunk.data(), (const uint8_t*)ctx->kpool + off, kQ4Chunk, cudaMemcpyDeviceToHost));
           float* dst = (float*)(which ? v_out : k_out) + ((size_t)g * L + (size_t)lp * kPageSize) * kHeadDim;
           for (int r = 0; r < nt; ++r)
             for (int d = 0; d < kHeadDim; ++d) {
@@ -1843,8 +1848,10 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
     return static_fail(errbuf, errbuf_len, OOMATTN_ERR_OUT_OF_RANGE, "pool of %d pages unsupported", n_pool_pages);
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u)
     return static_fail(errbuf, errbuf_len, OOMATTN_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
-  if (kv_dtype == OOMATTN_DTYPE_Q4 && ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15u))
-    return static_fail(errbuf, errbuf_len, OOMATTN_ERR_INVALID_ARG, "the pools must be 16-byte aligned");
+  if (kv_dtype == OOMATTN_DTYPE_Q4 && ((reinterpret_cast<uintptr_t>(k_pool) & 15u) ||
+                                       static_cast<const uint8_t*>(v_pool) != static_cast<const uint8_t*>(k_pool) + kQ4Chunk))
+    return static_fail(errbuf, errbuf_len, OOMATTN_ERR_INVALID_ARG,
+                       "a 4-bit pool must be 16-byte aligned, its V chunks %d bytes behind its K chunks", kQ4Chunk);
   SeqBatch sb;
   sb.n = n_rows;
   for (int z = 0; z < n_rows; ++z) {

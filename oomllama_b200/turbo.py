@@ -193,14 +193,13 @@ class TurboEngine:
 
     def kv_pool(self):
         """(k_pool, v_pool) device tensors [n_layers, n_pages+1, n_kv, 16, 128] aliasing the pools; of a 4-bit cache
-        uint8 [n_layers, n_pages+1, n_kv, Q4_CHUNK] in the layout that include/oomattn.h gives."""
+        uint8 [n_layers, n_pages+1, n_kv, Q4_CHUNK] (views of one pool) in the layout that include/oomattn.h gives."""
         kp, vp = ctypes.c_void_p(), ctypes.c_void_p()
         check(self._ctx, self._L.oomattn_kv_pool(self._ctx, ctypes.byref(kp), ctypes.byref(vp)))
         c = self.config
         if c.kv_dtype == "q4":
-            shape = (c.n_layers, self._n_pages + 1, c.n_kv_heads, _lib.Q4_CHUNK)
-            return (_alias(kp.value, shape, torch.uint8, self.device),
-                    _alias(vp.value, shape, torch.uint8, self.device))
+            shape = (c.n_layers, self._n_pages + 1, c.n_kv_heads, 2, _lib.Q4_CHUNK)
+            return _alias(kp.value, shape, torch.uint8, self.device).unbind(3)
         shape = (c.n_layers, self._n_pages + 1, c.n_kv_heads, PAGE_SIZE, HEAD_DIM)
         dt = torch.bfloat16 if c.kv_dtype == "bf16" else torch.float32
         return _alias(kp.value, shape, dt, self.device), _alias(vp.value, shape, dt, self.device)
