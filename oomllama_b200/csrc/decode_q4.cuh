@@ -11,10 +11,14 @@
 // is a product with the f16 values plus a small one with the offsets, which
 // are one column per group.
 //
-// Tiles.  m16n8k16 with the query heads of the group as rows: rows 0-7 hold
-// the f16 high parts and rows 8-15 the low parts (x - high), so one product
-// carries 22 bits of the f32 query (and probability) and the two halves of an
-// accumulator are added at the end.  K codes enter as subnormal halves (code *
+// Tiles.  m16n8k16 with keys (K) or dims (V) as the 16 rows and four query
+// heads as the 8 columns, column 2 h the f16 high part of head h's query (or
+// probability), column 2 h + 1 the low part (x - high): one product carries 22
+// bits of the f32 value, and the two columns of an accumulator, which lie in
+// one lane, are added at the end.  A group of five to eight heads takes two
+// such column sets (SETS = 2) over the same unpacked rows.  With the heads as
+// rows instead (8 high, 8 low) a group of four would cost as many products as
+// one of eight, and twice the softmax.  K codes enter as subnormal halves (code *
 // 2^-24, or 2^-20 for the upper nibble of a byte, whose q is prescaled by
 // 1/16): unpacking is one AND per two codes.  q is scaled by a power of two to
 // [2^14, 2^15) per head so that its low part keeps its bits.
@@ -37,11 +41,15 @@ namespace oomattn {
 constexpr int kQ4Pages = 2;                              // pages per tile
 constexpr int kQ4Tile = kQ4Pages * kPageSize;            // tokens per tile
 constexpr int kQ4TileBytes = kQ4Pages * kQ4Pair;         // 5 KB
-constexpr int kQ4Stages = 3;
-constexpr int kQ4CtasPerSm = 3;
-constexpr int kQ4RingBytes = kDecWarps * kQ4Stages * kQ4TileBytes;
-constexpr int kQ4SmemBytes = kQ4RingBytes + kDecWarps * kQ4Stages * 8 + 64 + kMaxGroup * 32 * 4;
-static_assert(sizeof(MergeSmem) <= kQ4RingBytes, "the merge is staged over the ring");
+// One column set needs 128 registers and two need 168: four CTAs of two stages
+// each, or three of three, per SM -- about 160 and 180 KB in flight.
+__host__ __device__ constexpr int q4_stages(int sets) { return sets == 1 ? 2 : 3; }
+__host__ __device__ constexpr int q4_ctas_per_sm(int sets) { return sets == 1 ? 4 : 3; }
+__host__ __device__ constexpr int q4_ring_bytes(int sets) { return kDecWarps * q4_stages(sets) * kQ4TileBytes; }
+__host__ __device__ constexpr int q4_smem_bytes(int sets) {
+  return q4_ring_bytes(sets) + kDecWarps * q4_stages(sets) * 8 + 64 + kMaxGroup * 32 * 4;
+}
+static_assert(sizeof(MergeSmem) <= q4_ring_bytes(1), "the merge is staged over the ring");
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -91,10 +99,10 @@ __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t m
 }
 __device__ __forceinline__ float h_lo(uint32_t v) { return __half2float(__ushort_as_half((uint16_t)v)); }
 __device__ __forceinline__ float h_hi(uint32_t v) { return __half2float(__ushort_as_half((uint16_t)(v >> 16))); }
-// (a, b) as f16 pairs hi + lo: lo = x - hi is exact in f32 and rounded once.
-__device__ __forceinline__ void split_f16x2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack_f16(a, b);
-  lo = pack_f16(a - h_lo(hi), b - h_hi(hi));
+// (a, b) rounded to f16, or (low) what that rounding leaves: exact in f32, rounded once.
+__device__ __forceinline__ uint32_t f16_part(float a, float b, bool low) {
+  const uint32_t hi = pack_f16(a, b);
+  return low ? pack_f16(a - h_lo(hi), b - h_hi(hi)) : hi;
 }
 
 // decode.cuh's prefetch_then_wait for 4-bit chunks.
@@ -116,14 +124,15 @@ __device__ __forceinline__ void q4_prefetch_then_wait(const KVPool& pool, const 
 
 // IO16: q and out in bf16 (the newest tokens of a sequence as one row each)
 // instead of f32 (a generation step).
-template <bool IO16>
-__global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
+template <int SETS, bool IO16>
+__global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(SETS))
     decode_q4_kernel(const KVPool pool, const DecodeArgs a, const __grid_constant__ SeqBatch sb,
                      const __grid_constant__ DecodeSched sched) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // as in decode_bf16_kernel
+  constexpr int kStages = q4_stages(SETS), kRing = q4_ring_bytes(SETS);
   extern __shared__ __align__(128) uint8_t smem_q4[];
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_q4 + kQ4RingBytes);
-  int* s_last = reinterpret_cast<int*>(bars + kDecWarps * kQ4Stages);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_q4 + kRing);
+  int* s_last = reinterpret_cast<int*>(bars + kDecWarps * kStages);
   float* s_w = reinterpret_cast<float*>(s_last + 16);  // [kMaxGroup][32] merge weights
 
   const DecodeItem item = decode_item(sched, sb, blockIdx.x);
@@ -137,10 +146,10 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem_q4 + warp * (kQ4Stages * kQ4TileBytes);
-  uint64_t* full = bars + warp * kQ4Stages;
+  uint8_t* ring = smem_q4 + warp * (kStages * kQ4TileBytes);
+  uint64_t* full = bars + warp * kStages;
   if (lane == 0)
-    for (int s = 0; s < kQ4Stages; ++s) mbar_init(&full[s], kQ4Pages);
+    for (int s = 0; s < kStages; ++s) mbar_init(&full[s], kQ4Pages);
   fence_mbar_init();
   __syncwarp();
 
@@ -170,7 +179,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
   const uint32_t page_bytes = (uint32_t)pool.n_kv * kQ4Pair;
   uint8_t* dst0 = ring + (lane & 1) * kQ4Pair;
   const bool drop = (a.test_flags & kTestDropDecodeCopies) != 0;
-  auto issue = [&](int k) {  // all lanes; copies of local tile k into its stage
+  auto issue = [&](int k, int s) {  // all lanes; copies of local tile k into stage s
     const int j = (k * kQ4Pages) & 31;
     if (j == 0 && k > 0) {
       ids = ids_next;
@@ -178,7 +187,6 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
     }
     const int id = __shfl_sync(0xffffffffu, ids, j + (lane & 1));
     if (drop) return;
-    const int s = k % kQ4Stages;
     // each of the two lanes arrives for its own page (a missing second one: no bytes)
     if (lane < kQ4Pages) {
       mbar_arrive_expect_tx(&full[s], id >= 0 ? kQ4Pair : 0);
@@ -186,15 +194,18 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
     }
     issued = k + 1;
   };
-  for (int k = 0; k < min(kQ4Stages, n_tiles); ++k) issue(k);
+  for (int k = 0; k < min(kStages, n_tiles); ++k) issue(k, k);
 
-  // ---- the query as A operand.  Of head g, lane t holds dims 32 w + 8 t + 0..7;
-  // product j of group w takes K nibbles (2j | 2j + 4) and (2j + 1 | 2j + 5) of the word.
-  uint32_t qa[8][4], am[2];
-  float f2;  // score = accumulated * f2, base-2 logits
-  {
-    const bool valid = g < a.group;
-    const size_t q0 = ((size_t)z * a.n_heads + g_kv * a.group + (valid ? g : 0)) * kHeadDim;
+  // ---- the query as B operand: of set u, lane (g, t) holds column g, the high
+  // (g even) or low part of head 4 u + g / 2, at dims 32 w + 8 t + 0..7; product
+  // j of group w meets K nibbles (2j | 2j + 4) and (2j + 1 | 2j + 5) of the word
+  uint32_t qb[SETS][8][2], bm[SETS];
+  float f2[SETS];  // of head 4 u + t: score * f2 is the base-2 logit
+#pragma unroll
+  for (int u = 0; u < SETS; ++u) {
+    const int j = 4 * u + (g >> 1);
+    const bool valid = j < a.group, low = g & 1;
+    const size_t q0 = ((size_t)z * a.n_heads + g_kv * a.group + (valid ? j : 0)) * kHeadDim;
     float x[4][8];
     float mx = 0.f;
 #pragma unroll
@@ -212,8 +223,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
     const int ex = (int)((__float_as_uint(mx) >> 23) & 255u);
     const int e = min(100, max(-100, 14 + 127 - (ex == 0 ? 127 : ex)));
     const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-    // codes enter as code * 2^-24: undo that and 2^e in two exact steps (f2 stays normal)
-    f2 = a.qscale * __uint_as_float((uint32_t)(127 + 24) << 23) * __uint_as_float((uint32_t)(127 - e) << 23);
+    // codes enter as code * 2^-24: undo that and 2^e (both powers of two, f2 stays normal)
+    const float f2_own = a.qscale * __uint_as_float((uint32_t)(127 + 24) << 23) * __uint_as_float((uint32_t)(127 - e) << 23);
+    f2[u] = __shfl_sync(0xffffffffu, f2_own, 8 * t);
     float qs[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -227,33 +239,37 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       qs[w] = sum * (1.f / 4096.f);  // within f16: |sum| < 2^20, times 8 below
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        split_f16x2(x[w][2 * j], x[w][2 * j + 4], qa[2 * w + j][0], qa[2 * w + j][1]);
-        split_f16x2(x[w][2 * j + 1] * 0.0625f, x[w][2 * j + 5] * 0.0625f, qa[2 * w + j][2], qa[2 * w + j][3]);
+      for (int i = 0; i < 2; ++i) {
+        qb[u][2 * w + i][0] = f16_part(x[w][2 * i], x[w][2 * i + 4], low);
+        qb[u][2 * w + i][1] = f16_part(x[w][2 * i + 1] * 0.0625f, x[w][2 * i + 5] * 0.0625f, low);
       }
     }
-    // columns [o0 o1 | o2 o3 | s0 s1 | s2 s3] of the token's stored numbers, lane t has its two
+    // rows [o0 o1 | o2 o3 | s0 s1 | s2 s3] of the token's stored numbers, lane t has its two
     const float u0 = (t & 1) ? qs[2] : qs[0], u1 = (t & 1) ? qs[3] : qs[1];
     const float m8 = t < 2 ? 1.f : -8.f;
-    split_f16x2(u0 * m8, u1 * m8, am[0], am[1]);
+    bm[u] = f16_part(u0 * m8, u1 * m8, low);
   }
 
-  uint64_t o[4][4];  // [group w][n]: head g, dims 32 w + 8 t + n (low) and + 4 (high)
+  uint64_t o[SETS][4][2];  // [group w][i]: head 4 u + t, dims 32 w + 4 g + 2 i and + 1
+  float oo[SETS];          // sum p * offset of group g % 4, head 4 u + t
+  float m[SETS], l[SETS];     // m: the running maximum as a base-2 logit
 #pragma unroll
-  for (int w = 0; w < 4; ++w)
+  for (int u = 0; u < SETS; ++u) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) o[w][n] = 0;
-  uint64_t oo = 0;   // sum p * offset of groups 2 (t & 1), 2 (t & 1) + 1
-  float m = -INFINITY, l = 0.f;
+    for (int w = 0; w < 4; ++w) o[u][w][0] = o[u][w][1] = 0;
+    oo[u] = 0.f;
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+  }
   const int tok_end = min(pe * kPageSize, L);
   uint32_t magic;  // 1024.0 in both halves, in a register
   asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
-  const uint64_t kMetaUnit = f2_pack(1.f / 4096.f, 1.f / 4096.f);  // 2^-24 / 2^-12
 
+  int s = 0;
+  uint32_t phase = 0;
   for (int k = 0; k < n_tiles; ++k) {
-    const int s = k % kQ4Stages;
     // all lanes leave together: the shuffles and products below are the whole warp's
-    if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (k / kQ4Stages) & 1, a.status, a.timeout_ns))) {
+    if (!__all_sync(0xffffffffu, mbar_wait(&full[s], phase, a.status, a.timeout_ns))) {
       gave_up = true;
       break;
     }
@@ -263,9 +279,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
       // the row's (or the split's) last tile: zero the V scales and offsets of the
       // tokens behind the end, which may be stale or never written; their scores
       // become -inf below.  (No copy follows into this stage.)
-      const int tok = lane;
-      if (tok >= lim) {
-        uint8_t* mp = st + (tok >> 4) * kQ4Pair + kQ4Chunk + kQ4Meta + q4_v_meta(tok & 15) + 2 * (tok & 1);
+      if (lane >= lim) {
+        uint8_t* mp = st + (lane >> 4) * kQ4Pair + kQ4Chunk + kQ4Meta + q4_v_meta(lane & 15) + 2 * (lane & 1);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           *reinterpret_cast<uint16_t*>(mp + 4 * w) = 0;
@@ -274,85 +289,104 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
       }
       __syncwarp();
     }
-    // ---- S = q K^T of 32 tokens: n-tile nt = tokens 8 nt .. + 7, lane's are 2t, 2t + 1
-    float sc[8];
+    // ---- scores of 2 x 16 tokens: rows g and g + 8 of a page, head 4 u + t
+    float sc[SETS][4];
 #pragma unroll
-    for (int nt = 0; nt < 4; ++nt) {
-      const uint8_t* kc = st + (nt >> 1) * kQ4Pair;
-      const int h = nt & 1;
-      const uint4 w4 = *reinterpret_cast<const uint4*>(kc + h * 512 + lane * 16);
-      const uint32_t bm = *reinterpret_cast<const uint32_t*>(kc + kQ4Meta + (8 * h + g) * 16 + t * 4);
-      const uint2 s0 = *reinterpret_cast<const uint2*>(kc + kQ4Meta + (8 * h + 2 * t) * 16 + 8);
-      const uint2 s1 = *reinterpret_cast<const uint2*>(kc + kQ4Meta + (8 * h + 2 * t + 1) * 16 + 8);
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-      float d[4];
-      mma_f16_1688_z(d, am[0], am[1], bm);
-      uint64_t acc = f2_fma(f2_pack(d[0], d[1]), kMetaUnit, 0);
-      acc = f2_fma(f2_pack(d[2], d[3]), kMetaUnit, acc);
+    for (int pg = 0; pg < 2; ++pg) {
+      const uint8_t* kc = st + pg * kQ4Pair;
+      const uint4 wa = *reinterpret_cast<const uint4*>(kc + lane * 16);
+      const uint4 wb = *reinterpret_cast<const uint4*>(kc + 512 + lane * 16);
+      const uint32_t am0 = *reinterpret_cast<const uint32_t*>(kc + kQ4Meta + g * 16 + t * 4);
+      const uint32_t am1 = *reinterpret_cast<const uint32_t*>(kc + kQ4Meta + (g + 8) * 16 + t * 4);
+      const uint2 sa = *reinterpret_cast<const uint2*>(kc + kQ4Meta + g * 16 + 8);
+      const uint2 sb2 = *reinterpret_cast<const uint2*>(kc + kQ4Meta + (g + 8) * 16 + 8);
+      float acc[SETS][2];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t x = w[q], y = w[q] >> 8;
-        float e[4];
-        mma_f16_16816_z(e, qa[2 * q], x & 0x000f000fu, x & 0x00f000f0u);
-        mma_f16_16816(e, qa[2 * q + 1], y & 0x000f000fu, y & 0x00f000f0u);
-        const uint32_t a0 = q < 2 ? s0.x : s0.y, a1 = q < 2 ? s1.x : s1.y;
-        const uint64_t sp = (q & 1) ? f2_pack(h_hi(a0), h_hi(a1)) : f2_pack(h_lo(a0), h_lo(a1));
-        acc = f2_fma(f2_pack(e[0], e[1]), sp, acc);
-        acc = f2_fma(f2_pack(e[2], e[3]), sp, acc);
+      for (int u = 0; u < SETS; ++u) {
+        float d[4];
+        mma_f16_1688_z(d, am0, am1, bm[u]);
+        acc[u][0] = (d[0] + d[1]) * (1.f / 4096.f);  // 2^-24 / 2^-12
+        acc[u][1] = (d[2] + d[3]) * (1.f / 4096.f);
       }
-      sc[2 * nt] = f2_lo(acc);
-      sc[2 * nt + 1] = f2_hi(acc);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t xa = w == 0 ? wa.x : (w == 1 ? wa.y : (w == 2 ? wa.z : wa.w));
+        const uint32_t xb = w == 0 ? wb.x : (w == 1 ? wb.y : (w == 2 ? wb.z : wb.w));
+        const uint32_t ya = xa >> 8, yb = xb >> 8;
+        const uint32_t f0[4] = {xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u};
+        const uint32_t f1[4] = {ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u, yb & 0x00f000f0u};
+        const uint32_t ha = w < 2 ? sa.x : sa.y, hb = w < 2 ? sb2.x : sb2.y;
+        const float s0 = (w & 1) ? h_hi(ha) : h_lo(ha), s1 = (w & 1) ? h_hi(hb) : h_lo(hb);
+#pragma unroll
+        for (int u = 0; u < SETS; ++u) {
+          float e[4];
+          mma_f16_16816_z(e, f0, qb[u][2 * w][0], qb[u][2 * w][1]);
+          mma_f16_16816(e, f1, qb[u][2 * w + 1][0], qb[u][2 * w + 1][1]);
+          acc[u][0] = fmaf(e[1], s0, fmaf(e[0], s0, acc[u][0]));
+          acc[u][1] = fmaf(e[3], s1, fmaf(e[2], s1, acc[u][1]));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < SETS; ++u) {
+        sc[u][2 * pg] = acc[u][0];
+        sc[u][2 * pg + 1] = acc[u][1];
+      }
     }
     if (lim < kQ4Tile) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (8 * (i >> 1) + 2 * t + (i & 1) >= lim) sc[i] = -INFINITY;
-    }
-    // ---- online softmax of head g over the tile
-    float mt = fmaxf(max3f(sc[0], sc[1], sc[2]), max3f(sc[3], sc[4], sc[5]));
-    mt = max3f(mt, sc[6], sc[7]);
-    mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-    mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-    // m is the running maximum as a base-2 logit, rounded: the same number in
-    // every weight, so its rounding cancels
-    const float mf = fmaxf(m, mt * f2);
-    const float alpha = ex2_ftz(m - mf);
-    m = mf;
-    float ps = 0.f;
+      for (int i = 0; i < 4; ++i)
+        if (8 * i + g >= lim) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sc[i] = ex2_ftz(fmaf(sc[i], f2, -mf));
-      ps += sc[i];
+          for (int u = 0; u < SETS; ++u) sc[u][i] = -INFINITY;
+        }
     }
-    l = fmaf(l, alpha, ps);
-    uint32_t pa[2][4];  // A operands of the two pages: rows hi, lo x tokens (2t, 2t+1), (8 + 2t, + 1)
+    // ---- online softmax of the lane's heads over the tile
+    uint32_t pb2[SETS][4];  // B operands: (high | low) of tokens 2t, 2t + 1 of each half page, column g
+    float alpha[SETS];
 #pragma unroll
-    for (int pg = 0; pg < 2; ++pg) {
-      split_f16x2(sc[4 * pg], sc[4 * pg + 1], pa[pg][0], pa[pg][1]);
-      split_f16x2(sc[4 * pg + 2], sc[4 * pg + 3], pa[pg][2], pa[pg][3]);
+    for (int u = 0; u < SETS; ++u) {
+      float mt = fmaxf(max3f(sc[u][0], sc[u][1], sc[u][2]), sc[u][3]);
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, off));
+      // the running maximum is rounded: the same number enters every weight, so its rounding cancels
+      const float mf = fmaxf(m[u], mt * f2[u]);
+      alpha[u] = ex2_ftz(m[u] - mf);
+      m[u] = mf;
+      float ps = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = ex2_ftz(fmaf(sc[u][i], f2[u], -mf));
+        ps += p;
+        // token row g, columns (2t, 2t + 1) = (high, low) of the head; transposed: tokens 2t, 2t + 1 of column g
+        pb2[u][i] = movmatrix_trans(pack_f16(p, p - h_lo(pack_f16(p, 0.f))));
+      }
+      l[u] = fmaf(l[u], alpha[u], ps);
     }
-    // ---- O = O * alpha + P V
-    const uint64_t al2 = f2_pack(alpha, alpha);
+    // ---- O = O * alpha + V^T P
     uint4 vw[4], vs[4];  // [page, half]: the four groups' codes and scales of the lane's token pair
-    float d[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint8_t* vc = st + (i >> 1) * kQ4Pair + kQ4Chunk;
       vw[i] = *reinterpret_cast<const uint4*>(vc + (i & 1) * 512 + lane * 16);
       vs[i] = *reinterpret_cast<const uint4*>(vc + kQ4Meta + (i & 1) * 64 + t * 16);
     }
+    uint32_t ao[2][4];  // offsets as A operand: row g (and g + 8) = group g % 4
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) {
       const uint8_t* vo = st + pg * kQ4Pair + kQ4Chunk + kQ4VOffsets + t * 16 + (g & 3) * 4;
-      const uint32_t b0 = *reinterpret_cast<const uint32_t*>(vo), b1 = *reinterpret_cast<const uint32_t*>(vo + 64);
-      if (pg == 0) mma_f16_16816_z(d, pa[pg], b0, b1);
-      else mma_f16_16816(d, pa[pg], b0, b1);
+      ao[pg][0] = ao[pg][1] = *reinterpret_cast<const uint32_t*>(vo);
+      ao[pg][2] = ao[pg][3] = *reinterpret_cast<const uint32_t*>(vo + 64);
     }
-    oo = f2_fma(oo, al2, f2_pack(d[0], d[1]));
-    oo = f2_add(oo, f2_pack(d[2], d[3]));
+#pragma unroll
+    for (int u = 0; u < SETS; ++u) {
+      float d[4];
+      mma_f16_16816_z(d, ao[0], pb2[u][0], pb2[u][1]);
+      mma_f16_16816(d, ao[1], pb2[u][2], pb2[u][3]);
+      oo[u] = fmaf(oo[u], alpha[u], d[0] + d[1]);
+    }
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      float e[4][4];
+      float e[SETS][2][4];
 #pragma unroll
       for (int pg = 0; pg < 2; ++pg) {
         uint32_t b[2][4];  // [half][n]
@@ -370,47 +404,58 @@ __global__ void __launch_bounds__(kDecWarps * 32, kQ4CtasPerSm)
           b[h][3] = h2_mul(h2_fma(and_or(y, 0x00f000f0u, magic), 0x2c002c00u, 0xd480d480u), s2);
         }
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          if (pg == 0) mma_f16_16816_z(e[n], pa[pg], b[0][n], b[1][n]);
-          else mma_f16_16816(e[n], pa[pg], b[0][n], b[1][n]);
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t av[4] = {b[0][2 * i], b[0][2 * i + 1], b[1][2 * i], b[1][2 * i + 1]};
+#pragma unroll
+          for (int u = 0; u < SETS; ++u) {
+            if (pg == 0) mma_f16_16816_z(e[u][i], av, pb2[u][0], pb2[u][1]);
+            else mma_f16_16816(e[u][i], av, pb2[u][2], pb2[u][3]);
+          }
         }
       }
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        o[w][n] = f2_fma(o[w][n], al2, f2_pack(e[n][0], e[n][1]));
-        o[w][n] = f2_add(o[w][n], f2_pack(e[n][2], e[n][3]));
+      for (int u = 0; u < SETS; ++u) {
+        const uint64_t al2 = f2_pack(alpha[u], alpha[u]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          o[u][w][i] = f2_fma(o[u][w][i], al2, f2_pack(e[u][i][0] + e[u][i][1], e[u][i][2] + e[u][i][3]));
+        }
       }
     }
     __syncwarp();  // every lane has read the stage
-    if (k + kQ4Stages < n_tiles) issue(k + kQ4Stages);
+    if (k + kStages < n_tiles) issue(k + kStages, s);
+    if (++s == kStages) {
+      s = 0;
+      phase ^= 1;
+    }
   }
   if (gave_up) {  // the copies that were issued land before the ring is used again
-    for (int k = max(0, issued - kQ4Stages); k < issued; ++k)
-      mbar_wait(&full[k % kQ4Stages], (k / kQ4Stages) & 1, a.status, a.timeout_ns);
+    for (int k = max(0, issued - kStages); k < issued; ++k)
+      mbar_wait(&full[k % kStages], (k / kStages) & 1, a.status, a.timeout_ns);
   }
 
-  l += __shfl_xor_sync(0xffffffffu, l, 1);
-  l += __shfl_xor_sync(0xffffffffu, l, 2);
+#pragma unroll
+  for (int u = 0; u < SETS; ++u)
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) l[u] += __shfl_xor_sync(0xffffffffu, l[u], off);
   consumer_bar();  // every warp is done with its ring
   MergeSmem& ms = *reinterpret_cast<MergeSmem*>(smem_q4);
-  if (t == 0) {
-    ms.m[warp][g] = m;
-    ms.l[warp][g] = l;
-  }
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const int src = (lane & ~3) | (w >> 1);
-    const float olo = __shfl_sync(0xffffffffu, f2_lo(oo), src), ohi = __shfl_sync(0xffffffffu, f2_hi(oo), src);
-    const float off = (w & 1) ? ohi : olo;
-    float* row = &ms.o[warp][g][32 * w + 8 * t];
-    *reinterpret_cast<float4*>(row) =
-        make_float4(f2_lo(o[w][0]) + off, f2_lo(o[w][1]) + off, f2_lo(o[w][2]) + off, f2_lo(o[w][3]) + off);
-    *reinterpret_cast<float4*>(row + 4) =
-        make_float4(f2_hi(o[w][0]) + off, f2_hi(o[w][1]) + off, f2_hi(o[w][2]) + off, f2_hi(o[w][3]) + off);
+  for (int u = 0; u < SETS; ++u) {
+    if (g == 0) {
+      ms.m[warp][4 * u + t] = m[u];
+      ms.l[warp][4 * u + t] = l[u];
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float off = __shfl_sync(0xffffffffu, oo[u], 4 * w + t);
+      *reinterpret_cast<float4*>(&ms.o[warp][4 * u + t][32 * w + 4 * g]) =
+          make_float4(f2_lo(o[u][w][0]) + off, f2_hi(o[u][w][0]) + off, f2_lo(o[u][w][1]) + off, f2_hi(o[u][w][1]) + off);
+    }
   }
   consumer_bar();
   combine_and_store<IO16>(ms, a, z, g_kv, item.split, item.nsplit, pool.n_kv, threadIdx.x, s_last,
-                    reinterpret_cast<float*>(smem_q4), kQ4RingBytes / 4, s_w);
+                          reinterpret_cast<float*>(smem_q4), kRing / 4, s_w);
 }
 
 }  // namespace oomattn

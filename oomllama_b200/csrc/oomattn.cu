@@ -36,7 +36,24 @@ static_assert((int)kKvF32 == OOMATTN_DTYPE_F32 && (int)kKvBf16 == OOMATTN_DTYPE_
 
 int split_cap(int kv_dtype) { return kv_dtype == OOMATTN_DTYPE_F32 ? kMaxSplits : kMaxSplitsBf16; }
 // Resident decode CTAs per SM, and the fixed cost of one in pages (plan_decode), by cache type.
-int decode_slots(int kv_dtype) { return kv_dtype == OOMATTN_DTYPE_Q4 ? kQ4CtasPerSm : kDecCtasPerSm; }
+int q4_sets(int group) { return group <= 4 ? 1 : 2; }  // column sets of the 4-bit decode: four heads each
+int decode_slots(int kv_dtype, int group) {
+  return kv_dtype == OOMATTN_DTYPE_Q4 ? q4_ctas_per_sm(q4_sets(group)) : kDecCtasPerSm;
+}
+typedef void (*DecodeQ4Fn)(const KVPool, const DecodeArgs, const SeqBatch, const DecodeSched);
+DecodeQ4Fn decode_q4_fn(int sets, bool io16) {
+  if (sets == 1) return io16 ? decode_q4_kernel<1, true> : decode_q4_kernel<1, false>;
+  return io16 ? decode_q4_kernel<2, true> : decode_q4_kernel<2, false>;
+}
+cudaError_t set_decode_q4_smem() {
+  cudaError_t e = cudaSuccess;
+  for (int sets = 1; sets <= 2; ++sets)
+    for (int io16 = 0; io16 < 2; ++io16)
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(decode_q4_fn(sets, io16), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 q4_smem_bytes(sets));
+  return e;
+}
 static_assert(kMaxGroup * kMaxSplits <= kDecWarps * kMaxGroup * kMergeStride,
               "the f32 decode merge stages [group][splits] lse values over the per-warp O area");
 constexpr unsigned long long kDefaultTimeoutNs = 2000000000ull;  // bounded device waits: 2 s
@@ -778,7 +795,7 @@ int plan_decode(const SeqBatch& sb, int n_kv, int slots, int max_splits, int fil
 int launch_decode_rows(oomattn_ctx* ctx, int layer, const SeqBatch& sb, const float* q, float* out, float* lse,
                        int o_stride, int lse_stride, bool io16 = false) {
   const int n_kv = ctx->cfg.n_kv_heads;
-  const int slots = ctx->num_sms * decode_slots(ctx->cfg.kv_dtype);
+  const int slots = ctx->num_sms * decode_slots(ctx->cfg.kv_dtype, ctx->group);
   int key[kMaxBatch + 1];
   key[0] = sb.n;
   for (int z = 0; z < sb.n; ++z) key[z + 1] = sb.len[z] > 0 ? (sb.len[z] + kPageSize - 1) / kPageSize : 0;
@@ -825,8 +842,8 @@ int launch_decode_rows(oomattn_ctx* ctx, int layer, const SeqBatch& sb, const fl
     le = cudaLaunchKernelEx(&cfg, decode_bf16_kernel, ctx->kmap, ctx->vmap, pool, a, sb, sched);
   } else if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4) {
     cfg.blockDim = dim3(kDecWarps * 32);
-    cfg.dynamicSmemBytes = kQ4SmemBytes;
-    le = cudaLaunchKernelEx(&cfg, io16 ? decode_q4_kernel<true> : decode_q4_kernel<false>, pool, a, sb, sched);
+    cfg.dynamicSmemBytes = q4_smem_bytes(q4_sets(ctx->group));
+    le = cudaLaunchKernelEx(&cfg, decode_q4_fn(q4_sets(ctx->group), io16), pool, a, sb, sched);
   } else {
     cfg.blockDim = dim3(kDecWarps * 32);
     le = cudaLaunchKernelEx(&cfg, decode_f32_kernel, pool, a, sb, sched);
@@ -1083,10 +1100,7 @@ int oomattn_create(const oomattn_config* cfg, int device, void* stream, oomattn_
   }
   if (cudaFuncSetAttribute(decode_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmemBytes) !=
           cudaSuccess ||
-      cudaFuncSetAttribute(decode_q4_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4SmemBytes) !=
-          cudaSuccess ||
-      cudaFuncSetAttribute(decode_q4_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4SmemBytes) !=
-          cudaSuccess ||
+      set_decode_q4_smem() != cudaSuccess ||
       cudaFuncSetAttribute(prefill_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPfSmemBytes) !=
           cudaSuccess ||
       cudaFuncSetAttribute(q8_linear_xs_kernel<2, 2, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1881,7 +1895,7 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
         return static_fail(errbuf, errbuf_len, OOMATTN_ERR_CUDA, "cudaGetSymbolAddress: %s", cudaGetErrorString(e));
       e = cudaFuncSetAttribute(decode_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmemBytes);
       if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(decode_q4_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4SmemBytes);
+        e = set_decode_q4_smem();
       if (e != cudaSuccess)
         return static_fail(errbuf, errbuf_len, OOMATTN_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       g_static_scratch[device] = p;
@@ -1900,7 +1914,7 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
   // partial fits the static array: nsplit <= slots / (rows * heads).
   const int cap_splits = std::max(1, std::min(split_cap(kv_dtype), kStaticPartSlots / (n_rows * n_heads)));
   DecodeSched sched;
-  const int n_items = plan_decode(sb, n_kv_heads, num_sms * decode_slots(kv_dtype), cap_splits,
+  const int n_items = plan_decode(sb, n_kv_heads, num_sms * decode_slots(kv_dtype, n_heads / n_kv_heads), cap_splits,
                                   decode_fill(kv_dtype), sched);
   if (n_items == 0) return OOMATTN_OK;
 
@@ -1955,7 +1969,8 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
     }
     decode_bf16_kernel<<<n_items, (kDecWarps + 1) * 32, kDecSmemBytes, st>>>(maps[0], maps[1], pool, a, sb, sched);
   } else if (kv_dtype == OOMATTN_DTYPE_Q4) {
-    decode_q4_kernel<false><<<n_items, kDecWarps * 32, kQ4SmemBytes, st>>>(pool, a, sb, sched);
+    const int sets = q4_sets(n_heads / n_kv_heads);
+    decode_q4_fn(sets, false)<<<n_items, kDecWarps * 32, q4_smem_bytes(sets), st>>>(pool, a, sb, sched);
   } else {
     decode_f32_kernel<<<n_items, kDecWarps * 32, 0, st>>>(pool, a, sb, sched);
   }
