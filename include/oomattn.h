@@ -68,10 +68,10 @@ enum { OOMATTN_DTYPE_F32 = 0, OOMATTN_DTYPE_BF16 = 1, OOMATTN_DTYPE_Q4 = 2 };
  * and, right behind it, one of V: one pool, whose chunk of K (layer, page, kv)
  * lies at ((layer*(n_pages+1) + page)*n_kv + kv) * 2 * OOMATTN_Q4_CHUNK.
  *   K: token r, dims 32w + 8t + n (w, t < 4, n < 8): nibble n of the 32-bit
- *      word at 64r + 16t + 4w; f16 o[0..3], s[0..3] at 1024 + 16r.
+ *      word at 512(w/2) + 32r + 8t + 4(w%2); f16 o[0..3], s[0..3] at 1024 + 16r.
  *   V: token r = 8h + 2t + p (p < 2), dims 32w + 4g + n (g < 8, n < 4): nibble
- *      n of the 16-bit piece at 512h + 64g + 16t + 4w + 2p; f16 s at
- *      1024 + 64h + 16t + 4w + 2p, f16 o 128 bytes behind it. */
+ *      n of the 16-bit piece at 512(w/2) + 256h + 32g + 8t + 4(w%2) + 2p; f16 s
+ *      at 1024 + 64h + 16t + 4w + 2p, f16 o 128 bytes behind it. */
 #define OOMATTN_Q4_CHUNK 1280
 /* Floats per (row, q head) in the packed decode output: O in [0, 128), the
  * natural-log LSE at 128, 3 floats of padding (16-byte aligned rows). */

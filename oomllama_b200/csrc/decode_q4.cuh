@@ -11,14 +11,16 @@
 // is a product with the f16 values plus a small one with the offsets, which
 // are one column per group.
 //
-// Tiles.  m16n8k16 with keys (K) or dims (V) as the 16 rows and four query
-// heads as the 8 columns, column 2 h the f16 high part of head h's query (or
-// probability), column 2 h + 1 the low part (x - high): one product carries 22
-// bits of the f32 value, and the two columns of an accumulator, which lie in
-// one lane, are added at the end.  A group of five to eight heads takes two
-// such column sets (SETS = 2) over the same unpacked rows.  With the heads as
-// rows instead (8 high, 8 low) a group of four would cost as many products as
-// one of eight, and twice the softmax.  K codes enter as subnormal halves (code *
+// Tiles.  m16n8k16 with keys (K) or dims (V) as the 16 rows and query heads as
+// the 8 columns; a query (or probability) enters as an f16 high part and a low
+// one (x - high), 22 bits of the f32 value together.  A group of up to four
+// heads (WIDE = false) has both parts side by side, column 2 h the high part
+// of head h, column 2 h + 1 the low: one product does both, and the two
+// columns of an accumulator lie in one lane.  A group of five to eight (WIDE)
+// has a column per head and adds the low parts' product onto the high parts'.
+// (Heads as rows, eight high and eight low, would cost a group of four as many
+// products as one of eight: 96.2 instead of 66.7 us for 8 x 32768 tokens of
+// 32q/8kv.)  K codes enter as subnormal halves (code *
 // 2^-24, or 2^-20 for the upper nibble of a byte, whose q is prescaled by
 // 1/16): unpacking is one AND per two codes.  q is scaled by a power of two to
 // [2^14, 2^15) per head so that its low part keeps its bits.
@@ -41,15 +43,19 @@ namespace oomattn {
 constexpr int kQ4Pages = 2;                              // pages per tile
 constexpr int kQ4Tile = kQ4Pages * kPageSize;            // tokens per tile
 constexpr int kQ4TileBytes = kQ4Pages * kQ4Pair;         // 5 KB
-// One column set needs 128 registers and two need 168: four CTAs of two stages
-// each, or three of three, per SM -- about 160 and 180 KB in flight.
-__host__ __device__ constexpr int q4_stages(int sets) { return sets == 1 ? 2 : 3; }
-__host__ __device__ constexpr int q4_ctas_per_sm(int sets) { return sets == 1 ? 4 : 3; }
-__host__ __device__ constexpr int q4_ring_bytes(int sets) { return kDecWarps * q4_stages(sets) * kQ4TileBytes; }
-__host__ __device__ constexpr int q4_smem_bytes(int sets) {
-  return q4_ring_bytes(sets) + kDecWarps * q4_stages(sets) * 8 + 64 + kMaxGroup * 32 * 4;
+// The narrow form fits 128 registers and the wide one 168: four CTAs of two
+// stages each, or three of three, per SM -- about 160 and 180 KB in flight.
+__host__ __device__ constexpr int q4_stages(bool wide) { return !wide ? 2 : 3; }
+__host__ __device__ constexpr int q4_ctas_per_sm(bool wide) { return !wide ? 4 : 3; }
+__host__ __device__ constexpr int q4_ring_bytes(bool wide) { return kDecWarps * q4_stages(wide) * kQ4TileBytes; }
+__host__ __device__ constexpr int q4_tail_bytes(bool wide) {  // barriers, a flag, merge weights
+  return kDecWarps * q4_stages(wide) * 8 + 64 + kMaxGroup * 32 * 4;
 }
-static_assert(sizeof(MergeSmem) <= q4_ring_bytes(1), "the merge is staged over the ring");
+__host__ __device__ constexpr int q4_smem_bytes(bool wide) {  // and the query
+  return q4_ring_bytes(wide) + q4_tail_bytes(wide) + (wide ? 4096 : 2048);
+}
+static_assert(q4_tail_bytes(false) % 16 == 0 && q4_tail_bytes(true) % 16 == 0, "the query's alignment");
+static_assert(sizeof(MergeSmem) <= q4_ring_bytes(false), "the merge is staged over the ring");
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -62,6 +68,12 @@ __device__ __forceinline__ void mma_f16_16816(float* d, const uint32_t* a, uint3
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_1688(float* d, uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm(
+      "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0));
 }
 // The same from zero: the accumulator's registers need no clearing.
 __device__ __forceinline__ void mma_f16_16816_z(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -124,16 +136,17 @@ __device__ __forceinline__ void q4_prefetch_then_wait(const KVPool& pool, const 
 
 // IO16: q and out in bf16 (the newest tokens of a sequence as one row each)
 // instead of f32 (a generation step).
-template <int SETS, bool IO16>
-__global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(SETS))
+template <bool WIDE, bool IO16>
+__global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
     decode_q4_kernel(const KVPool pool, const DecodeArgs a, const __grid_constant__ SeqBatch sb,
                      const __grid_constant__ DecodeSched sched) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // as in decode_bf16_kernel
-  constexpr int kStages = q4_stages(SETS), kRing = q4_ring_bytes(SETS);
+  constexpr int kStages = q4_stages(WIDE), kRing = q4_ring_bytes(WIDE);
   extern __shared__ __align__(128) uint8_t smem_q4[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem_q4 + kRing);
   int* s_last = reinterpret_cast<int*>(bars + kDecWarps * kStages);
   float* s_w = reinterpret_cast<float*>(s_last + 16);  // [kMaxGroup][32] merge weights
+  uint4* s_q = reinterpret_cast<uint4*>(smem_q4 + kRing + q4_tail_bytes(WIDE));  // [4][parts][32]: the query
 
   const DecodeItem item = decode_item(sched, sb, blockIdx.x);
   const int g_kv = item.g, z = item.z;
@@ -144,7 +157,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(SETS))
     if (!IO16 && L <= 0 && item.split == 0) write_empty_row(a, z, g_kv);  // a bf16 row sees its own token at least
     return;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  int lane;  // kept in a register
+  asm volatile("mov.u32 %0, %%laneid;" : "=r"(lane));
   const int g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem_q4 + warp * (kStages * kQ4TileBytes);
   uint64_t* full = bars + warp * kStages;
@@ -196,15 +211,16 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(SETS))
   };
   for (int k = 0; k < min(kStages, n_tiles); ++k) issue(k, k);
 
-  // ---- the query as B operand: of set u, lane (g, t) holds column g, the high
-  // (g even) or low part of head 4 u + g / 2, at dims 32 w + 8 t + 0..7; product
-  // j of group w meets K nibbles (2j | 2j + 4) and (2j + 1 | 2j + 5) of the word
-  uint32_t qb[SETS][8][2], bm[SETS];
-  float f2[SETS];  // of head 4 u + t: score * f2 is the base-2 logit
-#pragma unroll
-  for (int u = 0; u < SETS; ++u) {
-    const int j = 4 * u + (g >> 1);
-    const bool valid = j < a.group, low = g & 1;
+  // ---- the query as B operand: lane (g, t) holds column g at dims 32 w + 8 t +
+  // 0..7; product j of group w meets K nibbles (2j | 2j + 4) and (2j + 1 | 2j + 5)
+  // of the word.  Wide: both parts of head g.  Narrow: a part of head g / 2.
+  constexpr int HL = WIDE ? 2 : 1;  // heads of a lane's accumulators: 2 t and 2 t + 1, or t
+  // It stays in shared memory (one copy for the CTA's warps) and is read per tile.
+  uint32_t bm[HL];
+  float f2[HL];  // score * f2 is the base-2 logit
+  {
+    const int j = WIDE ? g : g >> 1;
+    const bool valid = j < a.group;
     const size_t q0 = ((size_t)z * a.n_heads + g_kv * a.group + (valid ? j : 0)) * kHeadDim;
     float x[4][8];
     float mx = 0.f;
@@ -225,7 +241,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(SETS))
     const float up = __uint_as_float((uint32_t)(127 + e) << 23);
     // codes enter as code * 2^-24: undo that and 2^e (both powers of two, f2 stays normal)
     const float f2_own = a.qscale * __uint_as_float((uint32_t)(127 + 24) << 23) * __uint_as_float((uint32_t)(127 - e) << 23);
-    f2[u] = __shfl_sync(0xffffffffu, f2_own, 8 * t);
+#pragma unroll
+    for (int h = 0; h < HL; ++h) f2[h] = __shfl_sync(0xffffffffu, f2_own, 8 * t + 4 * h);
     float qs[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -238,28 +255,41 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(SETS))
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       qs[w] = sum * (1.f / 4096.f);  // within f16: |sum| < 2^20, times 8 below
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        qb[u][2 * w + i][0] = f16_part(x[w][2 * i], x[w][2 * i + 4], low);
-        qb[u][2 * w + i][1] = f16_part(x[w][2 * i + 1] * 0.0625f, x[w][2 * i + 5] * 0.0625f, low);
-      }
     }
     // rows [o0 o1 | o2 o3 | s0 s1 | s2 s3] of the token's stored numbers, lane t has its two
-    const float u0 = (t & 1) ? qs[2] : qs[0], u1 = (t & 1) ? qs[3] : qs[1];
     const float m8 = t < 2 ? 1.f : -8.f;
-    bm[u] = f16_part(u0 * m8, u1 * m8, low);
+    const float u0 = ((t & 1) ? qs[2] : qs[0]) * m8, u1 = ((t & 1) ? qs[3] : qs[1]) * m8;
+#pragma unroll
+    for (int h = 0; h < HL; ++h) {
+      const bool low = WIDE ? h == 1 : (g & 1) != 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          v[2 * i] = f16_part(x[w][2 * i], x[w][2 * i + 4], low);
+          v[2 * i + 1] = f16_part(x[w][2 * i + 1] * 0.0625f, x[w][2 * i + 5] * 0.0625f, low);
+        }
+        if (warp == 0) s_q[(w * HL + h) * 32 + lane] = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+      bm[h] = f16_part(u0, u1, low);
+    }
+    consumer_bar();
   }
 
-  uint64_t o[SETS][4][2];  // [group w][i]: head 4 u + t, dims 32 w + 4 g + 2 i and + 1
-  float oo[SETS];          // sum p * offset of group g % 4, head 4 u + t
-  float m[SETS], l[SETS];     // m: the running maximum as a base-2 logit
+  // O of the lane: dims 32 w + 4 g + 2 i + r.  Wide: [w][2 i + r] of heads (2 t, 2 t + 1);
+  // narrow: [w][i] of head t, r = 0 and 1.  oo: sum p * offset of groups 2 (g % 2) and + 1.
+  uint64_t o[4][2 * HL];
+  float oo[HL][2], m[HL], l[HL];  // m: the running maximum as a base-2 logit
 #pragma unroll
-  for (int u = 0; u < SETS; ++u) {
+  for (int w = 0; w < 4; ++w)
 #pragma unroll
-    for (int w = 0; w < 4; ++w) o[u][w][0] = o[u][w][1] = 0;
-    oo[u] = 0.f;
-    m[u] = -INFINITY;
-    l[u] = 0.f;
+    for (int i = 0; i < 2 * HL; ++i) o[w][i] = 0;
+#pragma unroll
+  for (int h = 0; h < HL; ++h) {
+    oo[h][0] = oo[h][1] = 0.f;
+    m[h] = -INFINITY;
+    l[h] = 0.f;
   }
   const int tok_end = min(pe * kPageSize, L);
   uint32_t magic;  // 1024.0 in both halves, in a register
@@ -289,47 +319,57 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(SETS))
       }
       __syncwarp();
     }
-    // ---- scores of 2 x 16 tokens: rows g and g + 8 of a page, head 4 u + t
-    float sc[SETS][4];
+    // ---- scores of 2 x 16 tokens: rows g and g + 8 of a page, the lane's heads
+    float sc[HL][4];
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) {
       const uint8_t* kc = st + pg * kQ4Pair;
-      const uint4 wa = *reinterpret_cast<const uint4*>(kc + lane * 16);
-      const uint4 wb = *reinterpret_cast<const uint4*>(kc + 512 + lane * 16);
       const uint32_t am0 = *reinterpret_cast<const uint32_t*>(kc + kQ4Meta + g * 16 + t * 4);
       const uint32_t am1 = *reinterpret_cast<const uint32_t*>(kc + kQ4Meta + (g + 8) * 16 + t * 4);
-      const uint2 sa = *reinterpret_cast<const uint2*>(kc + kQ4Meta + g * 16 + 8);
-      const uint2 sb2 = *reinterpret_cast<const uint2*>(kc + kQ4Meta + (g + 8) * 16 + 8);
-      float acc[SETS][2];
+      float d[4];
+      mma_f16_1688_z(d, am0, am1, bm[0]);
+      if (WIDE) {
+        mma_f16_1688(d, am0, am1, bm[HL - 1]);
+        sc[0][2 * pg] = d[0] * (1.f / 4096.f);  // 2^-24 / 2^-12
+        sc[HL - 1][2 * pg] = d[1] * (1.f / 4096.f);
+        sc[0][2 * pg + 1] = d[2] * (1.f / 4096.f);
+        sc[HL - 1][2 * pg + 1] = d[3] * (1.f / 4096.f);
+      } else {
+        sc[0][2 * pg] = (d[0] + d[1]) * (1.f / 4096.f);
+        sc[0][2 * pg + 1] = (d[2] + d[3]) * (1.f / 4096.f);
+      }
+    }
 #pragma unroll
-      for (int u = 0; u < SETS; ++u) {
-        float d[4];
-        mma_f16_1688_z(d, am0, am1, bm[u]);
-        acc[u][0] = (d[0] + d[1]) * (1.f / 4096.f);  // 2^-24 / 2^-12
-        acc[u][1] = (d[2] + d[3]) * (1.f / 4096.f);
+    for (int wp = 0; wp < 2; ++wp) {  // two groups at a time: 64-bit loads of rows g and g + 8
+      uint2 wk[4];
+      uint32_t sk[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* kc = st + (i >> 1) * kQ4Pair;
+        wk[i] = *reinterpret_cast<const uint2*>(kc + wp * 512 + (i & 1) * 256 + lane * 8);
+        sk[i] = *reinterpret_cast<const uint32_t*>(kc + kQ4Meta + (g + 8 * (i & 1)) * 16 + 8 + wp * 4);
       }
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t xa = w == 0 ? wa.x : (w == 1 ? wa.y : (w == 2 ? wa.z : wa.w));
-        const uint32_t xb = w == 0 ? wb.x : (w == 1 ? wb.y : (w == 2 ? wb.z : wb.w));
-        const uint32_t ya = xa >> 8, yb = xb >> 8;
-        const uint32_t f0[4] = {xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u};
-        const uint32_t f1[4] = {ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u, yb & 0x00f000f0u};
-        const uint32_t ha = w < 2 ? sa.x : sa.y, hb = w < 2 ? sb2.x : sb2.y;
-        const float s0 = (w & 1) ? h_hi(ha) : h_lo(ha), s1 = (w & 1) ? h_hi(hb) : h_lo(hb);
+      for (int wl = 0; wl < 2; ++wl) {
+        const int w = 2 * wp + wl;
+        const uint4 q0 = s_q[w * HL * 32 + lane], q1 = s_q[(w * HL + HL - 1) * 32 + lane];
 #pragma unroll
-        for (int u = 0; u < SETS; ++u) {
+        for (int pg = 0; pg < 2; ++pg) {
+          const uint32_t xa = wl ? wk[2 * pg].y : wk[2 * pg].x, xb = wl ? wk[2 * pg + 1].y : wk[2 * pg + 1].x;
+          const uint32_t ya = xa >> 8, yb = xb >> 8;
+          const uint32_t f0[4] = {xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u};
+          const uint32_t f1[4] = {ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u, yb & 0x00f000f0u};
+          const float s0 = wl ? h_hi(sk[2 * pg]) : h_lo(sk[2 * pg]), s1 = wl ? h_hi(sk[2 * pg + 1]) : h_lo(sk[2 * pg + 1]);
           float e[4];
-          mma_f16_16816_z(e, f0, qb[u][2 * w][0], qb[u][2 * w][1]);
-          mma_f16_16816(e, f1, qb[u][2 * w + 1][0], qb[u][2 * w + 1][1]);
-          acc[u][0] = fmaf(e[1], s0, fmaf(e[0], s0, acc[u][0]));
-          acc[u][1] = fmaf(e[3], s1, fmaf(e[2], s1, acc[u][1]));
+          mma_f16_16816_z(e, f0, q0.x, q0.y);
+          if (WIDE) mma_f16_16816(e, f0, q1.x, q1.y);
+          mma_f16_16816(e, f1, q0.z, q0.w);
+          if (WIDE) mma_f16_16816(e, f1, q1.z, q1.w);
+          sc[0][2 * pg] = fmaf(e[0], s0, sc[0][2 * pg]);
+          sc[HL - 1][2 * pg] = fmaf(e[1], s0, sc[HL - 1][2 * pg]);
+          sc[0][2 * pg + 1] = fmaf(e[2], s1, sc[0][2 * pg + 1]);
+          sc[HL - 1][2 * pg + 1] = fmaf(e[3], s1, sc[HL - 1][2 * pg + 1]);
         }
-      }
-#pragma unroll
-      for (int u = 0; u < SETS; ++u) {
-        sc[u][2 * pg] = acc[u][0];
-        sc[u][2 * pg + 1] = acc[u][1];
       }
     }
     if (lim < kQ4Tile) {
@@ -337,88 +377,107 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(SETS))
       for (int i = 0; i < 4; ++i)
         if (8 * i + g >= lim) {
 #pragma unroll
-          for (int u = 0; u < SETS; ++u) sc[u][i] = -INFINITY;
+          for (int h = 0; h < HL; ++h) sc[h][i] = -INFINITY;
         }
     }
     // ---- online softmax of the lane's heads over the tile
-    uint32_t pb2[SETS][4];  // B operands: (high | low) of tokens 2t, 2t + 1 of each half page, column g
-    float alpha[SETS];
+    float alpha[HL];
 #pragma unroll
-    for (int u = 0; u < SETS; ++u) {
-      float mt = fmaxf(max3f(sc[u][0], sc[u][1], sc[u][2]), sc[u][3]);
+    for (int h = 0; h < HL; ++h) {
+      float mt = fmaxf(max3f(sc[h][0], sc[h][1], sc[h][2]), sc[h][3]);
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, off));
       // the running maximum is rounded: the same number enters every weight, so its rounding cancels
-      const float mf = fmaxf(m[u], mt * f2[u]);
-      alpha[u] = ex2_ftz(m[u] - mf);
-      m[u] = mf;
+      const float mf = fmaxf(m[h], mt * f2[h]);
+      alpha[h] = ex2_ftz(m[h] - mf);
+      m[h] = mf;
       float ps = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = ex2_ftz(fmaf(sc[u][i], f2[u], -mf));
-        ps += p;
-        // token row g, columns (2t, 2t + 1) = (high, low) of the head; transposed: tokens 2t, 2t + 1 of column g
-        pb2[u][i] = movmatrix_trans(pack_f16(p, p - h_lo(pack_f16(p, 0.f))));
+        sc[h][i] = ex2_ftz(fmaf(sc[h][i], f2[h], -mf));
+        ps += sc[h][i];
       }
-      l[u] = fmaf(l[u], alpha[u], ps);
+      l[h] = fmaf(l[h], alpha[h], ps);
     }
-    // ---- O = O * alpha + V^T P
-    uint4 vw[4], vs[4];  // [page, half]: the four groups' codes and scales of the lane's token pair
+    // as B operands: token row g, columns (2 t, 2 t + 1), transposed into tokens 2 t, 2 t + 1 of column g
+    uint32_t pb[HL][4];  // wide: high, low; narrow: both in one
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint8_t* vc = st + (i >> 1) * kQ4Pair + kQ4Chunk;
-      vw[i] = *reinterpret_cast<const uint4*>(vc + (i & 1) * 512 + lane * 16);
-      vs[i] = *reinterpret_cast<const uint4*>(vc + kQ4Meta + (i & 1) * 64 + t * 16);
+      if (WIDE) {
+        const uint32_t hi = pack_f16(sc[0][i], sc[HL - 1][i]);
+        pb[0][i] = movmatrix_trans(hi);
+        pb[HL - 1][i] = movmatrix_trans(pack_f16(sc[0][i] - h_lo(hi), sc[HL - 1][i] - h_hi(hi)));
+      } else {
+        pb[0][i] = movmatrix_trans(pack_f16(sc[0][i], sc[0][i] - h_lo(pack_f16(sc[0][i], 0.f))));
+      }
     }
-    uint32_t ao[2][4];  // offsets as A operand: row g (and g + 8) = group g % 4
-#pragma unroll
-    for (int pg = 0; pg < 2; ++pg) {
-      const uint8_t* vo = st + pg * kQ4Pair + kQ4Chunk + kQ4VOffsets + t * 16 + (g & 3) * 4;
-      ao[pg][0] = ao[pg][1] = *reinterpret_cast<const uint32_t*>(vo);
-      ao[pg][2] = ao[pg][3] = *reinterpret_cast<const uint32_t*>(vo + 64);
-    }
-#pragma unroll
-    for (int u = 0; u < SETS; ++u) {
+    // ---- O = O * alpha + V^T P
+    {
       float d[4];
-      mma_f16_16816_z(d, ao[0], pb2[u][0], pb2[u][1]);
-      mma_f16_16816(d, ao[1], pb2[u][2], pb2[u][3]);
-      oo[u] = fmaf(oo[u], alpha[u], d[0] + d[1]);
-    }
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      float e[SETS][2][4];
 #pragma unroll
       for (int pg = 0; pg < 2; ++pg) {
-        uint32_t b[2][4];  // [half][n]
+        // offsets as A operand: row g is group 2 (g % 2), row g + 8 the one after
+        const uint8_t* vo = st + pg * kQ4Pair + kQ4Chunk + kQ4VOffsets + t * 16 + (g & 1) * 8;
+        const uint2 o0 = *reinterpret_cast<const uint2*>(vo), o1 = *reinterpret_cast<const uint2*>(vo + 64);
+        const uint32_t ao[4] = {o0.x, o0.y, o1.x, o1.y};
+        if (pg == 0) mma_f16_16816_z(d, ao, pb[0][0], pb[0][1]);
+        else mma_f16_16816(d, ao, pb[0][2], pb[0][3]);
+        if (WIDE) mma_f16_16816(d, ao, pb[HL - 1][2 * pg], pb[HL - 1][2 * pg + 1]);
+      }
+      if (WIDE) {
+        oo[0][0] = fmaf(oo[0][0], alpha[0], d[0]);
+        oo[HL - 1][0] = fmaf(oo[HL - 1][0], alpha[HL - 1], d[1]);
+        oo[0][1] = fmaf(oo[0][1], alpha[0], d[2]);
+        oo[HL - 1][1] = fmaf(oo[HL - 1][1], alpha[HL - 1], d[3]);
+      } else {
+        oo[0][0] = fmaf(oo[0][0], alpha[0], d[0] + d[1]);
+        oo[0][1] = fmaf(oo[0][1], alpha[0], d[2] + d[3]);
+      }
+    }
+    const uint64_t al2 = f2_pack(alpha[0], alpha[HL - 1]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4& c4 = vw[2 * pg + h];
-          const uint4& s4 = vs[2 * pg + h];
-          const uint32_t x = w == 0 ? c4.x : (w == 1 ? c4.y : (w == 2 ? c4.z : c4.w));
-          const uint32_t s2 = w == 0 ? s4.x : (w == 1 ? s4.y : (w == 2 ? s4.z : s4.w));
-          const uint32_t y = x >> 8;
-          // 1024 + c, or 1024 + 16 c, to c - 8, times s: every step exact
-          b[h][0] = h2_mul(h2_add(and_or(x, 0x000f000fu, magic), 0xe408e408u), s2);
-          b[h][1] = h2_mul(h2_fma(and_or(x, 0x00f000f0u, magic), 0x2c002c00u, 0xd480d480u), s2);
-          b[h][2] = h2_mul(h2_add(and_or(y, 0x000f000fu, magic), 0xe408e408u), s2);
-          b[h][3] = h2_mul(h2_fma(and_or(y, 0x00f000f0u, magic), 0x2c002c00u, 0xd480d480u), s2);
-        }
+    for (int wp = 0; wp < 2; ++wp) {
+      uint2 vw[4], vs[4];  // [page, half]: two groups' codes and scales of the lane's token pair
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t av[4] = {b[0][2 * i], b[0][2 * i + 1], b[1][2 * i], b[1][2 * i + 1]};
-#pragma unroll
-          for (int u = 0; u < SETS; ++u) {
-            if (pg == 0) mma_f16_16816_z(e[u][i], av, pb2[u][0], pb2[u][1]);
-            else mma_f16_16816(e[u][i], av, pb2[u][2], pb2[u][3]);
-          }
-        }
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* vc = st + (i >> 1) * kQ4Pair + kQ4Chunk;
+        vw[i] = *reinterpret_cast<const uint2*>(vc + wp * 512 + (i & 1) * 256 + lane * 8);
+        vs[i] = *reinterpret_cast<const uint2*>(vc + kQ4Meta + (i & 1) * 64 + t * 16 + wp * 8);
       }
 #pragma unroll
-      for (int u = 0; u < SETS; ++u) {
-        const uint64_t al2 = f2_pack(alpha[u], alpha[u]);
+      for (int wl = 0; wl < 2; ++wl) {
+        const int w = 2 * wp + wl;
+        float e[2][4];
+#pragma unroll
+        for (int pg = 0; pg < 2; ++pg) {
+          uint32_t b[2][4];  // [half][n]
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t x = wl ? vw[2 * pg + h].y : vw[2 * pg + h].x;
+            const uint32_t s2 = wl ? vs[2 * pg + h].y : vs[2 * pg + h].x;
+            const uint32_t y = x >> 8;
+            // 1024 + c, or 1024 + 16 c, to c - 8, times s: every step exact
+            b[h][0] = h2_mul(h2_add(and_or(x, 0x000f000fu, magic), 0xe408e408u), s2);
+            b[h][1] = h2_mul(h2_fma(and_or(x, 0x00f000f0u, magic), 0x2c002c00u, 0xd480d480u), s2);
+            b[h][2] = h2_mul(h2_add(and_or(y, 0x000f000fu, magic), 0xe408e408u), s2);
+            b[h][3] = h2_mul(h2_fma(and_or(y, 0x00f000f0u, magic), 0x2c002c00u, 0xd480d480u), s2);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t av[4] = {b[0][2 * i], b[0][2 * i + 1], b[1][2 * i], b[1][2 * i + 1]};
+            if (pg == 0) mma_f16_16816_z(e[i], av, pb[0][0], pb[0][1]);
+            else mma_f16_16816(e[i], av, pb[0][2], pb[0][3]);
+            if (WIDE) mma_f16_16816(e[i], av, pb[HL - 1][2 * pg], pb[HL - 1][2 * pg + 1]);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          o[u][w][i] = f2_fma(o[u][w][i], al2, f2_pack(e[u][i][0] + e[u][i][1], e[u][i][2] + e[u][i][3]));
+          if (WIDE) {
+            o[w][2 * i] = f2_fma(o[w][2 * i], al2, f2_pack(e[i][0], e[i][1]));
+            o[w][2 * i + HL - 1] = f2_fma(o[w][2 * i + HL - 1], al2, f2_pack(e[i][2], e[i][3]));
+          } else {
+            o[w][i] = f2_fma(o[w][i], al2, f2_pack(e[i][0] + e[i][1], e[i][2] + e[i][3]));
+          }
         }
       }
     }
@@ -435,22 +494,28 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(SETS))
   }
 
 #pragma unroll
-  for (int u = 0; u < SETS; ++u)
+  for (int h = 0; h < HL; ++h)
 #pragma unroll
-    for (int off = 4; off < 32; off <<= 1) l[u] += __shfl_xor_sync(0xffffffffu, l[u], off);
+    for (int off = 4; off < 32; off <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
   consumer_bar();  // every warp is done with its ring
   MergeSmem& ms = *reinterpret_cast<MergeSmem*>(smem_q4);
 #pragma unroll
-  for (int u = 0; u < SETS; ++u) {
+  for (int h = 0; h < HL; ++h) {
+    const int head = HL * t + h;
     if (g == 0) {
-      ms.m[warp][4 * u + t] = m[u];
-      ms.l[warp][4 * u + t] = l[u];
+      ms.m[warp][head] = m[h];
+      ms.l[warp][head] = l[h];
     }
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float off = __shfl_sync(0xffffffffu, oo[u], 4 * w + t);
-      *reinterpret_cast<float4*>(&ms.o[warp][4 * u + t][32 * w + 4 * g]) =
-          make_float4(f2_lo(o[u][w][0]) + off, f2_hi(o[u][w][0]) + off, f2_lo(o[u][w][1]) + off, f2_hi(o[u][w][1]) + off);
+      const float off = __shfl_sync(0xffffffffu, oo[h][w & 1], 4 * (w >> 1) + t);
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t v = WIDE ? o[w][i & (2 * HL - 1)] : o[w][i >> 1];
+        x[i] = ((WIDE ? h : i & 1) ? f2_hi(v) : f2_lo(v)) + off;
+      }
+      *reinterpret_cast<float4*>(&ms.o[warp][head][32 * w + 4 * g]) = make_float4(x[0], x[1], x[2], x[3]);
     }
   }
   consumer_bar();

@@ -16,13 +16,14 @@
 // 16: 160 bytes instead of 512 for a token's K and V of one kv head.
 //
 // The codes lie in the order in which the decode kernel's lanes want them as
-// tensor-core operands, so that a lane's 128-bit load is its operand and no
+// tensor-core operands, so that a lane's 64-bit load is its operand and no
 // shuffle is needed (lane = 4 g + t, g = lane / 4 = 0..7, t = lane % 4):
 //   K: token r (0..15), dims 32 w + 8 t + n (w = group, n = 0..7): nibble n of
-//      the 32-bit word at r * 64 + t * 16 + w * 4;
+//      the 32-bit word at (w / 2) * 512 + r * 32 + t * 8 + (w % 2) * 4;
 //      then at 1024 + r * 16 the token's f16 o[0..3], s[0..3].
 //   V: token r = 8 h + 2 t + p (p = 0, 1), dims 32 w + 4 g + n (n = 0..3):
-//      nibble n of the 16-bit piece at h * 512 + g * 64 + t * 16 + w * 4 + p * 2;
+//      nibble n of the 16-bit piece at
+//      (w / 2) * 512 + h * 256 + g * 32 + t * 8 + (w % 2) * 4 + p * 2;
 //      then f16 s at 1024 and o at 1152, each at + h * 64 + t * 16 + w * 4 + p * 2.
 #pragma once
 #include <cuda_fp16.h>
@@ -84,10 +85,10 @@ __device__ __forceinline__ size_t q4_chunk_off(const KVPool& pool, int layer, in
 
 // Byte offsets inside a chunk.
 __host__ __device__ __forceinline__ int q4_k_word(int tok, int block) {  // the 8 dims [8 block, 8 block + 8)
-  return tok * 64 + (block & 3) * 16 + (block >> 2) * 4;
+  return (block >> 3) * 512 + tok * 32 + (block & 3) * 8 + ((block >> 2) & 1) * 4;
 }
-__host__ __device__ __forceinline__ int q4_v_pair(int tok, int g) {  // the 16 bytes of tok's pair (tok & ~1, tok | 1), piece g
-  return (tok >> 3) * 512 + g * 64 + ((tok >> 1) & 3) * 16;
+__host__ __device__ __forceinline__ int q4_v_pair(int tok, int g, int wp) {  // 8 bytes: tok's pair (tok & ~1, tok | 1), piece g of groups 2 wp, 2 wp + 1
+  return wp * 512 + (tok >> 3) * 256 + g * 32 + ((tok >> 1) & 3) * 8;
 }
 __host__ __device__ __forceinline__ int q4_v_meta(int tok) {  // the pair's 4 x 2 scales (or, at kQ4VOffsets, offsets)
   return (tok >> 3) * 64 + ((tok >> 1) & 3) * 16;
@@ -152,40 +153,44 @@ __global__ void __launch_bounds__(128)
     const uint8_t* c = static_cast<const uint8_t*>(is_v ? pool.v : pool.k) + q4_chunk_off(pool, a.layer, page, g);
     const uint4 w4 = *reinterpret_cast<const uint4*>(c + u * 16);
     const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+    const int wp = u >> 5;  // groups 2 wp and 2 wp + 1; the 16 bytes hold t and t + 1 of each
     if (!is_v) {
-      const int tok = u >> 2, t = u & 3, slot = s0 + tok;
-      const uint4 m4 = *reinterpret_cast<const uint4*>(c + kQ4Meta + tok * 16);
-      const uint32_t m[4] = {m4.x, m4.y, m4.z, m4.w};  // o01 o23 s01 s23
+      const int tok = (u & 31) >> 1, t = (u & 1) * 2, slot = s0 + tok;
+      const uint32_t o2 = *reinterpret_cast<const uint32_t*>(c + kQ4Meta + tok * 16 + wp * 4);
+      const uint32_t s2 = *reinterpret_cast<const uint32_t*>(c + kQ4Meta + tok * 16 + 8 + wp * 4);
       if (!wanted(slot) && !a.paged) return;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float o = __half2float(__ushort_as_half((uint16_t)(m[q >> 1] >> (16 * (q & 1)))));
-        const float s = __half2float(__ushort_as_half((uint16_t)(m[2 + (q >> 1)] >> (16 * (q & 1)))));
+      for (int q = 0; q < 2; ++q) {
+        const float o = __half2float(__ushort_as_half((uint16_t)(o2 >> (16 * q))));
+        const float s = __half2float(__ushort_as_half((uint16_t)(s2 >> (16 * q))));
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < 4; ++e) {  // t and t + 1 of this group: 16 dims in a row
           float x[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = q4_value((w[q] >> (16 * e + 4 * i)) & 15u, s, o);
-          store4<OUT_BF16>(out, at(slot, 32 * q + 8 * t + 4 * e), wanted(slot) ? x : zero);
+          for (int i = 0; i < 4; ++i) x[i] = q4_value((w[2 * (e >> 1) + q] >> (16 * (e & 1) + 4 * i)) & 15u, s, o);
+          store4<OUT_BF16>(out, at(slot, 32 * (2 * wp + q) + 8 * t + 4 * e), wanted(slot) ? x : zero);
         }
       }
     } else {
-      const int h = u >> 5, gg = (u >> 2) & 7, t = u & 3;
-      const uint4 s4 = *reinterpret_cast<const uint4*>(c + kQ4Meta + h * 64 + t * 16);
-      const uint4 o4 = *reinterpret_cast<const uint4*>(c + kQ4VOffsets + h * 64 + t * 16);
-      const uint32_t sw[4] = {s4.x, s4.y, s4.z, s4.w}, ow[4] = {o4.x, o4.y, o4.z, o4.w};
+      const int h = (u >> 4) & 1, gg = (u >> 1) & 7;
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int slot = s0 + 8 * h + 2 * t + p;
-        if (!wanted(slot) && !a.paged) continue;
+      for (int tt = 0; tt < 2; ++tt) {
+        const int t = (u & 1) * 2 + tt;
+        const uint2 s4 = *reinterpret_cast<const uint2*>(c + kQ4Meta + h * 64 + t * 16 + wp * 8);
+        const uint2 o4 = *reinterpret_cast<const uint2*>(c + kQ4VOffsets + h * 64 + t * 16 + wp * 8);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float o = __half2float(__ushort_as_half((uint16_t)(ow[q] >> (16 * p))));
-          const float s = __half2float(__ushort_as_half((uint16_t)(sw[q] >> (16 * p))));
-          float x[4];
+        for (int p = 0; p < 2; ++p) {
+          const int slot = s0 + 8 * h + 2 * t + p;
+          if (!wanted(slot) && !a.paged) continue;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = q4_value((w[q] >> (16 * p + 4 * i)) & 15u, s, o);
-          store4<OUT_BF16>(out, at(slot, 32 * q + 4 * gg), wanted(slot) ? x : zero);
+          for (int q = 0; q < 2; ++q) {
+            const float o = __half2float(__ushort_as_half((uint16_t)((q ? o4.y : o4.x) >> (16 * p))));
+            const float s = __half2float(__ushort_as_half((uint16_t)((q ? s4.y : s4.x) >> (16 * p))));
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = q4_value((w[2 * tt + q] >> (16 * p + 4 * i)) & 15u, s, o);
+            store4<OUT_BF16>(out, at(slot, 32 * (2 * wp + q) + 4 * gg), wanted(slot) ? x : zero);
+          }
         }
       }
     }

@@ -36,22 +36,22 @@ static_assert((int)kKvF32 == OOMATTN_DTYPE_F32 && (int)kKvBf16 == OOMATTN_DTYPE_
 
 int split_cap(int kv_dtype) { return kv_dtype == OOMATTN_DTYPE_F32 ? kMaxSplits : kMaxSplitsBf16; }
 // Resident decode CTAs per SM, and the fixed cost of one in pages (plan_decode), by cache type.
-int q4_sets(int group) { return group <= 4 ? 1 : 2; }  // column sets of the 4-bit decode: four heads each
+bool q4_wide(int group) { return group > 4; }  // the 4-bit decode's two forms: see decode_q4.cuh
 int decode_slots(int kv_dtype, int group) {
-  return kv_dtype == OOMATTN_DTYPE_Q4 ? q4_ctas_per_sm(q4_sets(group)) : kDecCtasPerSm;
+  return kv_dtype == OOMATTN_DTYPE_Q4 ? q4_ctas_per_sm(q4_wide(group)) : kDecCtasPerSm;
 }
 typedef void (*DecodeQ4Fn)(const KVPool, const DecodeArgs, const SeqBatch, const DecodeSched);
-DecodeQ4Fn decode_q4_fn(int sets, bool io16) {
-  if (sets == 1) return io16 ? decode_q4_kernel<1, true> : decode_q4_kernel<1, false>;
-  return io16 ? decode_q4_kernel<2, true> : decode_q4_kernel<2, false>;
+DecodeQ4Fn decode_q4_fn(bool wide, bool io16) {
+  if (wide) return io16 ? decode_q4_kernel<true, true> : decode_q4_kernel<true, false>;
+  return io16 ? decode_q4_kernel<false, true> : decode_q4_kernel<false, false>;
 }
 cudaError_t set_decode_q4_smem() {
   cudaError_t e = cudaSuccess;
-  for (int sets = 1; sets <= 2; ++sets)
-    for (int io16 = 0; io16 < 2; ++io16)
+  for (bool wide : {false, true})
+    for (bool io16 : {false, true})
       if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(decode_q4_fn(sets, io16), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 q4_smem_bytes(sets));
+        e = cudaFuncSetAttribute(decode_q4_fn(wide, io16), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 q4_smem_bytes(wide));
   return e;
 }
 static_assert(kMaxGroup * kMaxSplits <= kDecWarps * kMaxGroup * kMergeStride,
@@ -689,7 +689,7 @@ int rope_q_impl(oomattn_ctx* ctx, int n_rows, const int32_t* positions, const vo
 // (pipeline fill and merge).  Returns the number of items (the grid size).
 constexpr int kDecodeFillPages = 12;     // bf16 cache
 constexpr int kDecodeFillPagesF32 = 12;  // f32 cache (measured insensitive: 4 to 200 chose the same plans on C1)
-constexpr int kDecodeFillPagesQ4 = 12;   // 4-bit cache
+constexpr int kDecodeFillPagesQ4 = 24;   // 4-bit cache (12 to 48 measured alike, 96 slower: 65.5 against 55.6 us on 64 ragged rows)
 int decode_fill(int kv_dtype) {
   return kv_dtype == OOMATTN_DTYPE_BF16 ? kDecodeFillPages
                                         : (kv_dtype == OOMATTN_DTYPE_F32 ? kDecodeFillPagesF32 : kDecodeFillPagesQ4);
@@ -842,8 +842,8 @@ int launch_decode_rows(oomattn_ctx* ctx, int layer, const SeqBatch& sb, const fl
     le = cudaLaunchKernelEx(&cfg, decode_bf16_kernel, ctx->kmap, ctx->vmap, pool, a, sb, sched);
   } else if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4) {
     cfg.blockDim = dim3(kDecWarps * 32);
-    cfg.dynamicSmemBytes = q4_smem_bytes(q4_sets(ctx->group));
-    le = cudaLaunchKernelEx(&cfg, decode_q4_fn(q4_sets(ctx->group), io16), pool, a, sb, sched);
+    cfg.dynamicSmemBytes = q4_smem_bytes(q4_wide(ctx->group));
+    le = cudaLaunchKernelEx(&cfg, decode_q4_fn(q4_wide(ctx->group), io16), pool, a, sb, sched);
   } else {
     cfg.blockDim = dim3(kDecWarps * 32);
     le = cudaLaunchKernelEx(&cfg, decode_f32_kernel, pool, a, sb, sched);
@@ -1291,7 +1291,7 @@ int oomattn_kv_read(oomattn_ctx* ctx, int32_t layer, int32_t seq, void* k_out, v
                 o = half_at(kQ4Meta + r * 16 + 2 * w);
                 s = half_at(kQ4Meta + r * 16 + 8 + 2 * w);
               } else {
-                code = chunk[q4_v_pair(r, (d & 31) >> 2) + 4 * w + 2 * (r & 1) + ((d & 3) >> 1)] >> (4 * (d & 1)) & 15;
+                code = chunk[q4_v_pair(r, (d & 31) >> 2, w >> 1) + 4 * (w & 1) + 2 * (r & 1) + ((d & 3) >> 1)] >> (4 * (d & 1)) & 15;
                 s = half_at(kQ4Meta + q4_v_meta(r) + 4 * w + 2 * (r & 1));
                 o = half_at(kQ4VOffsets + q4_v_meta(r) + 4 * w + 2 * (r & 1));
               }
@@ -1969,8 +1969,8 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
     }
     decode_bf16_kernel<<<n_items, (kDecWarps + 1) * 32, kDecSmemBytes, st>>>(maps[0], maps[1], pool, a, sb, sched);
   } else if (kv_dtype == OOMATTN_DTYPE_Q4) {
-    const int sets = q4_sets(n_heads / n_kv_heads);
-    decode_q4_fn(sets, false)<<<n_items, kDecWarps * 32, q4_smem_bytes(sets), st>>>(pool, a, sb, sched);
+    const bool wide = q4_wide(n_heads / n_kv_heads);
+    decode_q4_fn(wide, false)<<<n_items, kDecWarps * 32, q4_smem_bytes(wide), st>>>(pool, a, sb, sched);
   } else {
     decode_f32_kernel<<<n_items, kDecWarps * 32, 0, st>>>(pool, a, sb, sched);
   }

@@ -50,7 +50,7 @@ __device__ __forceinline__ uint32_t q4_codes8(const float* x, float s, float o) 
 
 // A warp's task is four heads of one token (q, k, and v of f32 / bf16 caches)
 // or four heads of one pair of adjacent slots (v of a 4-bit cache, whose codes
-// lie pairwise: with both slots new the pair is written as 16-byte pieces).
+// lie pairwise: with both slots new the pair is written as 8-byte pieces).
 // Eight lanes per head; every lane stays with its warp through the shuffles,
 // lanes of heads past the last repeat it and store nothing.  Tasks run q, k, v.
 template <bool IN_BF16, bool Q_BF16, int KV>
@@ -131,10 +131,11 @@ __global__ void __launch_bounds__(256)
       }
       if (head0 >= hkv) continue;
       uint8_t* ch = static_cast<uint8_t*>(pool.v) + q4_chunk_off(pool, ap.layer, page, head);
-      uint8_t* cp = ch + q4_v_pair(tok, c);
+      uint8_t* cp = ch + q4_v_pair(tok, c, 0);
       uint8_t* mp = ch + kQ4Meta + q4_v_meta(tok);
       if (in0 && in1) {
-        *reinterpret_cast<uint4*>(cp) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+        *reinterpret_cast<uint2*>(cp) = make_uint2(codes[0], codes[1]);
+        *reinterpret_cast<uint2*>(cp + 512) = make_uint2(codes[2], codes[3]);
         if (c == 0) *reinterpret_cast<uint4*>(mp) = make_uint4(sw[0], sw[1], sw[2], sw[3]);
         if (c == 1) *reinterpret_cast<uint4*>(mp + kQ4VOffsets - kQ4Meta) = make_uint4(ow[0], ow[1], ow[2], ow[3]);
       } else {
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(256)
         const int p = in0 ? 0 : 1;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          *reinterpret_cast<uint16_t*>(cp + 4 * q + 2 * p) = (uint16_t)(codes[q] >> (16 * p));
+          *reinterpret_cast<uint16_t*>(cp + (q >> 1) * 512 + (q & 1) * 4 + 2 * p) = (uint16_t)(codes[q] >> (16 * p));
           if (c == 0) *reinterpret_cast<uint16_t*>(mp + 4 * q + 2 * p) = (uint16_t)(sw[q] >> (16 * p));
           if (c == 1)
             *reinterpret_cast<uint16_t*>(mp + kQ4VOffsets - kQ4Meta + 4 * q + 2 * p) = (uint16_t)(ow[q] >> (16 * p));

@@ -117,12 +117,12 @@ def test_pool_layout_is_the_documented_one():
             kch, vch = kp[page, h], vp[page, h]
             for d in range(0, 128, 3):
                 w, t, m = d // 32, d % 32 // 8, d % 8
-                word = int(kch[64 * r + 16 * t + 4 * w:][:4].view(np.uint32)[0])
+                word = int(kch[512 * (w // 2) + 32 * r + 8 * t + 4 * (w % 2):][:4].view(np.uint32)[0])
                 assert (word >> (4 * m)) & 15 == kc[tok, h, d]
                 assert half(kch, 1024 + 16 * r + 2 * w) == ko[tok, h, w]
                 assert half(kch, 1024 + 16 * r + 8 + 2 * w) == ks[tok, h, w]
                 hh, tt, p, g, m = r // 8, r % 8 // 2, r % 2, d % 32 // 4, d % 4
-                piece = int(vch[512 * hh + 64 * g + 16 * tt + 4 * w + 2 * p:][:2].view(np.uint16)[0])
+                piece = int(vch[512 * (w // 2) + 256 * hh + 32 * g + 8 * tt + 4 * (w % 2) + 2 * p:][:2].view(np.uint16)[0])
                 assert (piece >> (4 * m)) & 15 == vc[tok, h, d]
                 assert half(vch, 1024 + 64 * hh + 16 * tt + 4 * w + 2 * p) == vs[tok, h, w]
                 assert half(vch, 1152 + 64 * hh + 16 * tt + 4 * w + 2 * p) == vo[tok, h, w]
