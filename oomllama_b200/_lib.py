@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from array import array
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "liboomattn.so")
@@ -169,8 +170,14 @@ def load():
 
 
 def int_array(values):
-    vals = [int(v) for v in values]
-    return (ctypes.c_int32 * max(1, len(vals)))(*vals)
+    """A C int32 array of `values` (one element at least, so that it has an address)."""
+    try:
+        a = array("i", values)
+    except TypeError:  # numbers that are no integers of their own
+        a = array("i", [int(v) for v in values])
+    if not a:
+        a.append(0)
+    return (ctypes.c_int32 * len(a)).from_buffer(a)
 
 
 def check(ctx, code: int):

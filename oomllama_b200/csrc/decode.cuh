@@ -156,7 +156,8 @@ __device__ __forceinline__ void merge_splits_staged(const DecodeArgs& a, int z, 
 // (`stage`, and `s_w` for the weights) the merge is merge_splits_staged;
 // without one (the f32 kernel, which holds no shared ring) the partials are
 // loaded into registers.
-template <bool OUT16 = false>
+// kLate: the launch may leave the merge to a kernel after it (no counters).
+template <bool OUT16 = false, bool kLate = false>
 __device__ __forceinline__ void combine_and_store(const MergeSmem& ms, const DecodeArgs& a, int z, int g, int split,
                                                   int nsplit, int n_kv, int tid, int* s_last, float* stage,
                                                   int stage_floats, float* s_w) {
@@ -202,7 +203,7 @@ __device__ __forceinline__ void combine_and_store(const MergeSmem& ms, const Dec
       if ((tid & 15) == 0) a.part_lse[prow] = lse2;
     }
   }
-  if (nsplit == 1) return;
+  if (nsplit == 1 || (kLate && a.counters == nullptr)) return;
   consumer_bar();
   if (tid == 0) {
     const unsigned prev = atom_add_acq_rel_gpu(&a.counters[(size_t)z * n_kv + g], 1u);

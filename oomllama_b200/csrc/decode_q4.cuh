@@ -117,23 +117,6 @@ __device__ __forceinline__ uint32_t f16_part(float a, float b, bool low) {
   return low ? pack_f16(a - h_lo(hi), b - h_hi(hi)) : hi;
 }
 
-// decode.cuh's prefetch_then_wait for 4-bit chunks.
-__device__ __forceinline__ void q4_prefetch_then_wait(const KVPool& pool, const DecodeArgs& a, int seq, int g, int pb,
-                                                      int pe) {
-  const int np = min(pe - pb, kDecPrefetchPages);
-  if (np > 0) {
-    constexpr int lines = kQ4Pair / 128;
-    const int* bt = pool.block_table + (size_t)seq * pool.max_pages_per_seq;
-    for (int i = threadIdx.x; i < np * lines; i += blockDim.x) {
-      const int page = __ldg(bt + pb + i / lines), r = i % lines;
-      if ((unsigned)page >= (unsigned)pool.n_pool_pages) continue;  // reported by the main loop
-      const char* base = static_cast<const char*>(pool.k) + q4_chunk_off(pool, a.layer, page, g);
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(base + (size_t)r * 128));
-    }
-  }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 // IO16: q and out in bf16 (the newest tokens of a sequence as one row each)
 // instead of f32 (a generation step).
 template <bool WIDE, bool IO16>
@@ -152,8 +135,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
   const int g_kv = item.g, z = item.z;
   const int seq = sb.seq[z], L = sb.len[z];
   const int pb = item.pb, pe = item.pe;
-  q4_prefetch_then_wait(pool, a, seq, g_kv, pb, pe);
   if (pb >= pe) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (!IO16 && L <= 0 && item.split == 0) write_empty_row(a, z, g_kv);  // a bf16 row sees its own token at least
     return;
   }
@@ -209,6 +192,16 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
     }
     issued = k + 1;
   };
+  // Launched as a programmatic dependent of the kernel before it (the append):
+  // while that one finishes, the first tiles' pages are pulled into L2 (20 lines
+  // of 128 bytes each); q and the cache are read only after it.
+#pragma unroll
+  for (int j = 0; j < kStages * kQ4Pages; ++j) {
+    const int id = __shfl_sync(0xffffffffu, ids, j);
+    if (id >= 0 && lane < kQ4Pair / 128)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(base + (size_t)(uint32_t)id * page_bytes + lane * 128));
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int k = 0; k < min(kStages, n_tiles); ++k) issue(k, k);
 
   // ---- the query as B operand: lane (g, t) holds column g at dims 32 w + 8 t +
@@ -519,8 +512,69 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
     }
   }
   consumer_bar();
-  combine_and_store<IO16>(ms, a, z, g_kv, item.split, item.nsplit, pool.n_kv, threadIdx.x, s_last,
+  combine_and_store<IO16, true>(ms, a, z, g_kv, item.split, item.nsplit, pool.n_kv, threadIdx.x, s_last,
                           reinterpret_cast<float*>(smem_q4), kRing / 4, s_w);
+}
+
+// The merge of a launch with more splits per row than its last CTA could join
+// quickly (kMaxSplitsBf16): a kernel of its own, one CTA per (row, q head).
+// Its eight warps take every eighth split, a lane four dims; weights 2^(lse -
+// max) and the sums as in merge_splits_staged, in a fixed order.  Rows with a
+// single split were written by the decode kernel.
+constexpr int kMergeWarps = 8;
+template <bool IO16>
+__global__ void __launch_bounds__(kMergeWarps * 32)
+    merge_splits_kernel(const DecodeArgs a, const __grid_constant__ SeqBatch sb, const __grid_constant__ DecodeSched sched) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ float s_wt[kMaxSplitsQ4];
+  __shared__ float s_red[2][kMergeWarps];
+  __shared__ float4 s_acc[kMergeWarps][32];
+  const int r = blockIdx.x / a.n_heads, h = blockIdx.x - r * a.n_heads;
+  const int z = sched.order[r];
+  const int n_pages = (sb.len[z] + kPageSize - 1) / kPageSize;
+  const int pps = n_pages > 0 ? (n_pages + sched.nsplit[r] - 1) / sched.nsplit[r] : 0;
+  const int ns = pps > 0 ? (n_pages + pps - 1) / pps : 1;  // as decode_item
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (ns <= 1) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const size_t zh = (size_t)z * a.n_heads + h, p0 = zh * a.max_splits;
+  static_assert(kMaxSplitsQ4 <= kMergeWarps * 32, "one split weight per thread");
+  const float ls = (int)threadIdx.x < ns ? __ldcg(a.part_lse + p0 + threadIdx.x) : -INFINITY;
+  float M = ls;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  if (lane == 0) s_red[0][warp] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeWarps; ++w) M = fmaxf(M, s_red[0][w]);
+  const float wt = ls == -INFINITY ? 0.f : exp2f(ls - M);
+  s_wt[threadIdx.x] = wt;
+  float sum = wt;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  if (lane == 0) s_red[1][warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kMergeWarps; ++w) sum += s_red[1][w];
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int s = warp; s < ns; s += kMergeWarps) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + (p0 + s) * kHeadDim) + lane);
+    const float w = s_wt[s];
+    acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
+  }
+  s_acc[warp][lane] = acc;
+  __syncthreads();
+  if (warp != 0) return;
+#pragma unroll
+  for (int w = 1; w < kMergeWarps; ++w) {
+    const float4 v = s_acc[w][lane];
+    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+  }
+  const float inv = 1.f / sum;
+  store_out4<IO16>(a, zh, lane * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  if (a.lse && lane == 0) a.lse[zh * a.lse_stride] = (M + log2f(sum)) * 0.69314718055994531f;
 }
 
 }  // namespace oomattn

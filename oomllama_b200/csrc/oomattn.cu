@@ -145,6 +145,7 @@ struct oomattn_ctx {
   std::vector<int> sched_key;
   DecodeSched sched;
   int sched_items = 0;
+  int sched_splits = 0;  // its cap on the splits of a row
 };
 
 namespace {
@@ -694,6 +695,8 @@ int decode_fill(int kv_dtype) {
   return kv_dtype == OOMATTN_DTYPE_BF16 ? kDecodeFillPages
                                         : (kv_dtype == OOMATTN_DTYPE_F32 ? kDecodeFillPagesF32 : kDecodeFillPagesQ4);
 }
+// A 4-bit CTA's four warps take two pages each at a time: fewer than eight pages save nothing.
+int decode_min_pages(int kv_dtype) { return kv_dtype == OOMATTN_DTYPE_Q4 ? kDecWarps * kQ4Pages : 1; }
 constexpr int kDecodeMaxSimSlots = 2048;
 
 long long lpt_makespan(const int* size, const int* count, int groups, int slots, int fill, long long* heap) {
@@ -719,7 +722,8 @@ long long lpt_makespan(const int* size, const int* count, int groups, int slots,
   return mx;
 }
 
-int plan_decode(const SeqBatch& sb, int n_kv, int slots, int max_splits, int fill, DecodeSched& sched) {
+// min_pages: a range has that many at least (a row's last one may have fewer).
+int plan_decode(const SeqBatch& sb, int n_kv, int slots, int max_splits, int fill, int min_pages, DecodeSched& sched) {
   slots = std::max(1, std::min(slots, kDecodeMaxSimSlots));
   int pages[kMaxBatch];
   int mp = 0;
@@ -727,7 +731,7 @@ int plan_decode(const SeqBatch& sb, int n_kv, int slots, int max_splits, int fil
     pages[z] = sb.len[z] > 0 ? (sb.len[z] + kPageSize - 1) / kPageSize : 0;
     mp = std::max(mp, pages[z]);
   }
-  const int t_lo = std::max(1, (mp + max_splits - 1) / max_splits);
+  const int t_lo = std::max(min_pages, (mp + max_splits - 1) / max_splits);
   const int t_hi = std::max(t_lo, mp);
   auto ns_of = [&](int p, int t) { return p > 0 ? (p + t - 1) / t : 1; };
   auto ctas_of = [&](int t) {
@@ -791,6 +795,15 @@ int plan_decode(const SeqBatch& sb, int n_kv, int slots, int max_splits, int fil
   return items;
 }
 
+// The most splits of a row of a 4-bit decode.  32, which the last CTA of a row
+// joins; where that leaves SMs idle although the longest row has many pages for
+// each split, as many as the partials' memory holds for so few rows.
+constexpr int kQ4LatePages = 200;
+int q4_max_splits(int rows, int n_kv, int max_pages, int slots) {
+  if (rows * n_kv * kMaxSplitsBf16 >= slots || max_pages < kQ4LatePages) return kMaxSplitsBf16;
+  return std::min(kMaxSplitsQ4, kMaxBatch * kMaxSplitsBf16 / rows);
+}
+
 // io16: q and out are bf16 (4-bit cache only).
 int launch_decode_rows(oomattn_ctx* ctx, int layer, const SeqBatch& sb, const float* q, float* out, float* lse,
                        int o_stride, int lse_stride, bool io16 = false) {
@@ -800,8 +813,12 @@ int launch_decode_rows(oomattn_ctx* ctx, int layer, const SeqBatch& sb, const fl
   key[0] = sb.n;
   for (int z = 0; z < sb.n; ++z) key[z + 1] = sb.len[z] > 0 ? (sb.len[z] + kPageSize - 1) / kPageSize : 0;
   if (ctx->sched_key.size() != (size_t)sb.n + 1 || !std::equal(key, key + sb.n + 1, ctx->sched_key.begin())) {
-    ctx->sched_items = plan_decode(sb, n_kv, slots, split_cap(ctx->cfg.kv_dtype),
-                                   decode_fill(ctx->cfg.kv_dtype),
+    int mp = 0;
+    for (int z = 0; z < sb.n; ++z) mp = std::max(mp, key[z + 1]);
+    ctx->sched_splits = ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4 ? q4_max_splits(sb.n, n_kv, mp, slots)
+                                                              : split_cap(ctx->cfg.kv_dtype);
+    ctx->sched_items = plan_decode(sb, n_kv, slots, ctx->sched_splits,
+                                   decode_fill(ctx->cfg.kv_dtype), decode_min_pages(ctx->cfg.kv_dtype),
                                    ctx->sched);
     ctx->sched_key.assign(key, key + sb.n + 1);
   }
@@ -818,11 +835,12 @@ int launch_decode_rows(oomattn_ctx* ctx, int layer, const SeqBatch& sb, const fl
   a.layer = layer;
   a.n_heads = ctx->cfg.n_heads;
   a.group = ctx->group;
-  a.max_splits = split_cap(ctx->cfg.kv_dtype);
+  a.max_splits = ctx->sched_splits;
   a.qscale = ctx->scale * 1.4426950408889634f;
   a.part_o = ctx->d_part_o;
   a.part_lse = ctx->d_part_lse;
-  a.counters = ctx->d_counters;
+  const bool late = ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4 && a.max_splits > kMaxSplitsBf16;
+  a.counters = late ? nullptr : ctx->d_counters;
   a.status = ctx->d_status;
   a.timeout_ns = ctx->timeout_ns;
   KVPool pool = make_pool(ctx);
@@ -844,6 +862,9 @@ int launch_decode_rows(oomattn_ctx* ctx, int layer, const SeqBatch& sb, const fl
     cfg.blockDim = dim3(kDecWarps * 32);
     cfg.dynamicSmemBytes = q4_smem_bytes(q4_wide(ctx->group));
     le = cudaLaunchKernelEx(&cfg, decode_q4_fn(q4_wide(ctx->group), io16), pool, a, sb, sched);
+    if (le == cudaSuccess && late)
+      le = launch_pdl(io16 ? merge_splits_kernel<true> : merge_splits_kernel<false>, dim3(sb.n * a.n_heads),
+                      dim3(kMergeWarps * 32), 0, ctx->stream, a, sb, sched);
   } else {
     cfg.blockDim = dim3(kDecWarps * 32);
     le = cudaLaunchKernelEx(&cfg, decode_f32_kernel, pool, a, sb, sched);
@@ -1915,7 +1936,7 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
   const int cap_splits = std::max(1, std::min(split_cap(kv_dtype), kStaticPartSlots / (n_rows * n_heads)));
   DecodeSched sched;
   const int n_items = plan_decode(sb, n_kv_heads, num_sms * decode_slots(kv_dtype, n_heads / n_kv_heads), cap_splits,
-                                  decode_fill(kv_dtype), sched);
+                                  decode_fill(kv_dtype), decode_min_pages(kv_dtype), sched);
   if (n_items == 0) return OOMATTN_OK;
 
   // The counters must start at zero; a previous call that ended early could

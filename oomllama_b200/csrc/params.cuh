@@ -14,6 +14,9 @@ constexpr int kMaxGroup = 8;    // q heads per kv head handled by one decode CTA
 // layer step at 43 splits than at 26.
 constexpr int kMaxSplits = 64;
 constexpr int kMaxSplitsBf16 = 32;
+// 4-bit caches: 32 as well, and up to 256 where 32 leave SMs idle on a long
+// context (few rows of few kv heads), merged by a kernel of its own.
+constexpr int kMaxSplitsQ4 = 256;
 
 // Per-launch sequence rows, passed by value so a launch needs no host->device
 // metadata copy (and can be captured in a CUDA graph).
@@ -62,7 +65,7 @@ struct DecodeArgs {
   float qscale;         // softmax scale * log2(e)
   float* part_o;        // [rows][n_heads][max_splits][128]
   float* part_lse;      // [rows][n_heads][max_splits], base 2
-  unsigned* counters;   // [rows][n_kv], zero between launches
+  unsigned* counters;   // [rows][n_kv], zero between launches; null: another kernel merges the splits
   int* status;
   unsigned long long timeout_ns;
 };

@@ -40,7 +40,7 @@ def _dtype_code(t: torch.Tensor) -> int:
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()  # a c_void_p parameter takes the address as it is
 
 
 def _same_count(values, seq_ids, name: str):
@@ -49,6 +49,9 @@ def _same_count(values, seq_ids, name: str):
 
 
 def _dev(t: torch.Tensor, name: str, device: int, dtype=None, numel=None):
+    if (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == device and t.is_contiguous()
+            and (dtype is None or t.dtype is dtype) and (numel is None or t.numel() == numel)):
+        return t
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
     if t.device.index != device:
@@ -125,6 +128,7 @@ class TurboEngine:
     def __init__(self, config: TurboConfig, device: int = 0, assign_pages: bool = True):
         self.config = config
         self.device = int(device)
+        self._torch_device = torch.device("cuda", self.device)
         self._L = _lib.load()
         cfg = config.to_c()
         self._n_pages = cfg.n_pages
@@ -154,8 +158,7 @@ class TurboEngine:
             pass
 
     def _bind_stream(self):
-        s = torch.cuda.current_stream(self.device).cuda_stream
-        self._L.oomattn_set_stream(self._ctx, ctypes.c_void_p(s))
+        self._L.oomattn_set_stream(self._ctx, torch._C._cuda_getCurrentRawStream(self.device))
 
     def sync(self):
         """Wait for queued work; raises on a device-side timeout or index-check failure."""
@@ -235,11 +238,13 @@ class TurboEngine:
             n = self.seq_len(layer, seq_ids[0]) - (starts[0] if starts else 0)
         shape = (len(seq_ids) * n, self.config.n_kv_heads, HEAD_DIM)
         if k_out is None:
-            k_out = torch.empty(shape, dtype=out_dtype, device=self.device)
+            k_out = torch.empty(*shape, dtype=out_dtype, device=self._torch_device)
+        else:
+            _dev(k_out, "k_out", self.device, dtype=out_dtype, numel=shape[0] * shape[1] * HEAD_DIM)
         if v_out is None:
-            v_out = torch.empty(shape, dtype=out_dtype, device=self.device)
-        for name, t in (("k_out", k_out), ("v_out", v_out)):
-            _dev(t, name, self.device, dtype=out_dtype, numel=shape[0] * shape[1] * HEAD_DIM)
+            v_out = torch.empty(*shape, dtype=out_dtype, device=self._torch_device)
+        else:
+            _dev(v_out, "v_out", self.device, dtype=out_dtype, numel=shape[0] * shape[1] * HEAD_DIM)
         self._bind_stream()
         check(self._ctx, self._L.oomattn_kv_gather(
             self._ctx, layer, len(seq_ids), int_array(seq_ids), None if starts is None else int_array(starts), n,
@@ -278,7 +283,7 @@ class TurboEngine:
             if b is not None:
                 _dev(b, "bias", self.device, dtype=torch.float32, numel=n * HEAD_DIM)
         if q_out is None:
-            q_out = torch.empty(T, c.n_heads, HEAD_DIM, dtype=q_out_dtype, device=q.device)
+            q_out = torch.empty((T, c.n_heads, HEAD_DIM), dtype=q_out_dtype, device=self._torch_device)
         else:
             _dev(q_out, "q_out", self.device, dtype=q_out_dtype, numel=T * c.n_heads * HEAD_DIM)
         norm = self._qk_norm(q_norm, k_norm, eps)
@@ -337,9 +342,9 @@ class TurboEngine:
         rows = len(seq_ids)
         _dev(q, "q", self.device, dtype=torch.float32, numel=rows * c.n_heads * HEAD_DIM)
         if out is None:
-            out = torch.empty(rows, c.n_heads, HEAD_DIM, dtype=torch.float32, device=q.device)
+            out = torch.empty((rows, c.n_heads, HEAD_DIM), dtype=torch.float32, device=self._torch_device)
         if with_lse and lse is None:
-            lse = torch.empty(rows, c.n_heads, dtype=torch.float32, device=q.device)
+            lse = torch.empty((rows, c.n_heads), dtype=torch.float32, device=self._torch_device)
         self._bind_stream()
         check(self._ctx, self._L.oomattn_decode(
             self._ctx, layer, rows, int_array(seq_ids), None if lens is None else int_array(lens), _ptr(q),
