@@ -117,9 +117,9 @@ __device__ __forceinline__ uint32_t f16_part(float a, float b, bool low) {
   return low ? pack_f16(a - h_lo(hi), b - h_hi(hi)) : hi;
 }
 
-// IO16: q and out in bf16 (the newest tokens of a sequence as one row each)
+// Q16, OUT16: q and out in bf16 (the newest tokens of a sequence as one row each)
 // instead of f32 (a generation step).
-template <bool WIDE, bool IO16>
+template <bool WIDE, bool Q16, bool OUT16>
 __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
     decode_q4_kernel(const KVPool pool, const DecodeArgs a, const __grid_constant__ SeqBatch sb,
                      const __grid_constant__ DecodeSched sched) {
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
   const int pb = item.pb, pe = item.pe;
   if (pb >= pe) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (!IO16 && L <= 0 && item.split == 0) write_empty_row(a, z, g_kv);  // a bf16 row sees its own token at least
+    if (!OUT16 && L <= 0 && item.split == 0) write_empty_row(a, z, g_kv);  // a bf16 row sees its own token at least
     return;
   }
   const int warp = threadIdx.x >> 5;
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
     float mx = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      load8<IO16>(a.q, q0 + 32 * w + 8 * t, x[w]);
+      load8<Q16>(a.q, q0 + 32 * w + 8 * t, x[w]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (!valid) x[w][i] = 0.f;
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
     }
   }
   consumer_bar();
-  combine_and_store<IO16, true>(ms, a, z, g_kv, item.split, item.nsplit, pool.n_kv, threadIdx.x, s_last,
+  combine_and_store<OUT16, true>(ms, a, z, g_kv, item.split, item.nsplit, pool.n_kv, threadIdx.x, s_last,
                           reinterpret_cast<float*>(smem_q4), kRing / 4, s_w);
 }
 
@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
 // max) and the sums as in merge_splits_staged, in a fixed order.  Rows with a
 // single split were written by the decode kernel.
 constexpr int kMergeWarps = 8;
-template <bool IO16>
+template <bool OUT16>
 __global__ void __launch_bounds__(kMergeWarps * 32)
     merge_splits_kernel(const DecodeArgs a, const __grid_constant__ SeqBatch sb, const __grid_constant__ DecodeSched sched) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
     acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
   }
   const float inv = 1.f / sum;
-  store_out4<IO16>(a, zh, lane * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  store_out4<OUT16>(a, zh, lane * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
   if (a.lse && lane == 0) a.lse[zh * a.lse_stride] = (M + log2f(sum)) * 0.69314718055994531f;
 }
 

@@ -67,11 +67,36 @@ __device__ __forceinline__ void q4_params(float lo, float hi, __half& s, __half&
   o = __float2half_rn(__fadd_rn(lo, __fmul_rn(8.f, __half2float(s))));
 }
 
-__device__ __forceinline__ uint32_t q4_code(float x, float s, float o) {
-  if (!(s > 0.f)) return 8u;
-  // rint, then clamped: an infinite x gives an end of the range
-  const float c = rintf(__fdiv_rn(__fsub_rn(x, o), s));
-  return (uint32_t)(int)(fminf(fmaxf(c, -8.f), 7.f) + 8.f);
+// Codes of N values, nibble n = value n.  rint((x - o) / s) by one reciprocal for
+// all of them: the product is within 9 * 2^-23 of the quotient, clamped to 9, so it
+// rounds to the same integer unless it lies that close to a half; those few
+// groups are divided.
+template <int N>
+__device__ __forceinline__ uint32_t q4_codes(const float* x, float s, float o) {
+  uint32_t w = 0;
+  if (!(s > 0.f)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w |= 8u << (4 * i);
+    return w;
+  }
+  const float r = __frcp_rn(s);
+  bool near = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float q = fminf(fmaxf(__fsub_rn(x[i], o) * r, -9.f), 8.f);  // an infinite x gives an end of the range
+    const float c = rintf(q);
+    near |= fabsf(q - c) > 0.49999f;
+    w |= (uint32_t)(int)(fminf(fmaxf(c, -8.f), 7.f) + 8.f) << (4 * i);
+  }
+  if (near) {
+    w = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float c = rintf(__fdiv_rn(__fsub_rn(x[i], o), s));
+      w |= (uint32_t)(int)(fminf(fmaxf(c, -8.f), 7.f) + 8.f) << (4 * i);
+    }
+  }
+  return w;
 }
 
 __device__ __forceinline__ float q4_value(uint32_t code, float s, float o) {

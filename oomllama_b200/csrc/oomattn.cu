@@ -41,16 +41,21 @@ int decode_slots(int kv_dtype, int group) {
   return kv_dtype == OOMATTN_DTYPE_Q4 ? q4_ctas_per_sm(q4_wide(group)) : kDecCtasPerSm;
 }
 typedef void (*DecodeQ4Fn)(const KVPool, const DecodeArgs, const SeqBatch, const DecodeSched);
-DecodeQ4Fn decode_q4_fn(bool wide, bool io16) {
-  if (wide) return io16 ? decode_q4_kernel<true, true> : decode_q4_kernel<true, false>;
-  return io16 ? decode_q4_kernel<false, true> : decode_q4_kernel<false, false>;
+// Types of a decode's q and out: f32 both (a step), or (4-bit cache, the rows of a short prefill) q in bf16.
+enum class DecIo { kF32, kQ16, kQ16Out16 };
+DecodeQ4Fn decode_q4_fn(bool wide, DecIo io) {
+  switch (io) {
+    case DecIo::kQ16: return wide ? decode_q4_kernel<true, true, false> : decode_q4_kernel<false, true, false>;
+    case DecIo::kQ16Out16: return wide ? decode_q4_kernel<true, true, true> : decode_q4_kernel<false, true, true>;
+    default: return wide ? decode_q4_kernel<true, false, false> : decode_q4_kernel<false, false, false>;
+  }
 }
 cudaError_t set_decode_q4_smem() {
   cudaError_t e = cudaSuccess;
   for (bool wide : {false, true})
-    for (bool io16 : {false, true})
+    for (DecIo io : {DecIo::kF32, DecIo::kQ16, DecIo::kQ16Out16})
       if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(decode_q4_fn(wide, io16), cudaFuncAttributeMaxDynamicSharedMemorySize,
+        e = cudaFuncSetAttribute(decode_q4_fn(wide, io), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  q4_smem_bytes(wide));
   return e;
 }
@@ -568,14 +573,16 @@ int launch_qk_norm_append(oomattn_ctx* ctx, const AppendArgs& ap, const NormArgs
       return fail(ctx, OOMATTN_ERR_INVALID_ARG, "tensors, biases and norm weights must be 16-byte aligned");
   const int hq = ctx->cfg.n_heads, hkv = ctx->cfg.n_kv_heads, kv = ctx->cfg.kv_dtype;
   const long long qw = ap.q ? (hq + 3) / 4 : 0, kw = ap.k ? (hkv + 3) / 4 : 0;
-  const long long v_units = kv == OOMATTN_DTYPE_Q4 ? (long long)sb.n * (ap.n_new / 2 + 1) : T;
-  const long long tasks = T * (qw + kw) + v_units * kw;
+  const bool q4 = kv == OOMATTN_DTYPE_Q4;
+  const long long tasks = T * qw + (q4 ? (ap.k ? (long long)T * ((hkv + 1) / 2) : 0) + (long long)sb.n * (ap.n_new / 2 + 1) * kw
+                                       : 2ll * T * kw);
   if (tasks >= (1ll << 26)) return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "%d tokens in one append call", T);
-  const int grid = (int)std::max<long long>(1, std::min<long long>((tasks + 7) / 8, (long long)ctx->num_sms * kQkNormCtasPerSm));
+  const int grid = (int)std::max<long long>(
+      1, std::min<long long>((tasks + kQkNormWarps - 1) / kQkNormWarps, (long long)ctx->num_sms * kQkNormCtasPerSm));
   const KVPool pool = make_pool(ctx);
   cudaError_t le = cudaSuccess;
 #define OOMATTN_QN(I, Q, K) \
-  le = launch_pdl(qk_norm_append_kernel<I, Q, K>, dim3(grid), dim3(256), 0, ctx->stream, ap, na, pool, sb, T)
+  le = launch_pdl(qk_norm_append_kernel<I, Q, K>, dim3(grid), dim3(kQkNormWarps * 32), 0, ctx->stream, ap, na, pool, sb, T)
 #define OOMATTN_QN_IO(K)                                                   \
   do {                                                                     \
     if (ap.in_bf16 && ap.q_out_bf16) OOMATTN_QN(true, true, K);            \
@@ -804,9 +811,8 @@ int q4_max_splits(int rows, int n_kv, int max_pages, int slots) {
   return std::min(kMaxSplitsQ4, kMaxBatch * kMaxSplitsBf16 / rows);
 }
 
-// io16: q and out are bf16 (4-bit cache only).
 int launch_decode_rows(oomattn_ctx* ctx, int layer, const SeqBatch& sb, const float* q, float* out, float* lse,
-                       int o_stride, int lse_stride, bool io16 = false) {
+                       int o_stride, int lse_stride, DecIo io = DecIo::kF32) {
   const int n_kv = ctx->cfg.n_kv_heads;
   const int slots = ctx->num_sms * decode_slots(ctx->cfg.kv_dtype, ctx->group);
   int key[kMaxBatch + 1];
@@ -861,9 +867,9 @@ int launch_decode_rows(oomattn_ctx* ctx, int layer, const SeqBatch& sb, const fl
   } else if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4) {
     cfg.blockDim = dim3(kDecWarps * 32);
     cfg.dynamicSmemBytes = q4_smem_bytes(q4_wide(ctx->group));
-    le = cudaLaunchKernelEx(&cfg, decode_q4_fn(q4_wide(ctx->group), io16), pool, a, sb, sched);
+    le = cudaLaunchKernelEx(&cfg, decode_q4_fn(q4_wide(ctx->group), io), pool, a, sb, sched);
     if (le == cudaSuccess && late)
-      le = launch_pdl(io16 ? merge_splits_kernel<true> : merge_splits_kernel<false>, dim3(sb.n * a.n_heads),
+      le = launch_pdl(io == DecIo::kQ16Out16 ? merge_splits_kernel<true> : merge_splits_kernel<false>, dim3(sb.n * a.n_heads),
                       dim3(kMergeWarps * 32), 0, ctx->stream, a, sb, sched);
   } else {
     cfg.blockDim = dim3(kDecWarps * 32);
@@ -880,7 +886,7 @@ namespace {
 // Decode rows in launches of at most kMaxBatch rows; (row, head) outputs at
 // out + (row * n_heads + head) * o_stride and lse + (row * n_heads + head) * lse_stride.
 int decode_rows_impl(oomattn_ctx* ctx, int layer, int n_rows, const int32_t* seq_ids, const int32_t* lens,
-                     const float* q, float* out, float* lse, int o_stride, int lse_stride, bool io16 = false) {
+                     const float* q, float* out, float* lse, int o_stride, int lse_stride, DecIo io = DecIo::kF32) {
   int rc = check_layer(ctx, layer);
   if (rc) return rc;
   DeviceGuard dg(ctx->device);
@@ -901,10 +907,10 @@ int decode_rows_impl(oomattn_ctx* ctx, int layer, int n_rows, const int32_t* seq
       sb.len[z] = len;
       sb.pos[z] = 0;
     }
-    const size_t es = io16 ? 2 : 4;  // bytes of a q and an out element
-    rc = launch_decode_rows(ctx, layer, sb, (const float*)((const uint8_t*)q + (size_t)r0 * hq * kHeadDim * es),
-                            (float*)((uint8_t*)out + (size_t)r0 * hq * o_stride * es),
-                            lse ? lse + (size_t)r0 * hq * lse_stride : nullptr, o_stride, lse_stride, io16);
+    const size_t qs = io == DecIo::kF32 ? 4 : 2, os = io == DecIo::kQ16Out16 ? 2 : 4;  // bytes of an element
+    rc = launch_decode_rows(ctx, layer, sb, (const float*)((const uint8_t*)q + (size_t)r0 * hq * kHeadDim * qs),
+                            (float*)((uint8_t*)out + (size_t)r0 * hq * o_stride * os),
+                            lse ? lse + (size_t)r0 * hq * lse_stride : nullptr, o_stride, lse_stride, io);
     if (rc) return rc;
   }
   return OOMATTN_OK;
@@ -1026,12 +1032,17 @@ int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtenso
 }
 
 // Prefill over a 4-bit cache, few tokens (drafts to verify, a short tail of a
-// prompt): each as one decode row that sees the slots up to its own.
-constexpr int kQ4PrefillRows = 16;
-int q4_prefill_rows(oomattn_ctx* ctx, int layer, int seq, int n_new, const void* q, void* out, float* lse) {
+// prompt): each as one decode row that sees the slots up to its own.  Up to 24
+// tokens: by rows and expanded 14.8 and 24.7 us behind 2000 tokens (28q/4kv),
+// 54.0 and 59.5 behind 9001 (32q/8kv), 116 and 123 behind 30000 (28q/4kv); at
+// 32 tokens 18.1 and 24.7, 76.6 and 59.5, 154 and 123.
+constexpr int kQ4PrefillRows = 24;
+int q4_prefill_rows(oomattn_ctx* ctx, int layer, int seq, int n_new, const void* q, void* out, int out_dtype,
+                    float* lse) {
   if (!q || !out) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad prefill arguments");
   int rc = check_layer(ctx, layer);
   if (!rc) rc = check_seq(ctx, seq);
+  if (!rc) rc = validate_dtype(ctx, out_dtype, "prefill out");
   if (rc) return rc;
   if (!aligned16(q) || !aligned16(out)) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
   const int L = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq];
@@ -1039,7 +1050,8 @@ int q4_prefill_rows(oomattn_ctx* ctx, int layer, int seq, int n_new, const void*
   std::vector<int32_t> rows(n_new, seq), lens(n_new);
   for (int i = 0; i < n_new; ++i) lens[i] = L - n_new + i + 1;
   return decode_rows_impl(ctx, layer, n_new, rows.data(), lens.data(), static_cast<const float*>(q),
-                          static_cast<float*>(out), lse, kHeadDim, 1, true);
+                          static_cast<float*>(out), lse, kHeadDim, 1,
+                          out_dtype == OOMATTN_DTYPE_BF16 ? DecIo::kQ16Out16 : DecIo::kQ16);
 }
 }  // namespace
 
@@ -1595,8 +1607,8 @@ int oomattn_prefill(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_new,
                     int32_t out_dtype, float* lse) {
   if (!ctx) return OOMATTN_ERR_INVALID_ARG;
   if (n_new <= 0) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad prefill arguments");
-  if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4 && out_dtype == OOMATTN_DTYPE_BF16 && n_new <= kQ4PrefillRows)
-    return q4_prefill_rows(ctx, layer, seq, n_new, q, out, lse);
+  if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4 && n_new <= kQ4PrefillRows)
+    return q4_prefill_rows(ctx, layer, seq, n_new, q, out, out_dtype, lse);
   const int32_t all[2] = {0, (n_new + 255) / 256};
   return oomattn_prefill_blocks(ctx, layer, seq, n_new, q, out, out_dtype, lse, 1, all);
 }
@@ -1991,7 +2003,7 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
     decode_bf16_kernel<<<n_items, (kDecWarps + 1) * 32, kDecSmemBytes, st>>>(maps[0], maps[1], pool, a, sb, sched);
   } else if (kv_dtype == OOMATTN_DTYPE_Q4) {
     const bool wide = q4_wide(n_heads / n_kv_heads);
-    decode_q4_fn(wide, false)<<<n_items, kDecWarps * 32, q4_smem_bytes(wide), st>>>(pool, a, sb, sched);
+    decode_q4_fn(wide, DecIo::kF32)<<<n_items, kDecWarps * 32, q4_smem_bytes(wide), st>>>(pool, a, sb, sched);
   } else {
     decode_f32_kernel<<<n_items, kDecWarps * 32, 0, st>>>(pool, a, sb, sched);
   }
