@@ -58,7 +58,7 @@ typedef enum oomattn_status {
 enum { OOMATTN_DTYPE_F32 = 0, OOMATTN_DTYPE_BF16 = 1, OOMATTN_DTYPE_Q4 = 2 };
 /* The 4-bit cache.  The 128 values of a (token, kv head) row of K or V are
  * four groups of 32.  With x a group,
- *   s = f16(bf16((max x - min x) / 15)), o = f16(min x + 8 s),
+ *   s = f16(bf16((max x - min x) * (1/15))), o = f16(min x + 8 s),
  *   c = clamp(rint((x - o) / s) + 8, 0, 15)   (8 where s = 0)
  * and the row stands for o + (c - 8) s: 80 bytes instead of 256 in bf16, each
  * value off by at most 0.53 s + 2^-12 |o|.  Values saturate at +-60000; a

@@ -116,6 +116,15 @@ __device__ __forceinline__ uint32_t f16_part(float a, float b, bool low) {
   const uint32_t hi = pack_f16(a, b);
   return low ? pack_f16(a - h_lo(hi), b - h_hi(hi)) : hi;
 }
+// The query's parts times `by` (1 or 1/16), |a|, |b| < 2^15: the high part a
+// multiple of 16, so that its products with 32 codes add up to less than 2^20
+// such units and the tensor core's accumulator holds the sum exactly (it
+// truncates: with the high part rounded to its own 11 bits the decode's error
+// was twice as large); the low part, at most 8, is rounded to 2^-9.
+__device__ __forceinline__ uint32_t q_part(float a, float b, float by, bool low) {
+  const float ha = rintf(a * 0.0625f) * 16.f, hb = rintf(b * 0.0625f) * 16.f;
+  return low ? pack_f16((a - ha) * by, (b - hb) * by) : pack_f16(ha * by, hb * by);
+}
 
 // Q16, OUT16: q and out in bf16 (the newest tokens of a sequence as one row each)
 // instead of f32 (a generation step).
@@ -260,8 +269,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
         uint32_t v[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          v[2 * i] = f16_part(x[w][2 * i], x[w][2 * i + 4], low);
-          v[2 * i + 1] = f16_part(x[w][2 * i + 1] * 0.0625f, x[w][2 * i + 5] * 0.0625f, low);
+          v[2 * i] = q_part(x[w][2 * i], x[w][2 * i + 4], 1.f, low);
+          v[2 * i + 1] = q_part(x[w][2 * i + 1], x[w][2 * i + 5], 0.0625f, low);
         }
         if (warp == 0) s_q[(w * HL + h) * 32 + lane] = make_uint4(v[0], v[1], v[2], v[3]);
       }
@@ -355,9 +364,16 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
           const float s0 = wl ? h_hi(sk[2 * pg]) : h_lo(sk[2 * pg]), s1 = wl ? h_hi(sk[2 * pg + 1]) : h_lo(sk[2 * pg + 1]);
           float e[4];
           mma_f16_16816_z(e, f0, q0.x, q0.y);
-          if (WIDE) mma_f16_16816(e, f0, q1.x, q1.y);
           mma_f16_16816(e, f1, q0.z, q0.w);
-          if (WIDE) mma_f16_16816(e, f1, q1.z, q1.w);
+          if (WIDE) {  // the low parts by themselves: added onto the high ones they would be truncated at those' size
+            float el[4];
+            mma_f16_16816_z(el, f0, q1.x, q1.y);
+            mma_f16_16816(el, f1, q1.z, q1.w);
+            sc[0][2 * pg] = fmaf(el[0], s0, sc[0][2 * pg]);
+            sc[HL - 1][2 * pg] = fmaf(el[1], s0, sc[HL - 1][2 * pg]);
+            sc[0][2 * pg + 1] = fmaf(el[2], s1, sc[0][2 * pg + 1]);
+            sc[HL - 1][2 * pg + 1] = fmaf(el[3], s1, sc[HL - 1][2 * pg + 1]);
+          }
           sc[0][2 * pg] = fmaf(e[0], s0, sc[0][2 * pg]);
           sc[HL - 1][2 * pg] = fmaf(e[1], s0, sc[HL - 1][2 * pg]);
           sc[0][2 * pg + 1] = fmaf(e[2], s1, sc[0][2 * pg + 1]);
@@ -458,9 +474,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint32_t av[4] = {b[0][2 * i], b[0][2 * i + 1], b[1][2 * i], b[1][2 * i + 1]};
-            if (pg == 0) mma_f16_16816_z(e[i], av, pb[0][0], pb[0][1]);
-            else mma_f16_16816(e[i], av, pb[0][2], pb[0][3]);
-            if (WIDE) mma_f16_16816(e[i], av, pb[HL - 1][2 * pg], pb[HL - 1][2 * pg + 1]);
+            if (pg == 0) mma_f16_16816_z(e[i], av, pb[HL - 1][0], pb[HL - 1][1]);
+            else mma_f16_16816(e[i], av, pb[HL - 1][2], pb[HL - 1][3]);
+            if (WIDE) mma_f16_16816(e[i], av, pb[0][2 * pg], pb[0][2 * pg + 1]);
           }
         }
 #pragma unroll

@@ -4,7 +4,7 @@
 // A page of 16 tokens of one kv head is a chunk of 1280 bytes of K and, right
 // behind it (one copy brings both), one of V.  The 128 values of a token are four groups of 32; with x
 // the group,
-//   s = f16(bf16((max x - min x) / 15))      (f32 division; 8 significant bits)
+//   s = f16(bf16((max x - min x) * (1/15)))  (f32; 8 significant bits)
 //   o = f16(min x + 8 s)
 //   c = clamp(rint((x - o) / s) + 8, 0, 15)  (8 where s = 0)
 // and the group stands for o + (c - 8) s.  The roundings: a code is off by at
@@ -63,7 +63,7 @@ __device__ __forceinline__ void q4_params(float lo, float hi, __half& s, __half&
   }
   lo = fminf(fmaxf(lo, -kQ4Sat), kQ4Sat);
   hi = fminf(fmaxf(hi, -kQ4Sat), kQ4Sat);
-  s = __float2half_rn(__bfloat162float(__float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f))));
+  s = __float2half_rn(__bfloat162float(__float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f))));
   o = __float2half_rn(__fadd_rn(lo, __fmul_rn(8.f, __half2float(s))));
 }
 

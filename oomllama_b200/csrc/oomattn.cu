@@ -13,6 +13,8 @@
 
 #include <algorithm>
 #include <string>
+#include <system_error>
+#include <thread>
 #include <vector>
 
 #include "../../include/oomattn.h"
@@ -195,7 +197,10 @@ struct DeviceGuard {
 // f32 RoPE table exactly as the reference builds it on the host
 // (src/oomllama_turbo.rs:753-761): inv_freq = 1 / theta^(2i/d) with f32 powf,
 // angle = (f32)pos * inv_freq, cos/sin in f32.
-void build_rope_table(float theta, int n_pos, std::vector<float>& c, std::vector<float>& s) {
+// rounded: cos and sin of the f32 angle correctly rounded instead of the C
+// library's cosf and sinf, whose last bit differs from version to version: the
+// codes of a 4-bit cache hang on it.  The rows are built by several threads.
+void build_rope_table(float theta, int n_pos, std::vector<float>& c, std::vector<float>& s, bool rounded = false) {
   const int half = kHeadDim / 2;
   std::vector<float> inv(half);
   for (int i = 0; i < half; ++i) {
@@ -204,14 +209,30 @@ void build_rope_table(float theta, int n_pos, std::vector<float>& c, std::vector
   }
   c.resize((size_t)n_pos * half);
   s.resize((size_t)n_pos * half);
-  for (int p = 0; p < n_pos; ++p) {
-    const float pos = (float)p;
-    for (int i = 0; i < half; ++i) {
-      volatile float a = pos * inv[i];
-      c[(size_t)p * half + i] = cosf(a);
-      s[(size_t)p * half + i] = sinf(a);
+  auto rows = [&](int from, int to) {
+    for (int p = from; p < to; ++p) {
+      const float pos = (float)p;
+      for (int i = 0; i < half; ++i) {
+        volatile float a = pos * inv[i];
+        c[(size_t)p * half + i] = rounded ? (float)cos((double)a) : cosf(a);
+        s[(size_t)p * half + i] = rounded ? (float)sin((double)a) : sinf(a);
+      }
     }
+  };
+  const int n_threads = std::max(1, std::min({n_pos / 2048, (int)std::thread::hardware_concurrency(), 16}));
+  std::vector<std::thread> threads;
+  int from = 0;
+  for (int t = 1; t < n_threads; ++t) {
+    const int to = (int)((long long)n_pos * t / n_threads);
+    try {
+      threads.emplace_back(rows, from, to);
+    } catch (const std::system_error&) {  // no thread to be had: this one does the rest
+      break;
+    }
+    from = to;
   }
+  rows(from, n_pos);
+  for (std::thread& t : threads) t.join();
 }
 
 int encode_pool_map(oomattn_ctx* ctx, void* base, uint64_t n_pages, CUtensorMap* map) {
@@ -1109,7 +1130,7 @@ int oomattn_create(const oomattn_config* cfg, int device, void* stream, oomattn_
   if (cudaMemcpy(ctx->d_block_table, ctx->h_block_table.data(), bt_n * sizeof(int), cudaMemcpyHostToDevice) !=
       cudaSuccess)
     return bail(OOMATTN_ERR_CUDA);
-  build_rope_table(c.rope_theta, c.max_seq_len, ctx->h_cos, ctx->h_sin);
+  build_rope_table(c.rope_theta, c.max_seq_len, ctx->h_cos, ctx->h_sin, c.kv_dtype == OOMATTN_DTYPE_Q4);
   const size_t tab = ctx->h_cos.size() * sizeof(float);
   if (cudaMalloc(&ctx->d_cos, tab) != cudaSuccess || cudaMalloc(&ctx->d_sin, tab) != cudaSuccess)
     return bail(OOMATTN_ERR_NO_MEMORY);

@@ -12,7 +12,7 @@ def quantize(x):
     nan = torch.isnan(g).any(-1)
     lo, hi = (torch.nan_to_num(t, nan=0.0, posinf=math.inf, neginf=-math.inf).clamp(-60000, 60000)
               for t in (g.amin(-1), g.amax(-1)))
-    s = ((hi - lo) / 15).bfloat16().half().float()
+    s = ((hi - lo) * (torch.ones(()) / 15)).bfloat16().half().float()
     o = (lo + 8 * s).half().float()
     s, o = torch.where(nan, 0.0, s), torch.where(nan, math.nan, o)
     d = torch.where(s[..., None] > 0, (g - o[..., None]) / s[..., None], torch.zeros(()))
