@@ -30,6 +30,7 @@
 
 #include "common.cuh"
 #include "params.cuh"
+#include "rope_append.cuh"
 
 namespace oomattn {
 
@@ -189,11 +190,11 @@ __global__ void __launch_bounds__(128)
         const float o = __half2float(__ushort_as_half((uint16_t)(o2 >> (16 * q))));
         const float s = __half2float(__ushort_as_half((uint16_t)(s2 >> (16 * q))));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {  // t and t + 1 of this group: 16 dims in a row
-          float x[4];
+        for (int e = 0; e < 2; ++e) {  // t and t + 1 of this group: 16 dims in a row
+          float x[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = q4_value((w[2 * (e >> 1) + q] >> (16 * (e & 1) + 4 * i)) & 15u, s, o);
-          store4<OUT_BF16>(out, at(slot, 32 * (2 * wp + q) + 8 * t + 4 * e), wanted(slot) ? x : zero);
+          for (int i = 0; i < 8; ++i) x[i] = wanted(slot) ? q4_value((w[2 * e + q] >> (4 * i)) & 15u, s, o) : 0.f;
+          store8<OUT_BF16>(out, at(slot, 32 * (2 * wp + q) + 8 * (t + e)), x);
         }
       }
     } else {

@@ -824,11 +824,13 @@ int plan_decode(const SeqBatch& sb, int n_kv, int slots, int max_splits, int fil
 }
 
 // The most splits of a row of a 4-bit decode.  32, which the last CTA of a row
-// joins; where that leaves SMs idle although the longest row has many pages for
-// each split, as many as the partials' memory holds for so few rows.
-constexpr int kQ4LatePages = 200;
+// joins (merge_splits_staged), where the rows fill the GPU with them: a merge
+// kernel after the decode costs 64 ragged rows of 28q/4kv 64.8 us instead of
+// 61.8.  Where they do not, that kernel is the faster way to join any number
+// (one row of 8q/1kv: 1500 tokens 6.2 us instead of 7.0, 4096 6.9 instead of
+// 10.5), so as many as the partials' memory holds for so few rows.
 int q4_max_splits(int rows, int n_kv, int max_pages, int slots) {
-  if (rows * n_kv * kMaxSplitsBf16 >= slots || max_pages < kQ4LatePages) return kMaxSplitsBf16;
+  if (rows * n_kv * kMaxSplitsBf16 >= slots || max_pages <= decode_min_pages(OOMATTN_DTYPE_Q4)) return kMaxSplitsBf16;
   return std::min(kMaxSplitsQ4, kMaxBatch * kMaxSplitsBf16 / rows);
 }
 

@@ -214,6 +214,26 @@ def test_decode_lens_packed_and_many_rows():
     eng.close()
 
 
+@pytest.mark.parametrize("heads", [(8, 1), (4, 1)])
+def test_many_splits_merged_after(heads):
+    """One long row of one kv head: more splits than the decode's last CTA joins, f32, packed and bf16 outputs, beside
+    a short row, an empty one and one of a single split."""
+    lens = [30000, 0, 100, 3001]
+    eng, ks, vs = _filled(*heads, lens, seed=15, dtype=torch.float32)
+    out = _check_decode(eng, heads[0], lens, ks, vs, 15)
+    q = randn((4, heads[0], 128), 15 + 77).cuda()
+    packed = eng.decode_packed(0, [0, 1, 2, 3], q)
+    np.testing.assert_array_equal(packed[..., :128].cpu().numpy(), out.cpu().numpy())
+    for _ in range(3):
+        assert torch.equal(eng.decode(0, [0, 1, 2, 3], q), out)
+    q16 = randn((2, heads[0], 128), 16, torch.bfloat16)
+    want, _ = q4_ref.attend(q16, ks[0], vs[0], [29999, 30000])
+    for dt in (torch.float32, torch.bfloat16):
+        got = eng.prefill(0, 0, q16.cuda(), out_dtype=dt)
+        assert_close(as_f32_np(got), want, ATOL + (2.0 ** -8 if dt == torch.bfloat16 else 0), BF16_RTOL, what="rows")
+    eng.close()
+
+
 def test_nan_reaches_only_rows_that_see_it():
     n = 40
     k, v = randn((n, 2, 128), 1), randn((n, 2, 128), 2)
@@ -265,7 +285,7 @@ def test_decode_static_scratch(lib):
 
 # ----------------------------------------------------------------------------------------------- prefill
 @pytest.mark.parametrize("heads", [(28, 4), (8, 8)])
-@pytest.mark.parametrize("n_new,prefix", [(1, 0), (1, 50), (7, 9), (16, 100), (17, 0), (17, 111), (100, 28), (300, 500)])
+@pytest.mark.parametrize("n_new,prefix", [(1, 0), (1, 50), (7, 9), (16, 100), (24, 0), (25, 0), (25, 111), (100, 28), (300, 500)])
 @pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
 def test_prefill(heads, n_new, prefix, out_dtype):
     n = n_new + prefix
