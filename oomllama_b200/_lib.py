@@ -171,6 +171,7 @@ def load():
 
 def int_array(values):
     """A C int32 array of `values` (one element at least, so that it has an address)."""
+    values = values if isinstance(values, (list, tuple, range)) else list(values)
     try:
         a = array("i", values)
     except TypeError:  # numbers that are no integers of their own

@@ -121,6 +121,11 @@ __host__ __device__ __forceinline__ int q4_v_meta(int tok) {  // the pair's 4 x 
 }
 
 // ---------------------------------------------------------------- rows read back
+__global__ void iota_kernel(int* p, int n) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n) p[i] = i;
+}
+
 struct GatherArgs {
   void* k_out;
   void* v_out;

@@ -128,7 +128,8 @@ struct oomattn_ctx {
   // prefill over a 4-bit cache: one sequence's rows of one layer as bf16 pages
   // [exp_pages + 1][n_kv][16][128] of K, then of V (the last page zero), and the
   // block table that names them in order
-  std::vector<void*> exp_blocks;
+  void* exp_blocks[64] = {};  // all that were allocated, each at least half as large again as the one before
+  int n_exp_blocks = 0;
   uint8_t* d_exp = nullptr;
   int exp_pages = 0;
   int* d_exp_table = nullptr;
@@ -221,6 +222,7 @@ void build_rope_table(float theta, int n_pos, std::vector<float>& c, std::vector
   };
   const int n_threads = std::max(1, std::min({n_pos / 2048, (int)std::thread::hardware_concurrency(), 16}));
   std::vector<std::thread> threads;
+  threads.reserve(n_threads);  // nothing but the start of a thread can fail below
   int from = 0;
   for (int t = 1; t < n_threads; ++t) {
     const int to = (int)((long long)n_pos * t / n_threads);
@@ -1001,7 +1003,7 @@ int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtenso
   const size_t page_bytes = (size_t)n_kv * kPageSize * kHeadDim * 2;
   if (pages > ctx->exp_pages) {
     const int cap = pages + pages / 2;  // a growing sequence does not reallocate at every chunk
-    if ((long long)(cap + 1) * n_kv * kPageSize >= (1ll << 31))
+    if ((long long)(cap + 1) * n_kv * kPageSize >= (1ll << 31) || ctx->n_exp_blocks == 64)
       return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "prefill over %d tokens of a 4-bit cache", L);
     cudaStreamCaptureStatus cap_st = cudaStreamCaptureStatusNone;
     CK(cudaStreamIsCapturing(ctx->stream, &cap_st));
@@ -1016,16 +1018,15 @@ int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtenso
       cudaGetLastError();
       return fail(ctx, OOMATTN_ERR_NO_MEMORY, "prefill scratch of %zu bytes failed", bytes);
     }
-    ctx->exp_blocks.push_back(p);
+    ctx->exp_blocks[ctx->n_exp_blocks++] = p;
     uint8_t* b = static_cast<uint8_t*>(p);
-    std::vector<int> table(cap);
-    for (int i = 0; i < cap; ++i) table[i] = i;
+    int* table = reinterpret_cast<int*>(b + 2 * half_bytes);
     CK(cudaMemsetAsync(b + half_bytes - page_bytes, 0, page_bytes, ctx->stream));  // the null pages
     CK(cudaMemsetAsync(b + 2 * half_bytes - page_bytes, 0, page_bytes, ctx->stream));
-    CK(cudaMemcpyAsync(b + 2 * half_bytes, table.data(), (size_t)cap * sizeof(int), cudaMemcpyHostToDevice, ctx->stream));
-    CK(cudaStreamSynchronize(ctx->stream));  // the host table ends here
+    iota_kernel<<<(cap + 255) / 256, 256, 0, ctx->stream>>>(table, cap);
+    CKLAUNCH();
     ctx->d_exp = b;
-    ctx->d_exp_table = reinterpret_cast<int*>(b + 2 * half_bytes);
+    ctx->d_exp_table = table;
     ctx->exp_pages = cap;
   }
   const size_t half = (size_t)(ctx->exp_pages + 1) * page_bytes;
@@ -1070,9 +1071,12 @@ int q4_prefill_rows(oomattn_ctx* ctx, int layer, int seq, int n_new, const void*
   if (!aligned16(q) || !aligned16(out)) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
   const int L = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq];
   if (n_new > L) return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "n_new %d exceeds the cached length %d", n_new, L);
-  std::vector<int32_t> rows(n_new, seq), lens(n_new);
-  for (int i = 0; i < n_new; ++i) lens[i] = L - n_new + i + 1;
-  return decode_rows_impl(ctx, layer, n_new, rows.data(), lens.data(), static_cast<const float*>(q),
+  int32_t rows[kQ4PrefillRows], lens[kQ4PrefillRows];
+  for (int i = 0; i < n_new; ++i) {
+    rows[i] = seq;
+    lens[i] = L - n_new + i + 1;
+  }
+  return decode_rows_impl(ctx, layer, n_new, rows, lens, static_cast<const float*>(q),
                           static_cast<float*>(out), lse, kHeadDim, 1,
                           out_dtype == OOMATTN_DTYPE_BF16 ? DecIo::kQ16Out16 : DecIo::kQ16);
 }
@@ -1195,7 +1199,7 @@ int oomattn_destroy(oomattn_ctx* ctx) {
                   ctx->d_argmax_part, ctx->d_kf, ctx->d_pf_part};
   for (void* p : ptrs)
     if (p) cudaFree(p);
-  for (void* p : ctx->exp_blocks) cudaFree(p);
+  for (int i = 0; i < ctx->n_exp_blocks; ++i) cudaFree(ctx->exp_blocks[i]);
   delete ctx;
   return OOMATTN_OK;
 }
@@ -1323,10 +1327,10 @@ int oomattn_kv_read(oomattn_ctx* ctx, int32_t layer, int32_t seq, void* k_out, v
   const int L = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq];
   const int n_kv = ctx->cfg.n_kv_heads;
   if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4) {
-    std::vector<uint8_t> chunk(kQ4Chunk);
+    uint8_t chunk[kQ4Chunk];
     auto half_at = [&](int off) {
       __half h;
-      memcpy(&h, chunk.data() + off, 2);
+      memcpy(&h, chunk + off, 2);
       return __half2float(h);
     };
     for (int lp = 0; lp * kPageSize < L; ++lp) {
@@ -1335,7 +1339,7 @@ int oomattn_kv_read(oomattn_ctx* ctx, int32_t layer, int32_t seq, void* k_out, v
       for (int g = 0; g < n_kv; ++g)
         for (int which = 0; which < 2; ++which) {
           const size_t off = (((size_t)layer * ctx->n_pool_pages + pg) * n_kv + g) * kQ4Pair + which * kQ4Chunk;
-          CK(cudaMemcpy(chunk.data(), (const uint8_t*)ctx->kpool + off, kQ4Chunk, cudaMemcpyDeviceToHost));
+          CK(cudaMemcpy(chunk, (const uint8_t*)ctx->kpool + off, kQ4Chunk, cudaMemcpyDeviceToHost));
           float* dst = (float*)(which ? v_out : k_out) + ((size_t)g * L + (size_t)lp * kPageSize) * kHeadDim;
           for (int r = 0; r < nt; ++r)
             for (int d = 0; d < kHeadDim; ++d) {

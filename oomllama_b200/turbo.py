@@ -256,9 +256,10 @@ class TurboEngine:
         """The oomattn_qk_norm of two weights [128] f32 (either may be None), or None without any."""
         if q_norm is None and k_norm is None:
             return None
-        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-            if w is not None:
-                _dev(w, name, self.device, dtype=torch.float32, numel=HEAD_DIM)
+        if q_norm is not None:
+            _dev(q_norm, "q_norm", self.device, dtype=torch.float32, numel=HEAD_DIM)
+        if k_norm is not None:
+            _dev(k_norm, "k_norm", self.device, dtype=torch.float32, numel=HEAD_DIM)
         return _lib.QkNorm(None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
                            float(eps))
 
@@ -271,25 +272,28 @@ class TurboEngine:
         seq_ids = list(seq_ids)
         starts = None if starts is None else list(starts)
         _same_count(starts, seq_ids, "starts")
-        T = q.shape[0]
-        if not seq_ids or T % len(seq_ids):
+        T, n_seqs = q.size(0), len(seq_ids)
+        if not n_seqs or T % n_seqs:
             raise ValueError("token count is not a multiple of the number of sequences")
-        n_new = T // len(seq_ids)
-        c = self.config
-        _dev(q, "q", self.device, numel=T * c.n_heads * HEAD_DIM)
-        _dev(k, "k", self.device, dtype=q.dtype, numel=T * c.n_kv_heads * HEAD_DIM)
-        _dev(v, "v", self.device, dtype=q.dtype, numel=T * c.n_kv_heads * HEAD_DIM)
-        for b, n in ((bq, c.n_heads), (bk, c.n_kv_heads), (bv, c.n_kv_heads)):
-            if b is not None:
-                _dev(b, "bias", self.device, dtype=torch.float32, numel=n * HEAD_DIM)
+        n_new = T // n_seqs
+        hq, nk = self.config.n_heads, T * self.config.n_kv_heads * HEAD_DIM
+        _dev(q, "q", self.device, numel=T * hq * HEAD_DIM)
+        _dev(k, "k", self.device, dtype=q.dtype, numel=nk)
+        _dev(v, "v", self.device, dtype=q.dtype, numel=nk)
+        if bq is not None:
+            _dev(bq, "bias", self.device, dtype=torch.float32, numel=hq * HEAD_DIM)
+        if bk is not None:
+            _dev(bk, "bias", self.device, dtype=torch.float32, numel=self.config.n_kv_heads * HEAD_DIM)
+        if bv is not None:
+            _dev(bv, "bias", self.device, dtype=torch.float32, numel=self.config.n_kv_heads * HEAD_DIM)
         if q_out is None:
-            q_out = torch.empty((T, c.n_heads, HEAD_DIM), dtype=q_out_dtype, device=self._torch_device)
+            q_out = torch.empty(T, hq, HEAD_DIM, dtype=q_out_dtype, device=q.device)
         else:
-            _dev(q_out, "q_out", self.device, dtype=q_out_dtype, numel=T * c.n_heads * HEAD_DIM)
+            _dev(q_out, "q_out", self.device, dtype=q_out_dtype, numel=T * hq * HEAD_DIM)
         norm = self._qk_norm(q_norm, k_norm, eps)
         self._bind_stream()
         check(self._ctx, self._L.oomattn_rope_append_qk_norm(
-            self._ctx, layer, len(seq_ids), int_array(seq_ids), None if starts is None else int_array(starts), n_new,
+            self._ctx, layer, n_seqs, int_array(seq_ids), None if starts is None else int_array(starts), n_new,
             _ptr(q), _ptr(k), _ptr(v), _dtype_code(q), _ptr(bq), _ptr(bk), _ptr(bv), norm, _ptr(q_out),
             _DT[q_out_dtype]))
         return q_out
@@ -342,9 +346,9 @@ class TurboEngine:
         rows = len(seq_ids)
         _dev(q, "q", self.device, dtype=torch.float32, numel=rows * c.n_heads * HEAD_DIM)
         if out is None:
-            out = torch.empty((rows, c.n_heads, HEAD_DIM), dtype=torch.float32, device=self._torch_device)
+            out = torch.empty(rows, c.n_heads, HEAD_DIM, dtype=torch.float32, device=q.device)
         if with_lse and lse is None:
-            lse = torch.empty((rows, c.n_heads), dtype=torch.float32, device=self._torch_device)
+            lse = torch.empty(rows, c.n_heads, dtype=torch.float32, device=q.device)
         self._bind_stream()
         check(self._ctx, self._L.oomattn_decode(
             self._ctx, layer, rows, int_array(seq_ids), None if lens is None else int_array(lens), _ptr(q),
@@ -778,7 +782,7 @@ class Q8Model:
 
     def c_norms(self, engine: "TurboEngine"):
         """The layers' oomattn_qk_norm array, or None where no layer norms its heads."""
-        norms = [engine._qk_norm(l.q_norm, l.k_norm, l.eps) for l in self.layers]
-        if not any(norms):
+        if all(l.q_norm is None and l.k_norm is None for l in self.layers):
             return None
+        norms = [engine._qk_norm(l.q_norm, l.k_norm, l.eps) for l in self.layers]
         return (_lib.QkNorm * len(norms))(*[n or _lib.QkNorm(None, None, 0.0) for n in norms])

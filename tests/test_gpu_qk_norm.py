@@ -69,7 +69,8 @@ def test_append(kv_dtype, variant, theta, dtype, bias, heads):
 
 @pytest.mark.parametrize("kv_dtype", ["q4", "bf16", "f32"])
 @pytest.mark.parametrize("n_new", [1, 2, 3, 16, 31])
-def test_starts_give_up_rows(kv_dtype, n_new):
+@pytest.mark.parametrize("norm", [True, False])
+def test_starts_give_up_rows(kv_dtype, n_new, norm):
     """Drafts replaced from a slot on: the rows before it stay, those behind it are the new ones, alone and in a batch
     where every sequence starts on its own parity."""
     n, n_kv, starts = 60, 2, [7, 12, 60, 0]
@@ -79,7 +80,7 @@ def test_starts_give_up_rows(kv_dtype, n_new):
         eng.kv_write(0, s, k, -k)
     before = [eng.kv_read(0, s) for s in range(4)]
     q, k, v, _, w = _inputs(4 * n_new, 4, n_kv, torch.float32, 40, False)
-    eng.rope_append(0, [0, 1, 2, 3], q.cuda(), k.cuda(), v.cuda(), k_norm=w[1].cuda(), starts=starts)
+    eng.rope_append(0, [0, 1, 2, 3], q.cuda(), k.cuda(), v.cuda(), k_norm=w[1].cuda() if norm else None, starts=starts)
     eng.sync()
     for s, at in enumerate(starts):
         assert eng.seq_len(0, s) == at + n_new
@@ -87,7 +88,7 @@ def test_starts_give_up_rows(kv_dtype, n_new):
         np.testing.assert_array_equal(as_f32_np(kc[:, :at]), as_f32_np(before[s][0][:, :at]))
         np.testing.assert_array_equal(as_f32_np(vc[:, :at]), as_f32_np(before[s][1][:, :at]))
         rows = slice(s * n_new, (s + 1) * n_new)
-        kr = q4_ref.normed_rope(k[rows].view(n_new, n_kv, 128), None, w[1], 1e-6, np.arange(at, at + n_new), 1e6,
+        kr = q4_ref.normed_rope(k[rows].view(n_new, n_kv, 128), None, w[1] if norm else None, 1e-6, np.arange(at, at + n_new), 1e6,
                                 "interleaved")
         bound = q4_ref.code_bound(kr) if kv_dtype == "q4" else F32 + (2.0 ** -8 * kr.abs() if kv_dtype == "bf16" else 0)
         assert ((kc[:, at:].double().transpose(0, 1) - kr).abs() <= bound).all()
