@@ -136,9 +136,12 @@ struct GatherArgs {
   int* status;
 };
 
-template <bool BF16>
+enum : int { kOutF32 = 0, kOutBf16 = 1, kOutF16 = 2 };
+template <int OUT>
 __device__ __forceinline__ void store4(void* p, size_t i, const float* x) {
-  if (BF16) {
+  if (OUT == kOutF16) {
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]));
+  } else if (OUT == kOutBf16) {
     *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
   } else {
     *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = make_float4(x[0], x[1], x[2], x[3]);
@@ -149,7 +152,7 @@ __device__ __forceinline__ void store4(void* p, size_t i, const float* x) {
 // values.  One CTA of 128 threads per (row, page, kv head): 64 threads read the
 // K chunk, 64 the V chunk; a thread's 128-bit load is 32 codes (4-bit cache).
 // Bound by bytes: a 4-bit page is 2.5 KB read for 8 KB (bf16) written.
-template <int KV, bool OUT_BF16>
+template <int KV, int OUT>
 __global__ void __launch_bounds__(128)
     kv_gather_kernel(const GatherArgs a, const KVPool pool, const __grid_constant__ SeqBatch sb) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -199,7 +202,12 @@ __global__ void __launch_bounds__(128)
           float x[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = wanted(slot) ? q4_value((w[2 * e + q] >> (4 * i)) & 15u, s, o) : 0.f;
-          store8<OUT_BF16>(out, at(slot, 32 * (2 * wp + q) + 8 * (t + e)), x);
+          const size_t d = at(slot, 32 * (2 * wp + q) + 8 * (t + e));
+          if (OUT == kOutF16)
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + d) =
+                make_uint4(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
+          else
+            store8<OUT == kOutBf16>(out, d, x);
         }
       }
     } else {
@@ -220,7 +228,7 @@ __global__ void __launch_bounds__(128)
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = q4_value((w[2 * tt + q] >> (16 * p + 4 * i)) & 15u, s, o);
-            store4<OUT_BF16>(out, at(slot, 32 * (2 * wp + q) + 4 * gg), wanted(slot) ? x : zero);
+            store4<OUT>(out, at(slot, 32 * (2 * wp + q) + 4 * gg), wanted(slot) ? x : zero);
           }
         }
       }
@@ -240,7 +248,7 @@ __global__ void __launch_bounds__(128)
         const float4 v = *reinterpret_cast<const float4*>(c + (size_t)i * 16);
         x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
       }
-      store4<OUT_BF16>(out, at(slot, d), x);
+      store4<OUT>(out, at(slot, d), x);
     }
   }
 }

@@ -109,7 +109,7 @@ struct oomattn_ctx {
   int* d_status = nullptr;
   CUtensorMap kmap{}, vmap{};
   bool have_maps = false;
-  int prefill_regs = 0;  // compiled register count of the prefill kernel
+  int prefill_regs[2] = {0, 0};  // compiled register counts of the prefill kernel (bf16 pages, fp16 pages)
   int kf_q8_regs = 0;    // and of the Q8 tensor-core linear (its register split needs kKfLaunchRegs)
   // host mirrors (authoritative for lengths; updated at enqueue time)
   std::vector<int> h_block_table;  // [max_seqs][max_pages_per_seq]
@@ -125,7 +125,7 @@ struct oomattn_ctx {
   // key-split prefill: the chunks' partial O and lse
   uint8_t* d_pf_part = nullptr;
   size_t pf_part_bytes = 0;
-  // prefill over a 4-bit cache: one sequence's rows of one layer as bf16 pages
+  // prefill over a 4-bit cache: one sequence's rows of one layer as fp16 pages
   // [exp_pages + 1][n_kv][16][128] of K, then of V (the last page zero), and the
   // block table that names them in order
   void* exp_blocks[64] = {};  // all that were allocated, each at least half as large again as the one before
@@ -957,19 +957,20 @@ cudaError_t launch_gemv(const GemvArgs& ga, const KVPool& pool, const SeqBatch& 
   return cudaLaunchKernelEx(&cfg, qkv_gemv_rope_append_kernel<T, WBF16>, ga, pool, sb);
 }
 
-int launch_gather(oomattn_ctx* ctx, const GatherArgs& a, const SeqBatch& sb, int out_dtype) {
+// out: kOutF32, kOutBf16, or kOutF16 (a 4-bit cache's rows for its prefill).
+int launch_gather(oomattn_ctx* ctx, const GatherArgs& a, const SeqBatch& sb, int out) {
   const long long grid = (long long)sb.n * a.pages * ctx->cfg.n_kv_heads;
   if (grid >= (1ll << 31)) return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "%d tokens in one gather", a.n);
   const KVPool pool = make_pool(ctx);
-  const bool b = out_dtype == OOMATTN_DTYPE_BF16;
   cudaError_t le;
-#define OOMATTN_KG(K)                                                                                      \
-  (b ? launch_pdl(kv_gather_kernel<K, true>, dim3((unsigned)grid), dim3(128), 0, ctx->stream, a, pool, sb) \
-     : launch_pdl(kv_gather_kernel<K, false>, dim3((unsigned)grid), dim3(128), 0, ctx->stream, a, pool, sb))
+#define OOMATTN_KG(K, O) launch_pdl(kv_gather_kernel<K, O>, dim3((unsigned)grid), dim3(128), 0, ctx->stream, a, pool, sb)
+  const bool b = out == kOutBf16;
   switch (ctx->cfg.kv_dtype) {
-    case OOMATTN_DTYPE_Q4: le = OOMATTN_KG(kKvQ4); break;
-    case OOMATTN_DTYPE_BF16: le = OOMATTN_KG(kKvBf16); break;
-    default: le = OOMATTN_KG(kKvF32); break;
+    case OOMATTN_DTYPE_Q4:
+      le = out == kOutF16 ? OOMATTN_KG(kKvQ4, kOutF16) : (b ? OOMATTN_KG(kKvQ4, kOutBf16) : OOMATTN_KG(kKvQ4, kOutF32));
+      break;
+    case OOMATTN_DTYPE_BF16: le = b ? OOMATTN_KG(kKvBf16, kOutBf16) : OOMATTN_KG(kKvBf16, kOutF32); break;
+    default: le = b ? OOMATTN_KG(kKvF32, kOutBf16) : OOMATTN_KG(kKvF32, kOutF32); break;
   }
 #undef OOMATTN_KG
   if (le != cudaSuccess) return fail(ctx, OOMATTN_ERR_CUDA, "gather launch: %s", cudaGetErrorString(le));
@@ -994,7 +995,9 @@ int project(oomattn_ctx* ctx, const float* x, int T, int k, const KfJob* jobs, i
 }
 
 // Prefill over a 4-bit cache, many tokens: the sequence's rows of one layer as
-// bf16 pages, in order, which the tensor-core prefill then reads as its pool.
+// fp16 pages (11 bits of the held values; bf16 would keep 8: 0.0029 to 0.0032
+// off the exact output instead of 0.0017, which is that of its own rounding), in
+// order, which the tensor-core prefill then reads as its pool.
 // It reads 160 and writes 512 bytes per token and kv head once, for the 4 * 128
 // * group * n_new products that each of those tokens takes part in.
 int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtensorMap* kmap, CUtensorMap* vmap) {
@@ -1043,7 +1046,7 @@ int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtenso
   a.pages = pages;
   a.paged = 1;
   a.status = ctx->d_status;
-  int rc = launch_gather(ctx, a, sb, OOMATTN_DTYPE_BF16);
+  int rc = launch_gather(ctx, a, sb, kOutF16);
   if (!rc) rc = encode_pool_map(ctx, ctx->d_exp, (uint64_t)ctx->exp_pages + 1, kmap);
   if (!rc) rc = encode_pool_map(ctx, ctx->d_exp + half, (uint64_t)ctx->exp_pages + 1, vmap);
   pool->k = ctx->d_exp;
@@ -1161,7 +1164,9 @@ int oomattn_create(const oomattn_config* cfg, int device, void* stream, oomattn_
   if (cudaFuncSetAttribute(decode_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmemBytes) !=
           cudaSuccess ||
       set_decode_q4_smem() != cudaSuccess ||
-      cudaFuncSetAttribute(prefill_bf16_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPfSmemBytes) !=
+      cudaFuncSetAttribute(prefill_bf16_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPfSmemBytes) !=
+          cudaSuccess ||
+      cudaFuncSetAttribute(prefill_bf16_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPfSmemBytes) !=
           cudaSuccess ||
       cudaFuncSetAttribute(q8_linear_xs_kernel<2, 2, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            (int)q8_xs_smem_bytes(2, q8_xs_max_chunks(2))) != cudaSuccess ||
@@ -1180,8 +1185,10 @@ int oomattn_create(const oomattn_config* cfg, int device, void* stream, oomattn_
       cudaFuncSetAttribute(q8_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmemBytes) != cudaSuccess)
     return bail(OOMATTN_ERR_CUDA);
   cudaFuncAttributes fa;
-  if (cudaFuncGetAttributes(&fa, prefill_bf16_kernel) != cudaSuccess) return bail(OOMATTN_ERR_CUDA);
-  ctx->prefill_regs = fa.numRegs;
+  if (cudaFuncGetAttributes(&fa, prefill_bf16_kernel<false>) != cudaSuccess) return bail(OOMATTN_ERR_CUDA);
+  ctx->prefill_regs[0] = fa.numRegs;
+  if (cudaFuncGetAttributes(&fa, prefill_bf16_kernel<true>) != cudaSuccess) return bail(OOMATTN_ERR_CUDA);
+  ctx->prefill_regs[1] = fa.numRegs;
   if (cudaFuncGetAttributes(&fa, kf_gemm_kernel<true, 1>) != cudaSuccess) return bail(OOMATTN_ERR_CUDA);
   ctx->kf_q8_regs = fa.numRegs;
   if (cudaDeviceSynchronize() != cudaSuccess) return bail(OOMATTN_ERR_CUDA);
@@ -1223,7 +1230,7 @@ int oomattn_sync(oomattn_ctx* ctx) {
     if (st & kDevErrTimeout) return fail(ctx, OOMATTN_ERR_TIMEOUT, "a device-side wait timed out (status %d)", st);
     if (st & kDevErrRange)
       return fail(ctx, OOMATTN_ERR_DEVICE_CHECK,
-                  "prefill met a cached V value of magnitude >= 65536, outside the fp16 P.V product (status %d)", st);
+                  "prefill met a cached V value (4-bit cache: a q value) of magnitude >= 65536, outside its fp16 product (status %d)", st);
     if (st & kDevErrFormat)
       return fail(ctx, OOMATTN_ERR_DEVICE_CHECK,
                   "q8_repack met a block whose length field disagrees with its position (status %d)", st);
@@ -1417,7 +1424,7 @@ int oomattn_kv_gather(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int
     a.pages = (n + kPageSize - 2) / kPageSize + 1;  // the most that n slots can touch
     a.paged = 0;
     a.status = ctx->d_status;
-    rc = launch_gather(ctx, a, sb, out_dtype);
+    rc = launch_gather(ctx, a, sb, out_dtype == OOMATTN_DTYPE_BF16 ? kOutBf16 : kOutF32);
     if (rc) return rc;
   }
   return OOMATTN_OK;
@@ -1652,9 +1659,10 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
   if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_F32)
     return fail(ctx, OOMATTN_ERR_UNSUPPORTED, "the tensor-core prefill needs a bf16 or 4-bit cache");
   // The kernel's register split (setmaxnreg) balances only at this launch count.
-  if (ctx->prefill_regs != kPfLaunchRegs)
+  const bool q4 = ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4;
+  if (ctx->prefill_regs[q4] != kPfLaunchRegs)
     return fail(ctx, OOMATTN_ERR_UNSUPPORTED, "prefill kernel compiled with %d registers per thread, expected %d",
-                ctx->prefill_regs, kPfLaunchRegs);
+                ctx->prefill_regs[q4], kPfLaunchRegs);
   if (reinterpret_cast<uintptr_t>(q) % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0)
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
   const int L = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq];
@@ -1736,7 +1744,7 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
   CUtensorMap kmap = ctx->kmap, vmap = ctx->vmap;
   a.seq = seq;
   a.layer = layer;
-  if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4) {
+  if (q4) {
     rc = q4_expand(ctx, layer, seq, L, &pool, &kmap, &vmap);
     if (rc) return rc;
     a.seq = 0;
@@ -1748,7 +1756,8 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
   a.qscale = ctx->scale * 1.4426950408889634f;
   a.status = ctx->d_status;
   a.timeout_ns = ctx->timeout_ns;
-  prefill_bf16_kernel<<<dim3((unsigned)(blocks * a.n_heads), n_chunks), kPfThreads, kPfSmemBytes, ctx->stream>>>(
+  (q4 ? prefill_bf16_kernel<true> : prefill_bf16_kernel<false>)<<<dim3((unsigned)(blocks * a.n_heads), n_chunks),
+                                                                  kPfThreads, kPfSmemBytes, ctx->stream>>>(
       qmap, kmap, vmap, omap, pmap, pool, a);
   CKLAUNCH();
   if (n_chunks > 1) {

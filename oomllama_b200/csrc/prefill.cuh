@@ -219,6 +219,11 @@ __host__ __device__ constexpr uint32_t make_idesc_f16kind(bool bf16, bool b_mn_m
 __host__ __device__ constexpr uint32_t make_idesc_bf16(bool b_mn_major) { return make_idesc_f16kind(true, b_mn_major); }
 
 // ------------------------------------------------------------ the kernel
+// F16: the pool's pages hold fp16 (a 4-bit cache's rows, expanded).  V is then an
+// operand as it lands, S = Q K^T runs as fp16 x fp16, and the softmax warps,
+// which have nothing to do yet, first rewrite their Q tile from bf16 to fp16 in
+// place (exact below 65504, subnormals to 2^-25).
+template <bool F16>
 __global__ void __launch_bounds__(kPfThreads, 1)
     prefill_bf16_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap omap,
@@ -239,7 +244,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   uint64_t* p_full = s_full + 2;                     // [2 tiles][2 halves of P]
   uint64_t* o_full = p_full + 4;                     // [2]
   uint64_t* mma_done = o_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  uint64_t* q_conv = mma_done + 1;                   // F16: both Q tiles converted to fp16
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_conv + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // heaviest work first: block b -> the (b / n_heads)-th pair of the ranges
@@ -300,6 +306,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       mbar_init(&o_full[i], 1);
     }
     mbar_init(mma_done, 1);
+    mbar_init(q_conv, kPfThreads - 128);
     fence_mbar_init();
   }
   if (warp == 0) {
@@ -388,9 +395,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     // ------------------------------------------------ MMA issuer
     OOMATTN_REGS_DEC();
     if (lane == 0) {
-      constexpr uint32_t idesc_qk = make_idesc_bf16(false);
+      constexpr uint32_t idesc_qk = make_idesc_f16kind(!F16, false);
       constexpr uint32_t idesc_pv = make_idesc_f16kind(false, true);  // P fp16 x V fp16
-      bool ok = mbar_wait(q_full, 0, a.status, a.timeout_ns);
+      bool ok = mbar_wait(F16 ? q_conv : q_full, 0, a.status, a.timeout_ns);
       tc_fence_after();
       // Descriptor bases are built once; each MMA only adds a compile-time
       // offset (in 16-byte units) to the start-address field, which cannot
@@ -436,7 +443,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       };
       auto wait_v = [&](int j) {
         if (ok && j > v_waited) {
-          ok = mbar_wait(&v_conv[j % kPfVStages], (j / kPfVStages) & 1, a.status, a.timeout_ns);
+          ok = mbar_wait(&(F16 ? v_full : v_conv)[j % kPfVStages], (j / kPfVStages) & 1, a.status, a.timeout_ns);
           tc_fence_after();
           v_waited = j;
         }
@@ -495,7 +502,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     const int ct = threadIdx.x - 64;  // 0..63
     bool ok = true;
     uint32_t big = 0;
-    for (int j = 0; j < n_kv_tiles && ok; ++j) {
+    for (int j = 0; !F16 && j < n_kv_tiles && ok; ++j) {
       const int s = j % kPfVStages;
       ok = mbar_wait(&v_full[s], (j / kPfVStages) & 1, a.status, a.timeout_ns);
       if (!ok) break;
@@ -526,6 +533,26 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     const float cl = a.qscale;
+    if (F16) {
+      ok = mbar_wait(q_full, 0, a.status, a.timeout_ns);
+      if (ok) {
+        uint4* tile = reinterpret_cast<uint4*>(sQ + i * kTileBytes);
+        uint32_t big = 0;
+#pragma unroll 4
+        for (int c = (threadIdx.x & 127); c < kTileBytes / 16; c += 128) {
+          uint4 w = tile[c];
+          big = max(big, max_exp_bf16x8(w.x, w.y, w.z, w.w));
+          w.x = bf16x2_to_f16x2(w.x);
+          w.y = bf16x2_to_f16x2(w.y);
+          w.z = bf16x2_to_f16x2(w.z);
+          w.w = bf16x2_to_f16x2(w.w);
+          tile[c] = w;
+        }
+        if (big >= 0x4780u) report_error(a.status, kDevErrRange);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(q_conv);
+    }
     for (int j = 0; j < (i ? ntl[1] : ntl[0]) && ok; ++j) {
       ok = mbar_wait(&s_full[i], j & 1, a.status, a.timeout_ns);
       if (!ok) break;
