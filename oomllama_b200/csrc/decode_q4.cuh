@@ -88,27 +88,6 @@ __device__ __forceinline__ void mma_f16_1688_z(float* d, uint32_t a0, uint32_t a
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
 }
-__device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-// (x & mask) | magic in one instruction (with both as immediates it takes two).
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t magic) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(mask), "r"(magic));
-  return d;
-}
 __device__ __forceinline__ float h_lo(uint32_t v) { return __half2float(__ushort_as_half((uint16_t)v)); }
 __device__ __forceinline__ float h_hi(uint32_t v) { return __half2float(__ushort_as_half((uint16_t)(v >> 16))); }
 // (a, b) rounded to f16, or (low) what that rounding leaves: exact in f32, rounded once.
@@ -464,12 +443,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
           for (int h = 0; h < 2; ++h) {
             const uint32_t x = wl ? vw[2 * pg + h].y : vw[2 * pg + h].x;
             const uint32_t s2 = wl ? vs[2 * pg + h].y : vs[2 * pg + h].x;
-            const uint32_t y = x >> 8;
-            // 1024 + c, or 1024 + 16 c, to c - 8, times s: every step exact
-            b[h][0] = h2_mul(h2_add(and_or(x, 0x000f000fu, magic), 0xe408e408u), s2);
-            b[h][1] = h2_mul(h2_fma(and_or(x, 0x00f000f0u, magic), 0x2c002c00u, 0xd480d480u), s2);
-            b[h][2] = h2_mul(h2_add(and_or(y, 0x000f000fu, magic), 0xe408e408u), s2);
-            b[h][3] = h2_mul(h2_fma(and_or(y, 0x00f000f0u, magic), 0x2c002c00u, 0xd480d480u), s2);
+            q4_centered(x, magic, b[h]);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) b[h][n] = h2_mul(b[h][n], s2);  // exact: 4 bits times 8
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
