@@ -17,20 +17,31 @@
 // heads (WIDE = false) has both parts side by side, column 2 h the high part
 // of head h, column 2 h + 1 the low: one product does both, and the two
 // columns of an accumulator lie in one lane.  A group of five to eight (WIDE)
-// has a column per head and adds the low parts' product onto the high parts'.
-// (Heads as rows, eight high and eight low, would cost a group of four as many
-// products as one of eight: 96.2 instead of 66.7 us for 8 x 32768 tokens of
-// 32q/8kv.)  K codes enter as subnormal halves (code *
-// 2^-24, or 2^-20 for the upper nibble of a byte, whose q is prescaled by
-// 1/16): unpacking is one AND per two codes.  q is scaled by a power of two to
-// [2^14, 2^15) per head so that its low part keeps its bits.
+// has a column per head and a second product for the low parts.  (Heads as rows,
+// eight high and eight low, would cost a group of four as many products as one
+// of eight: 96.2 instead of 66.7 us for 8 x 32768 tokens of 32q/8kv.)
+// K codes enter as subnormal halves (code * 2^-24, or 2^-20 for the upper nibble
+// of a byte, whose q is prescaled by 1/16): unpacking is one AND per two codes.
+// q is scaled by a power of two to [2^14, 2^15) per head, and its high part put
+// on a grid on which the products' sums are exact (q_part).
 // The P V products of a 32-token tile start from zero and are added to O in
 // f32 (one packed FMA with the softmax rescale): the tensor core truncates
 // when it accumulates, which over a long context would shrink O.
 //
 // Each warp works alone: its own ring of tiles in shared memory, filled by
-// bulk copies (one of 2560 bytes per page: K, then V) that one of its lanes issues, its
-// own running maximum and sum; the four warps of a CTA join at the end.
+// bulk copies (one of 2560 bytes per page: K, then V) that two of its lanes issue,
+// its own running maximum and sum; the four warps of a CTA join at the end.
+//
+// Measured: 8 x 32768 tokens of 32q/8kv (335 MB) in 65 us, 5.13 TB/s, 0.78 of
+// the copy rate (75 us under the 1000 W cap, 1.70 GHz, in a loop of seconds); 64
+// ragged rows of 28q/4kv (209 MB) in 62 us, 0.51.  Copies alone take 53 and 38
+// us, the arithmetic alone 58 and 52: about 320 (narrow) and 400 (wide)
+// instructions per warp and 16 tokens -- 40 + 104 to unpack K and V, 18 or 36
+// tensor products of 8.4 cycles each, which overlap the ALU and f16 pipes only
+// in part (16 products with 64 LOP3 and 64 HMUL2: 196 cycles; 136, 126 and 125
+// alone).  Neither two tiles in flight in one warp, nor 16 warps of the wide form
+// (it spills), nor e4m3 digits of q (an exact product of K = 32, but slow as
+// mma.sync) made it faster.
 #pragma once
 #include "common.cuh"
 #include "decode.cuh"
@@ -508,19 +519,19 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
                           reinterpret_cast<float*>(smem_q4), kRing / 4, s_w);
 }
 
-// The merge of a launch with more splits per row than its last CTA could join
-// quickly (kMaxSplitsBf16): a kernel of its own, one CTA per (row, q head).
-// Its eight warps take every eighth split, a lane four dims; weights 2^(lse -
-// max) and the sums as in merge_splits_staged, in a fixed order.  Rows with a
-// single split were written by the decode kernel.
-constexpr int kMergeWarps = 8;
+// The merge of a launch whose rows do not fill the GPU, with up to kMaxSplitsQ4
+// splits: a kernel of its own, one CTA per (row, q head, 32 dims).  A warp takes
+// four splits at a time, eight lanes with four dims each; weights 2^(lse - max)
+// and the sums as in merge_splits_staged, in a fixed order.  Rows with a single
+// split were written by the decode kernel.
+constexpr int kMergeWarps = 16;
 template <bool OUT16>
 __global__ void __launch_bounds__(kMergeWarps * 32)
     merge_splits_kernel(const DecodeArgs a, const __grid_constant__ SeqBatch sb, const __grid_constant__ DecodeSched sched) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float s_wt[kMaxSplitsQ4];
   __shared__ float s_red[2][kMergeWarps];
-  __shared__ float4 s_acc[kMergeWarps][32];
+  __shared__ float4 s_acc[kMergeWarps][8];
   const int r = blockIdx.x / a.n_heads, h = blockIdx.x - r * a.n_heads;
   const int z = sched.order[r];
   const int n_pages = (sb.len[z] + kPageSize - 1) / kPageSize;
@@ -550,23 +561,31 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
 #pragma unroll
   for (int w = 0; w < kMergeWarps; ++w) sum += s_red[1][w];
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int sub = lane >> 3, d = blockIdx.y * 32 + (lane & 7) * 4;
 #pragma unroll 8
-  for (int s = warp; s < ns; s += kMergeWarps) {
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + (p0 + s) * kHeadDim) + lane);
+  for (int s = warp * 4 + sub; s < ns; s += kMergeWarps * 4) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + (p0 + s) * kHeadDim + d));
     const float w = s_wt[s];
     acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
   }
-  s_acc[warp][lane] = acc;
+#pragma unroll
+  for (int off = 8; off < 32; off <<= 1) {
+    acc.x += __shfl_xor_sync(0xffffffffu, acc.x, off);
+    acc.y += __shfl_xor_sync(0xffffffffu, acc.y, off);
+    acc.z += __shfl_xor_sync(0xffffffffu, acc.z, off);
+    acc.w += __shfl_xor_sync(0xffffffffu, acc.w, off);
+  }
+  if (sub == 0) s_acc[warp][lane] = acc;
   __syncthreads();
-  if (warp != 0) return;
+  if (warp != 0 || sub != 0) return;
 #pragma unroll
   for (int w = 1; w < kMergeWarps; ++w) {
     const float4 v = s_acc[w][lane];
     acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
   }
   const float inv = 1.f / sum;
-  store_out4<OUT16>(a, zh, lane * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-  if (a.lse && lane == 0) a.lse[zh * a.lse_stride] = (M + log2f(sum)) * 0.69314718055994531f;
+  store_out4<OUT16>(a, zh, d, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  if (a.lse && blockIdx.y == 0 && lane == 0) a.lse[zh * a.lse_stride] = (M + log2f(sum)) * 0.69314718055994531f;
 }
 
 }  // namespace oomattn

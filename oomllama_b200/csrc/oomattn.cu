@@ -829,8 +829,8 @@ int plan_decode(const SeqBatch& sb, int n_kv, int slots, int max_splits, int fil
 // joins (merge_splits_staged), where the rows fill the GPU with them: a merge
 // kernel after the decode costs 64 ragged rows of 28q/4kv 64.8 us instead of
 // 61.8.  Where they do not, that kernel is the faster way to join any number
-// (one row of 8q/1kv: 1500 tokens 6.2 us instead of 7.0, 4096 6.9 instead of
-// 10.5), so as many as the partials' memory holds for so few rows.
+// (one row of 8q/1kv: 1500 tokens 6.5 us instead of 7.0, 4096 6.5 instead of
+// 10.5, 100003 13.9 instead of 36.2), so as many as the partials' memory holds for so few rows.
 int q4_max_splits(int rows, int n_kv, int max_pages, int slots) {
   if (rows * n_kv * kMaxSplitsBf16 >= slots || max_pages <= decode_min_pages(OOMATTN_DTYPE_Q4)) return kMaxSplitsBf16;
   return std::min(kMaxSplitsQ4, kMaxBatch * kMaxSplitsBf16 / rows);
@@ -894,7 +894,7 @@ int launch_decode_rows(oomattn_ctx* ctx, int layer, const SeqBatch& sb, const fl
     cfg.dynamicSmemBytes = q4_smem_bytes(q4_wide(ctx->group));
     le = cudaLaunchKernelEx(&cfg, decode_q4_fn(q4_wide(ctx->group), io), pool, a, sb, sched);
     if (le == cudaSuccess && late)
-      le = launch_pdl(io == DecIo::kQ16Out16 ? merge_splits_kernel<true> : merge_splits_kernel<false>, dim3(sb.n * a.n_heads),
+      le = launch_pdl(io == DecIo::kQ16Out16 ? merge_splits_kernel<true> : merge_splits_kernel<false>, dim3(sb.n * a.n_heads, kHeadDim / 32),
                       dim3(kMergeWarps * 32), 0, ctx->stream, a, sb, sched);
   } else {
     cfg.blockDim = dim3(kDecWarps * 32);

@@ -14,9 +14,9 @@ constexpr int kMaxGroup = 8;    // q heads per kv head handled by one decode CTA
 // layer step at 43 splits than at 26.
 constexpr int kMaxSplits = 64;
 constexpr int kMaxSplitsBf16 = 32;
-// 4-bit caches: 32 as well, and up to 256 where 32 leave SMs idle on a long
-// context (few rows of few kv heads), merged by a kernel of its own.
-constexpr int kMaxSplitsQ4 = 256;
+// 4-bit caches: 32 as well, and up to 512 where 32 leave SMs idle (few rows of
+// few kv heads), merged by a kernel of its own.
+constexpr int kMaxSplitsQ4 = 512;
 
 // Per-launch sequence rows, passed by value so a launch needs no host->device
 // metadata copy (and can be captured in a CUDA graph).
