@@ -14,7 +14,7 @@ enum : int {
   kDevErrTimeout = 1,      // a bounded wait on an mbarrier gave up
   kDevErrBounds = 2,       // a page / position index failed its device check
   kDevErrTmem = 4,         // tensor-memory allocation returned an unusable address
-  kDevErrRange = 8,        // a cached V value of magnitude >= 65536 met the fp16 P.V product
+  kDevErrRange = 8,        // a cached V value (4-bit cache: a V group's NaN, or a q value) outside the prefill's fp16 products
   kDevErrX16 = 16,         // a Q8-linear activation of magnitude >= 65504 met its fp16 hi/lo split
   kDevErrFormat = 32,      // a .oom Q8 block's length field disagrees with its position in the tensor
 };

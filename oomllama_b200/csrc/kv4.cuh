@@ -115,6 +115,8 @@ __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
+// Nonzero where a half of the pair is a NaN (its magnitude's bits above 0x7c00).
+__device__ __forceinline__ uint32_t h2_nan(uint32_t a) { return ((a & 0x7fff7fffu) + 0x03ff03ffu) & 0x80008000u; }
 // (x & mask) | magic in one instruction (with both as immediates it takes two).
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t magic) {
   uint32_t d;
@@ -251,6 +253,8 @@ __global__ void __launch_bounds__(128)
           const uint2 s4 = *reinterpret_cast<const uint2*>(c + kQ4Meta + h8 * 64 + t * 16 + wp * 8);
           const uint2 o4 = *reinterpret_cast<const uint2*>(c + kQ4VOffsets + h8 * 64 + t * 16 + wp * 8);
           const uint32_t keep = (wanted(slot) ? 0xffffu : 0u) | (wanted(slot + 1) ? 0xffff0000u : 0u);
+          // a NaN group would reach queries that do not see its token, as 0 * NaN
+          if ((h2_nan(o4.x & keep) | h2_nan(o4.y & keep)) != 0) report_error(a.status, kDevErrRange);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             uint32_t h[4];  // dim n of both tokens

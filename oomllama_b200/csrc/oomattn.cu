@@ -1060,9 +1060,10 @@ int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtenso
 
 // Prefill over a 4-bit cache, few tokens (drafts to verify, a short tail of a
 // prompt): each as one decode row that sees the slots up to its own.  Up to 24
-// tokens: by rows and expanded 14.8 and 24.7 us behind 2000 tokens (28q/4kv),
-// 54.0 and 59.5 behind 9001 (32q/8kv), 116 and 123 behind 30000 (28q/4kv); at
-// 32 tokens 18.1 and 24.7, 76.6 and 59.5, 154 and 123.
+// tokens: 24 by rows and 32 expanded (which pads either to 256) take 11.1 and
+// 20.6 us behind 500 tokens (40q/8kv), 15.2 and 23.1 behind 2000 (28q/4kv), 54.3
+// and 52.8 behind 9001 (32q/8kv), 119 and 112 behind 30000 (28q/4kv); 16 by rows
+// 9.4, 13.0, 42.9 and 88.5.
 constexpr int kQ4PrefillRows = 24;
 int q4_prefill_rows(oomattn_ctx* ctx, int layer, int seq, int n_new, const void* q, void* out, int out_dtype,
                     float* lse) {
@@ -1230,7 +1231,8 @@ int oomattn_sync(oomattn_ctx* ctx) {
     if (st & kDevErrTimeout) return fail(ctx, OOMATTN_ERR_TIMEOUT, "a device-side wait timed out (status %d)", st);
     if (st & kDevErrRange)
       return fail(ctx, OOMATTN_ERR_DEVICE_CHECK,
-                  "prefill met a cached V value (4-bit cache: a q value) of magnitude >= 65536, outside its fp16 product (status %d)", st);
+                  "prefill met a cached V value (4-bit cache: a q value) of magnitude >= 65536, or a NaN, outside its fp16 "
+                  "product (status %d)", st);
     if (st & kDevErrFormat)
       return fail(ctx, OOMATTN_ERR_DEVICE_CHECK,
                   "q8_repack met a block whose length field disagrees with its position (status %d)", st);

@@ -32,8 +32,9 @@ struct SeqBatch {
 };
 
 // Paged KV pool of all layers: element (layer, page, kv, slot, d) lives at
-// (((layer * n_pool_pages + page) * n_kv + kv) * kPageSize + slot) * kHeadDim + d.
-// Page n_pool_pages - 1 is the null page: zero, never written, and the
+// (((layer * n_pool_pages + page) * n_kv + kv) * kPageSize + slot) * kHeadDim + d,
+// of a 4-bit cache in the chunk (layer, page, kv) that kv4.cuh describes (v = k +
+// kQ4Chunk).  Page n_pool_pages - 1 is the null page: zero, never written, and the
 // block-table entry of every unassigned logical page.
 struct KVPool {
   void* k;
@@ -47,7 +48,7 @@ struct KVPool {
 
 // Test-only launch flags of the decode kernel (DecodeArgs::test_flags).
 enum : int {
-  kTestDropDecodeCopies = 1,  // the bf16 producer issues no copies: every consumer wait runs out its limit
+  kTestDropDecodeCopies = 1,  // the bf16 or 4-bit decode issues no copies: every consumer wait runs out its limit
   kTestDropLinearCopies = 2,  // the Q8 tensor-core pass's producer issues no copies: its MMA and promoter waits run out
 };
 

@@ -272,7 +272,6 @@ __global__ void __launch_bounds__(kQkNormWarps * 32, kQkNormCtasPerSm)
         }
       }
       continue;
-      continue;
     }
     const int sec = w < n_v ? 2 : (w < n_v + n_k ? 1 : 0);
     const int i = sec == 2 ? w : (sec == 1 ? w - n_v : w - n_v - n_k);

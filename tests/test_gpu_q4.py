@@ -384,6 +384,62 @@ def test_prefill_in_a_capture_needs_its_scratch():
     eng.close()
 
 
+def test_many_splits_captured_and_replayed():
+    """A row long enough for the merge by a kernel of its own, behind an append, in a graph: the replays follow the data."""
+    n = 9000
+    eng, ks, vs = _filled(4, 1, [n], seed=15, cap=[n + 1])
+    q, k, v = (randn((1, h * 128), 150 + h).cuda() for h in (4, 1, 2))
+    v = v[:, :128].contiguous()
+    out, qr = torch.empty(1, 4, 128, device="cuda"), torch.empty(1, 4, 128, device="cuda")
+
+    def step():
+        eng.rope_append(0, [0], q, k, v, starts=[n], q_out=qr)
+        eng.decode(0, [0], qr, out=out)
+        eng.rope_append(0, [0], q, k, v, starts=[n], q_out=qr)  # and again: two merges in a row share the partials
+        eng.decode(0, [0], qr, out=out)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for seed in (1, 2):
+        q.copy_(randn(q.shape, 160 + seed))
+        k.copy_(randn(k.shape, 170 + seed))
+        v.copy_(randn(v.shape, 180 + seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.cpu().numpy()
+        kc, vc = eng.kv_read(0, 0)
+        want, _ = q4_ref.attend(qr.cpu(), kc, vc, [n + 1])
+        assert_close(got, want, ATOL, RTOL, what=f"replay {seed}")
+    eng.close()
+
+
+def test_prefill_reports_values_outside_fp16():
+    """More than 24 queries: a NaN of V (which a product with a weight of zero would spread) and a q value that fp16 does
+    not hold are reported; up to 24 queries take both."""
+    from oomllama_b200._lib import OomAttnError
+    n = 200
+    k, v = randn((n, 2, 128), 1), randn((n, 2, 128), 2)
+    v[199, 1, 3] = math.nan
+    big = torch.ones(100, 4, 128, dtype=torch.bfloat16)
+    big[50, 3, 77] = 70000.0
+    for vv, q in ((v, big.clamp(-1, 1)), (torch.nan_to_num(v), big)):
+        eng = make_engine(4, 2, [n], kv_dtype="q4")
+        eng.kv_write(0, 0, k.cuda(), vv.cuda())
+        eng.prefill(0, 0, q.cuda())
+        with pytest.raises(OomAttnError) as e:
+            eng.sync()
+        assert e.value.code == 9
+        out = eng.prefill(0, 0, q[30:54].cuda())
+        eng.sync()
+        want, _ = q4_ref.attend(q[30:53], *eng.kv_read(0, 0), [n - 23 + i for i in range(23)])
+        assert_close(out[:20].cpu().numpy(), want[:20], ATOL, RTOL, what="rows of neither")
+        assert torch.isfinite(out[:23]).all()
+        eng.close()
+
+
 def test_results_repeat_to_the_bit():
     lens = [3000, 17, 900]
     eng, _, _ = _filled(28, 4, lens, seed=13)
