@@ -125,11 +125,12 @@ struct oomattn_ctx {
   // key-split prefill: the chunks' partial O and lse
   uint8_t* d_pf_part = nullptr;
   size_t pf_part_bytes = 0;
+  // scratch blocks that a larger one replaced: captured graphs may still name them
+  void* kept[96] = {};
+  int n_kept = 0;
   // prefill over a 4-bit cache: one sequence's rows of one layer as fp16 pages
   // [exp_pages + 1][n_kv][16][128] of K, then of V (the last page zero), and the
   // block table that names them in order
-  void* exp_blocks[64] = {};  // all that were allocated, each at least half as large again as the one before
-  int n_exp_blocks = 0;
   uint8_t* d_exp = nullptr;
   int exp_pages = 0;
   int* d_exp_table = nullptr;
@@ -327,17 +328,35 @@ int validate_dtype(oomattn_ctx* ctx, int dt, const char* what) {
   return OOMATTN_OK;
 }
 
+// A larger block in place of *p (null: the first).  The old one stays until the
+// context is destroyed, since a captured graph may name it; each is half as large
+// again as what was asked for, so that few are kept.  Not during a capture: the
+// block would be new to the graph alone.
+int grow_block(oomattn_ctx* ctx, void** p, size_t bytes, const char* what) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  CK(cudaStreamIsCapturing(ctx->stream, &st));
+  if (st != cudaStreamCaptureStatusNone)
+    return fail(ctx, OOMATTN_ERR_UNSUPPORTED, "%s has to grow: run a call of this size once before the capture", what);
+  if (*p && ctx->n_kept == (int)(sizeof(ctx->kept) / sizeof(ctx->kept[0])))
+    return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "%s has grown too often", what);
+  void* q = nullptr;
+  if (cudaMalloc(&q, bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(ctx, OOMATTN_ERR_NO_MEMORY, "%s of %zu bytes failed", what, bytes);
+  }
+  if (*p) ctx->kept[ctx->n_kept++] = *p;
+  *p = q;
+  return OOMATTN_OK;
+}
+
 int ensure_scratch(oomattn_ctx* ctx, size_t bytes) {
   if (bytes <= ctx->scratch_bytes) return OOMATTN_OK;
-  if (ctx->d_scratch) {
-    cudaStreamSynchronize(ctx->stream);
-    cudaFree(ctx->d_scratch);
-    ctx->d_scratch = nullptr;
-    ctx->scratch_bytes = 0;
-  }
-  if (cudaMalloc(&ctx->d_scratch, bytes) != cudaSuccess)
-    return fail(ctx, OOMATTN_ERR_NO_MEMORY, "scratch allocation of %zu bytes failed", bytes);
-  ctx->scratch_bytes = bytes;
+  const size_t want = ctx->d_scratch ? bytes + bytes / 2 : bytes;
+  void* p = ctx->d_scratch;
+  const int rc = grow_block(ctx, &p, want, "the scratch");
+  if (rc) return rc;
+  ctx->d_scratch = static_cast<float*>(p);
+  ctx->scratch_bytes = want;
   return OOMATTN_OK;
 }
 
@@ -1006,29 +1025,21 @@ int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtenso
   const size_t page_bytes = (size_t)n_kv * kPageSize * kHeadDim * 2;
   if (pages > ctx->exp_pages) {
     const int cap = pages + pages / 2;  // a growing sequence does not reallocate at every chunk
-    if ((long long)(cap + 1) * n_kv * kPageSize >= (1ll << 31) || ctx->n_exp_blocks == 64)
+    if ((long long)(cap + 1) * n_kv * kPageSize >= (1ll << 31))
       return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "prefill over %d tokens of a 4-bit cache", L);
-    cudaStreamCaptureStatus cap_st = cudaStreamCaptureStatusNone;
-    CK(cudaStreamIsCapturing(ctx->stream, &cap_st));
-    if (cap_st != cudaStreamCaptureStatusNone)
-      return fail(ctx, OOMATTN_ERR_UNSUPPORTED,
-                  "the prefill's scratch has to grow: run a prefill of this length once before the capture");
-    // K pages, V pages, table.  An earlier, smaller block stays until the context
-    // is destroyed: a captured graph may still name it.
+    // K pages, V pages, table
     const size_t half_bytes = (size_t)(cap + 1) * page_bytes, bytes = 2 * half_bytes + (size_t)cap * sizeof(int);
-    void* p = nullptr;
-    if (cudaMalloc(&p, bytes) != cudaSuccess) {
-      cudaGetLastError();
-      return fail(ctx, OOMATTN_ERR_NO_MEMORY, "prefill scratch of %zu bytes failed", bytes);
-    }
-    ctx->exp_blocks[ctx->n_exp_blocks++] = p;
+    void* p = ctx->d_exp;
+    const int rc = grow_block(ctx, &p, bytes, "the prefill's scratch");
+    if (rc) return rc;
+    ctx->d_exp = static_cast<uint8_t*>(p);
+    ctx->exp_pages = 0;  // until it is set up
     uint8_t* b = static_cast<uint8_t*>(p);
     int* table = reinterpret_cast<int*>(b + 2 * half_bytes);
     CK(cudaMemsetAsync(b + half_bytes - page_bytes, 0, page_bytes, ctx->stream));  // the null pages
     CK(cudaMemsetAsync(b + 2 * half_bytes - page_bytes, 0, page_bytes, ctx->stream));
     iota_kernel<<<(cap + 255) / 256, 256, 0, ctx->stream>>>(table, cap);
     CKLAUNCH();
-    ctx->d_exp = b;
     ctx->d_exp_table = table;
     ctx->exp_pages = cap;
   }
@@ -1207,7 +1218,8 @@ int oomattn_destroy(oomattn_ctx* ctx) {
                   ctx->d_argmax_part, ctx->d_kf, ctx->d_pf_part};
   for (void* p : ptrs)
     if (p) cudaFree(p);
-  for (int i = 0; i < ctx->n_exp_blocks; ++i) cudaFree(ctx->exp_blocks[i]);
+  if (ctx->d_exp) cudaFree(ctx->d_exp);
+  for (int i = 0; i < ctx->n_kept; ++i) cudaFree(ctx->kept[i]);
   delete ctx;
   return OOMATTN_OK;
 }
@@ -1722,15 +1734,12 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
     const size_t rows_all = (size_t)n_chunks * a.n_pad;
     const size_t ob = rows_all * ctx->cfg.n_heads * kHeadDim * 4, lb = rows_all * ctx->cfg.n_heads * 4;
     if (ob + lb > ctx->pf_part_bytes) {
-      if (ctx->d_pf_part) {
-        cudaStreamSynchronize(ctx->stream);
-        cudaFree(ctx->d_pf_part);
-        ctx->d_pf_part = nullptr;
-        ctx->pf_part_bytes = 0;
-      }
-      if (cudaMalloc(&ctx->d_pf_part, ob + lb) != cudaSuccess)
-        return fail(ctx, OOMATTN_ERR_NO_MEMORY, "prefill partial scratch of %zu bytes failed", ob + lb);
-      ctx->pf_part_bytes = ob + lb;
+      const size_t want = ctx->d_pf_part ? (ob + lb) + (ob + lb) / 2 : ob + lb;
+      void* p = ctx->d_pf_part;
+      rc = grow_block(ctx, &p, want, "the prefill's partials");
+      if (rc) return rc;
+      ctx->d_pf_part = static_cast<uint8_t*>(p);
+      ctx->pf_part_bytes = want;
     }
     part_o = reinterpret_cast<float*>(ctx->d_pf_part);
     a.part_lse = reinterpret_cast<float*>(ctx->d_pf_part + ob);

@@ -440,6 +440,35 @@ def test_prefill_reports_values_outside_fp16():
         eng.close()
 
 
+def test_captured_prefill_outlives_larger_ones():
+    """Scratch that a larger prefill replaces stays for the graphs that name it: expanded pages and key-split partials."""
+    lens = [600, 3000]
+    eng, ks, vs = _filled(4, 2, lens, seed=16)
+    q = [randn((n, 4, 128), 190 + n, torch.bfloat16).cuda() for n in (60, 400)]
+    out = torch.empty(60, 4, 128, device="cuda")
+    eng.prefill(0, 0, q[0], out=out)
+    first = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        eng.prefill(0, 0, q[0], out=out)
+    eng.prefill(0, 1, q[1])  # both kinds of scratch grow
+    out.zero_()
+    graph.replay()
+    eng.sync()
+    assert torch.equal(out, first)
+    want, _ = q4_ref.attend(q[0].cpu(), ks[0], vs[0], [541 + i for i in range(60)])
+    assert_close(out.cpu().numpy(), want, 4.5 * 2 * 2.0 ** -8, BF16_RTOL, what="replayed")
+    graph = torch.cuda.CUDAGraph()
+    from oomllama_b200._lib import OomAttnError
+    big = torch.empty(3000, 4, 128, device="cuda", dtype=torch.bfloat16)
+    with torch.cuda.graph(graph):
+        with pytest.raises(OomAttnError) as e:  # partials of 3000 rows: more than any call so far
+            eng.prefill(0, 1, big)
+        assert e.value.code == 8
+        out.zero_()
+    eng.close()
+
+
 def test_results_repeat_to_the_bit():
     lens = [3000, 17, 900]
     eng, _, _ = _filled(28, 4, lens, seed=13)
