@@ -1767,14 +1767,18 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
   a.qscale = ctx->scale * 1.4426950408889634f;
   a.status = ctx->d_status;
   a.timeout_ns = ctx->timeout_ns;
-  (q4 ? prefill_bf16_kernel<true> : prefill_bf16_kernel<false>)<<<dim3((unsigned)(blocks * a.n_heads), n_chunks),
-                                                                  kPfThreads, kPfSmemBytes, ctx->stream>>>(
-      qmap, kmap, vmap, omap, pmap, pool, a);
-  CKLAUNCH();
+  const dim3 grid((unsigned)(blocks * a.n_heads), n_chunks);
+  if (q4) {
+    CK(launch_pdl(prefill_bf16_kernel<true>, grid, dim3(kPfThreads), kPfSmemBytes, ctx->stream, qmap, kmap, vmap, omap,
+                  pmap, pool, a));
+  } else {
+    prefill_bf16_kernel<false><<<grid, kPfThreads, kPfSmemBytes, ctx->stream>>>(qmap, kmap, vmap, omap, pmap, pool, a);
+    CKLAUNCH();
+  }
   if (n_chunks > 1) {
     const long long warps = (long long)n_new * a.n_heads;
-    prefill_chunk_merge_kernel<<<(unsigned)((warps * 32 + 255) / 256), 256, 0, ctx->stream>>>(part_o, a);
-    CKLAUNCH();
+    CK(launch_pdl(prefill_chunk_merge_kernel, dim3((unsigned)((warps * 32 + 255) / 256)), dim3(256), 0, ctx->stream,
+                  (const float*)part_o, a));
   }
   return OOMATTN_OK;
 }

@@ -285,7 +285,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 #pragma unroll
   for (int i = 0; i < 2; ++i) ntl[i] = max(0, min(ntile[i], jb + a.key_chunk) - jb);
   const int n_kv_tiles = max(ntl[0], ntl[1]);
-  if (n_kv_tiles == 0) return;  // a chunk past this pair's keys: the whole CTA leaves
+  if (n_kv_tiles == 0) {  // a chunk past this pair's keys: the whole CTA leaves
+    if (F16) asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const bool split_pair = max(ntile[0], ntile[1]) > a.key_chunk;
 
   if (threadIdx.x == 0) {
@@ -317,6 +320,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // F16: a programmatic dependent of the expansion, which ends while this kernel sets up
+  if (F16) asm volatile("griddepcontrol.wait;" ::: "memory");
   // Register split: the kernel launches with kPfLaunchRegs per thread (the host
   // checks the compiled count before launching); warpgroup 0 (TMA, MMA and two
   // idle warps) gives (168-88)*128 registers back at the top of its branches and
@@ -732,6 +737,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 // head), 4 dimensions per lane; rows of unsplit pairs, or outside the
 // launch's block ranges, were written by the prefill kernel itself.
 __global__ void prefill_chunk_merge_kernel(const float* __restrict__ part_o, const PrefillArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // a programmatic dependent of the prefill
   const long long item = (blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (item >= (long long)a.n_new * a.n_heads) return;
