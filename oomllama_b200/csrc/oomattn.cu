@@ -253,12 +253,13 @@ int encode_pool_map(oomattn_ctx* ctx, void* base, uint64_t n_pages, CUtensorMap*
   return OOMATTN_OK;
 }
 
-int encode_q_map(oomattn_ctx* ctx, const void* q, int n_new, CUtensorMap* map) {
+// A tile of pack heads of 128 / pack queries each.
+int encode_q_map(oomattn_ctx* ctx, const void* q, int n_new, int pack, CUtensorMap* map) {
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) return fail(ctx, OOMATTN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   cuuint64_t dims[3] = {(cuuint64_t)kHeadDim, (cuuint64_t)ctx->cfg.n_heads, (cuuint64_t)n_new};
   cuuint64_t strides[2] = {(cuuint64_t)kHeadDim * 2, (cuuint64_t)ctx->cfg.n_heads * kHeadDim * 2};
-  cuuint32_t box[3] = {64, 1, 128};
+  cuuint32_t box[3] = {64, (cuuint32_t)pack, (cuuint32_t)(128 / pack)};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -269,14 +270,15 @@ int encode_q_map(oomattn_ctx* ctx, const void* q, int n_new, CUtensorMap* map) {
 
 // The prefill output [n_new][n_heads][128] (f32 or bf16) as the target of
 // the epilogue's TMA stores: boxes of 128 rows x 128 bytes (32 f32 or 64 bf16
-// columns) of one head, 128-byte swizzled; rows past n_new are clipped.
-int encode_out_map(oomattn_ctx* ctx, void* out, int n_new, bool bf16, CUtensorMap* map) {
+// columns) of one head (pack heads of 128 / pack queries), 128-byte swizzled;
+// rows past n_new are clipped.
+int encode_out_map(oomattn_ctx* ctx, void* out, int n_new, bool bf16, int pack, CUtensorMap* map) {
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) return fail(ctx, OOMATTN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   const uint64_t es = bf16 ? 2 : 4;
   cuuint64_t dims[3] = {(cuuint64_t)kHeadDim, (cuuint64_t)ctx->cfg.n_heads, (cuuint64_t)n_new};
   cuuint64_t strides[2] = {(cuuint64_t)kHeadDim * es, (cuuint64_t)ctx->cfg.n_heads * kHeadDim * es};
-  cuuint32_t box[3] = {(cuuint32_t)(128 / es), 1, 128};
+  cuuint32_t box[3] = {(cuuint32_t)(128 / es), (cuuint32_t)pack, (cuuint32_t)(128 / pack)};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, out, dims,
                    strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -1651,18 +1653,9 @@ int oomattn_set_test_flags(oomattn_ctx* ctx, int32_t flags) {
   return OOMATTN_OK;
 }
 
-int oomattn_prefill(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_new, const void* q, void* out,
-                    int32_t out_dtype, float* lse) {
-  if (!ctx) return OOMATTN_ERR_INVALID_ARG;
-  if (n_new <= 0) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad prefill arguments");
-  if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4 && n_new <= kQ4PrefillRows)
-    return q4_prefill_rows(ctx, layer, seq, n_new, q, out, out_dtype, lse);
-  const int32_t all[2] = {0, (n_new + 255) / 256};
-  return oomattn_prefill_blocks(ctx, layer, seq, n_new, q, out, out_dtype, lse, 1, all);
-}
-
-int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_new, const void* q, void* out,
-                           int32_t out_dtype, float* lse, int32_t n_ranges, const int32_t* ranges) {
+// ranges: blocks of 2 * (128 / pack) queries.  pack: q heads per tile (1, or the group over a 4-bit cache).
+static int prefill_impl(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_new, const void* q, void* out,
+                        int32_t out_dtype, float* lse, int32_t n_ranges, const int32_t* ranges, int pack) {
   if (!ctx) return OOMATTN_ERR_INVALID_ARG;
   if (!q || !out || n_new <= 0 || !ranges || n_ranges <= 0)
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad prefill arguments");
@@ -1681,7 +1674,8 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
   const int L = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq];
   if (n_new > L) return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "n_new %d exceeds the cached length %d", n_new, L);
-  const int n_pairs = (n_new + 255) / 256;
+  const int tpt = 128 / pack, n_units = ctx->cfg.n_heads / pack;
+  const int n_pairs = (n_new + 2 * tpt - 1) / (2 * tpt);
   if (n_ranges > kPfMaxRanges)
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "%d block ranges (at most %d)", n_ranges, kPfMaxRanges);
   PrefillArgs a;
@@ -1709,12 +1703,12 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
   // the heaviest block no longer sets the launch time; their partials are
   // merged by one more kernel.  A whole 28-head 4096-token launch is not split.
   const int prefix = L - n_new;
-  auto pair_tiles = [&](int p) { return (prefix + std::min(n_new, 256 * p + 256) + 127) / 128; };
+  auto pair_tiles = [&](int p) { return (prefix + std::min(n_new, 2 * tpt * (p + 1)) + 127) / 128; };
   long long work = 0;
   int max_tiles = 1;
   for (int i = 0; i < n_ranges; ++i)
     for (int p = a.range_lo[i]; p < a.range_hi[i]; ++p) {
-      work += (long long)pair_tiles(p) * ctx->cfg.n_heads;
+      work += (long long)pair_tiles(p) * n_units;
       max_tiles = std::max(max_tiles, pair_tiles(p));
     }
   const int per_sm = (int)((work + ctx->num_sms - 1) / ctx->num_sms);
@@ -1722,12 +1716,14 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
   if (2 * max_tiles > 3 * per_sm) key_chunk = std::max(kPfMinKeyChunk, per_sm);
   const int n_chunks = (max_tiles + key_chunk - 1) / key_chunk;
   a.key_chunk = key_chunk;
-  a.n_pad = (n_new + 127) / 128 * 128;
+  a.n_pad = (n_new + tpt - 1) / tpt * tpt;
+  a.pack = pack;
+  a.tile_tokens = tpt;
   a.part_lse = nullptr;
   float* part_o = nullptr;
   CUtensorMap qmap, omap, pmap;
-  rc = encode_q_map(ctx, q, n_new, &qmap);
-  if (!rc) rc = encode_out_map(ctx, out, n_new, out_dtype == OOMATTN_DTYPE_BF16, &omap);
+  rc = encode_q_map(ctx, q, n_new, pack, &qmap);
+  if (!rc) rc = encode_out_map(ctx, out, n_new, out_dtype == OOMATTN_DTYPE_BF16, pack, &omap);
   if (rc) return rc;
   pmap = omap;
   if (n_chunks > 1) {
@@ -1743,7 +1739,7 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
     }
     part_o = reinterpret_cast<float*>(ctx->d_pf_part);
     a.part_lse = reinterpret_cast<float*>(ctx->d_pf_part + ob);
-    rc = encode_out_map(ctx, part_o, (int)rows_all, false, &pmap);
+    rc = encode_out_map(ctx, part_o, (int)rows_all, false, pack, &pmap);
     if (rc) return rc;
   }
   a.out = out;
@@ -1767,7 +1763,7 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
   a.qscale = ctx->scale * 1.4426950408889634f;
   a.status = ctx->d_status;
   a.timeout_ns = ctx->timeout_ns;
-  const dim3 grid((unsigned)(blocks * a.n_heads), n_chunks);
+  const dim3 grid((unsigned)(blocks * n_units), n_chunks);
   if (q4) {
     CK(launch_pdl(prefill_bf16_kernel<true>, grid, dim3(kPfThreads), kPfSmemBytes, ctx->stream, qmap, kmap, vmap, omap,
                   pmap, pool, a));
@@ -1781,6 +1777,40 @@ int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t
                   (const float*)part_o, a));
   }
   return OOMATTN_OK;
+}
+
+// Heads per tile of a prefill over a 4-bit cache: the group, or one, whichever
+// has fewer key tiles to multiply in all.
+static int prefill_pack(const oomattn_ctx* ctx, int n_new, int L) {
+  auto tiles = [&](int pack) {
+    const int step = 2 * (128 / pack);
+    long long sum = 0;
+    for (int q = 0; q < n_new; q += step) sum += (L - n_new + std::min(n_new, q + step) + 127) / 128;
+    return sum * (ctx->cfg.n_heads / pack);
+  };
+  return tiles(ctx->group) < tiles(1) ? ctx->group : 1;
+}
+
+int oomattn_prefill(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_new, const void* q, void* out,
+                    int32_t out_dtype, float* lse) {
+  if (!ctx) return OOMATTN_ERR_INVALID_ARG;
+  if (n_new <= 0) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad prefill arguments");
+  int pack = 1;
+  if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4) {
+    if (n_new <= kQ4PrefillRows) return q4_prefill_rows(ctx, layer, seq, n_new, q, out, out_dtype, lse);
+    int rc = check_layer(ctx, layer);
+    if (!rc) rc = check_seq(ctx, seq);
+    if (rc) return rc;
+    pack = prefill_pack(ctx, n_new, ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq]);
+  }
+  const int block = 2 * (128 / pack);
+  const int32_t all[2] = {0, (n_new + block - 1) / block};
+  return prefill_impl(ctx, layer, seq, n_new, q, out, out_dtype, lse, 1, all, pack);
+}
+
+int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_new, const void* q, void* out,
+                           int32_t out_dtype, float* lse, int32_t n_ranges, const int32_t* ranges) {
+  return prefill_impl(ctx, layer, seq, n_new, q, out, out_dtype, lse, n_ranges, ranges, 1);
 }
 
 int oomattn_attention_forward_with_bias(oomattn_ctx* ctx, int32_t layer, int32_t batch, int32_t seq_len,
