@@ -84,6 +84,12 @@ EncodeTiledFn get_encode_fn() {
 
 }  // namespace
 
+// How a prefill is cut: q heads per tile (1, or the group over a 4-bit cache) and
+// key tiles per chunk (0: the rule of prefill_impl).
+struct PrefillPlan {
+  int pack, key_chunk;
+};
+
 struct oomattn_ctx {
   oomattn_config cfg;
   int device = 0;
@@ -134,6 +140,8 @@ struct oomattn_ctx {
   uint8_t* d_exp = nullptr;
   int exp_pages = 0;
   int* d_exp_table = nullptr;
+  PrefillPlan plan{1, 0};  // of the last such prefill: plan_n queries, plan_len tokens
+  int plan_n = 0, plan_len = 0;
   // Q8 linear: activation splits and split-K partials, and per-row-tile
   // arrival counters (zero between launches)
   uint8_t* d_q8_scratch = nullptr;
@@ -750,26 +758,31 @@ int decode_fill(int kv_dtype) {
 int decode_min_pages(int kv_dtype) { return kv_dtype == OOMATTN_DTYPE_Q4 ? kDecWarps * kQ4Pages : 1; }
 constexpr int kDecodeMaxSimSlots = 2048;
 
+// count items of one size, each to the slot of a min-heap of finish times that is free first.  Returns the last finish.
+long long take_slots(long long* heap, int slots, long long size, int count) {
+  long long end = 0;
+  for (int k = 0; k < count; ++k) {
+    heap[0] += size;
+    end = std::max(end, heap[0]);
+    int i = 0;
+    for (;;) {  // sift it down
+      const int l = 2 * i + 1, r = l + 1;
+      int m = i;
+      if (l < slots && heap[l] < heap[m]) m = l;
+      if (r < slots && heap[r] < heap[m]) m = r;
+      if (m == i) break;
+      std::swap(heap[i], heap[m]);
+      i = m;
+    }
+  }
+  return end;
+}
+
 long long lpt_makespan(const int* size, const int* count, int groups, int slots, int fill, long long* heap) {
   // min-heap of slot finish times, in pages
   for (int i = 0; i < slots; ++i) heap[i] = 0;
-  for (int gi = 0; gi < groups; ++gi) {
-    for (int k = 0; k < count[gi]; ++k) {
-      heap[0] += size[gi] + fill;  // the earliest free slot takes the item; sift it down
-      int i = 0;
-      for (;;) {
-        const int l = 2 * i + 1, r = l + 1;
-        int m = i;
-        if (l < slots && heap[l] < heap[m]) m = l;
-        if (r < slots && heap[r] < heap[m]) m = r;
-        if (m == i) break;
-        std::swap(heap[i], heap[m]);
-        i = m;
-      }
-    }
-  }
   long long mx = 0;
-  for (int i = 0; i < slots; ++i) mx = std::max(mx, heap[i]);
+  for (int gi = 0; gi < groups; ++gi) mx = std::max(mx, take_slots(heap, slots, size[gi] + fill, count[gi]));
   return mx;
 }
 
@@ -1071,13 +1084,59 @@ int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtenso
   return rc;
 }
 
+// The cut of a prefill over a 4-bit cache: heads per tile and key chunk with the
+// shortest schedule, in key tiles' time (2.1 us).  A launch's CTAs go to the SMs
+// in order, chunk by chunk and, in a chunk, the last queries first; each costs its
+// tiles and kUnit more, and the chunks' partials are written and read once.
+// Against the rule of prefill_impl (chunks of the work per SM): 700 queries behind
+// 9001 tokens of 32q/8kv 140 instead of 150 us, 32 behind 2000 17 instead of 19,
+// 1024 behind 9001 of 40q/8kv 251 instead of 299.  Making a plan takes 30 to 110 us
+// of the host.
+PrefillPlan plan_prefill(const oomattn_ctx* ctx, int n_new, int L) {
+  constexpr int kScale = 16, kUnit = 2 * kScale, kMaxChunks = 32, kMaxItems = 1500;
+  constexpr int kMaxSms = 1024;
+  const int sms = std::min(ctx->num_sms, kMaxSms);
+  long long heap[kMaxSms];
+  long long best = 0;
+  PrefillPlan plan{1, 0};
+  for (int pack = 1; pack <= ctx->group; pack += std::max(1, ctx->group - 1)) {
+    const int step = 2 * (128 / pack), pairs = (n_new + step - 1) / step, units = ctx->cfg.n_heads / pack;
+    auto tiles = [&](int p) { return (L - n_new + std::min(n_new, step * (p + 1)) + 127) / 128; };
+    const int most = tiles(pairs - 1);
+    int last_chunk = 0;
+    for (int c = 1; c <= std::min(kMaxChunks, most); ++c) {
+      if (c > 1 && (long long)pairs * units * c > kMaxItems) break;
+      const int chunk = (most + c - 1) / c, chunks = (most + chunk - 1) / chunk;
+      if (chunk == last_chunk) continue;
+      last_chunk = chunk;
+      for (int i = 0; i < sms; ++i) heap[i] = 0;
+      long long end = 0;
+      for (int y = 0; y < chunks; ++y)
+        for (int p = pairs - 1; p >= 0; --p) {
+          const int s = std::min(tiles(p) - y * chunk, chunk);
+          if (s > 0) end = std::max(end, take_slots(heap, sms, (long long)s * kScale + kUnit, units));
+        }
+      if (chunks > 1) end += 3 * kScale / 2 + (long long)chunks * n_new * ctx->cfg.n_heads * kScale / 8200;  // 1 KB each at 4 TB/s
+      if (!plan.key_chunk || end < best) {
+        best = end;
+        plan = PrefillPlan{pack, chunk};
+      }
+    }
+  }
+  return plan;
+}
+
 // Prefill over a 4-bit cache, few tokens (drafts to verify, a short tail of a
-// prompt): each as one decode row that sees the slots up to its own.  Up to 24
-// tokens: 24 by rows and 32 expanded (which pads either to 256) take 11.1 and
-// 20.6 us behind 500 tokens (40q/8kv), 15.2 and 23.1 behind 2000 (28q/4kv), 54.3
-// and 52.8 behind 9001 (32q/8kv), 119 and 112 behind 30000 (28q/4kv); 16 by rows
-// 9.4, 13.0, 42.9 and 88.5.
-constexpr int kQ4PrefillRows = 24;
+// prompt): each as one decode row that sees the slots up to its own.  The rows'
+// time grows with queries * tokens * kv heads, the expanded form's hardly with the
+// queries; by rows and expanded (us) 8 queries behind 30000 tokens of 28q/4kv take
+// 46.3 and 44.9, 12 behind 8000 21.9 and 24.5, 20 behind 4000 20.9 and 20.6, 32
+// behind 2000 18.5 and 17.2, 48 behind 1000 15.9 and 16.3; of 32q/8kv 12 behind
+// 9001 31.2 and 29.2, 20 behind 2000 17.6 and 16.8.
+constexpr int kQ4PrefillRows = 48;
+int q4_prefill_max_rows(const oomattn_ctx* ctx, int L) {
+  return std::min<long long>(kQ4PrefillRows, 5 + 200000 / ((long long)L * ctx->cfg.n_kv_heads));
+}
 int q4_prefill_rows(oomattn_ctx* ctx, int layer, int seq, int n_new, const void* q, void* out, int out_dtype,
                     float* lse) {
   if (!q || !out) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad prefill arguments");
@@ -1653,9 +1712,10 @@ int oomattn_set_test_flags(oomattn_ctx* ctx, int32_t flags) {
   return OOMATTN_OK;
 }
 
-// ranges: blocks of 2 * (128 / pack) queries.  pack: q heads per tile (1, or the group over a 4-bit cache).
+// ranges: blocks of 2 * (128 / pack) queries.
 static int prefill_impl(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_new, const void* q, void* out,
-                        int32_t out_dtype, float* lse, int32_t n_ranges, const int32_t* ranges, int pack) {
+                        int32_t out_dtype, float* lse, int32_t n_ranges, const int32_t* ranges,
+                        const PrefillPlan plan) {
   if (!ctx) return OOMATTN_ERR_INVALID_ARG;
   if (!q || !out || n_new <= 0 || !ranges || n_ranges <= 0)
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad prefill arguments");
@@ -1674,7 +1734,7 @@ static int prefill_impl(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
   const int L = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq];
   if (n_new > L) return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "n_new %d exceeds the cached length %d", n_new, L);
-  const int tpt = 128 / pack, n_units = ctx->cfg.n_heads / pack;
+  const int pack = plan.pack, tpt = 128 / pack, n_units = ctx->cfg.n_heads / pack;
   const int n_pairs = (n_new + 2 * tpt - 1) / (2 * tpt);
   if (n_ranges > kPfMaxRanges)
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "%d block ranges (at most %d)", n_ranges, kPfMaxRanges);
@@ -1713,7 +1773,8 @@ static int prefill_impl(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_
     }
   const int per_sm = (int)((work + ctx->num_sms - 1) / ctx->num_sms);
   int key_chunk = max_tiles;
-  if (2 * max_tiles > 3 * per_sm) key_chunk = std::max(kPfMinKeyChunk, per_sm);
+  if (plan.key_chunk > 0) key_chunk = plan.key_chunk;
+  else if (2 * max_tiles > 3 * per_sm) key_chunk = std::max(kPfMinKeyChunk, per_sm);
   const int n_chunks = (max_tiles + key_chunk - 1) / key_chunk;
   a.key_chunk = key_chunk;
   a.n_pad = (n_new + tpt - 1) / tpt * tpt;
@@ -1779,38 +1840,33 @@ static int prefill_impl(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_
   return OOMATTN_OK;
 }
 
-// Heads per tile of a prefill over a 4-bit cache: the group, or one, whichever
-// has fewer key tiles to multiply in all.
-static int prefill_pack(const oomattn_ctx* ctx, int n_new, int L) {
-  auto tiles = [&](int pack) {
-    const int step = 2 * (128 / pack);
-    long long sum = 0;
-    for (int q = 0; q < n_new; q += step) sum += (L - n_new + std::min(n_new, q + step) + 127) / 128;
-    return sum * (ctx->cfg.n_heads / pack);
-  };
-  return tiles(ctx->group) < tiles(1) ? ctx->group : 1;
-}
-
 int oomattn_prefill(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_new, const void* q, void* out,
                     int32_t out_dtype, float* lse) {
   if (!ctx) return OOMATTN_ERR_INVALID_ARG;
   if (n_new <= 0) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "bad prefill arguments");
-  int pack = 1;
   if (ctx->cfg.kv_dtype == OOMATTN_DTYPE_Q4) {
-    if (n_new <= kQ4PrefillRows) return q4_prefill_rows(ctx, layer, seq, n_new, q, out, out_dtype, lse);
     int rc = check_layer(ctx, layer);
     if (!rc) rc = check_seq(ctx, seq);
     if (rc) return rc;
-    pack = prefill_pack(ctx, n_new, ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq]);
+    const int L = ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + seq];
+    if (n_new > L) return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "n_new %d exceeds the cached length %d", n_new, L);
+    if (n_new <= q4_prefill_max_rows(ctx, L)) return q4_prefill_rows(ctx, layer, seq, n_new, q, out, out_dtype, lse);
+    if (ctx->plan_n != n_new || ctx->plan_len != L) {  // the layers of a step ask for the same plan
+      ctx->plan = plan_prefill(ctx, n_new, L);
+      ctx->plan_n = n_new;
+      ctx->plan_len = L;
+    }
+    const int block = 2 * (128 / ctx->plan.pack);
+    const int32_t all[2] = {0, (n_new + block - 1) / block};
+    return prefill_impl(ctx, layer, seq, n_new, q, out, out_dtype, lse, 1, all, ctx->plan);
   }
-  const int block = 2 * (128 / pack);
-  const int32_t all[2] = {0, (n_new + block - 1) / block};
-  return prefill_impl(ctx, layer, seq, n_new, q, out, out_dtype, lse, 1, all, pack);
+  const int32_t all[2] = {0, (n_new + 255) / 256};
+  return prefill_impl(ctx, layer, seq, n_new, q, out, out_dtype, lse, 1, all, PrefillPlan{1, 0});
 }
 
 int oomattn_prefill_blocks(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_new, const void* q, void* out,
                            int32_t out_dtype, float* lse, int32_t n_ranges, const int32_t* ranges) {
-  return prefill_impl(ctx, layer, seq, n_new, q, out, out_dtype, lse, n_ranges, ranges, 1);
+  return prefill_impl(ctx, layer, seq, n_new, q, out, out_dtype, lse, n_ranges, ranges, PrefillPlan{1, 0});
 }
 
 int oomattn_attention_forward_with_bias(oomattn_ctx* ctx, int32_t layer, int32_t batch, int32_t seq_len,

@@ -286,7 +286,7 @@ def test_decode_static_scratch(lib):
 # ----------------------------------------------------------------------------------------------- prefill
 @pytest.mark.parametrize("heads", [(28, 4), (8, 8), (10, 2), (16, 2), (9, 3)])
 @pytest.mark.parametrize("n_new,prefix", [(1, 0), (1, 50), (7, 9), (16, 100), (24, 0), (25, 0), (25, 111), (100, 28), (300, 500),
-                                          (37, 2000)])
+                                          (24, 3000), (60, 2000)])
 @pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
 def test_prefill(heads, n_new, prefix, out_dtype):
     n = n_new + prefix
@@ -305,10 +305,10 @@ def test_prefill(heads, n_new, prefix, out_dtype):
 
 def test_prefill_grows_and_shrinks():
     """One engine, two sequences of unlike length in turn: what an earlier, longer one left in the scratch stays out."""
-    lens = [700, 40, 1500, 33]
+    lens = [700, 55, 1500, 49]
     eng, ks, vs = _filled(8, 2, lens, seed=9)
     for s in (0, 1, 2, 3, 1):
-        n_new = min(30, lens[s])
+        n_new = min(60, lens[s])
         q = randn((n_new, 8, 128), 90 + s, torch.bfloat16)
         out = eng.prefill(0, s, q.cuda())
         eng.sync()
@@ -418,8 +418,8 @@ def test_many_splits_captured_and_replayed():
 
 
 def test_prefill_reports_values_outside_fp16():
-    """More than 24 queries: a NaN of V (which a product with a weight of zero would spread) and a q value that fp16 does
-    not hold are reported; up to 24 queries take both."""
+    """Many queries: a NaN of V (which a product with a weight of zero would spread) and a q value that fp16 does
+    not hold are reported; few queries take both."""
     from oomllama_b200._lib import OomAttnError
     n = 200
     k, v = randn((n, 2, 128), 1), randn((n, 2, 128), 2)
