@@ -1090,11 +1090,10 @@ int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtenso
 // tiles and kUnit more, and the chunks' partials are written and read once.
 // Against the rule of prefill_impl (chunks of the work per SM): 700 queries behind
 // 9001 tokens of 32q/8kv 140 instead of 150 us, 32 behind 2000 17 instead of 19,
-// 1024 behind 9001 of 40q/8kv 251 instead of 299.  Making a plan takes 30 to 110 us
+// 1024 behind 9001 of 40q/8kv 251 instead of 299.  Making a plan takes 20 to 60 us
 // of the host.
 PrefillPlan plan_prefill(const oomattn_ctx* ctx, int n_new, int L) {
-  constexpr int kScale = 16, kUnit = 2 * kScale, kMaxChunks = 32, kMaxItems = 1500;
-  constexpr int kMaxSms = 1024;
+  constexpr int kScale = 16, kUnit = 2 * kScale, kMaxChunks = 32, kMaxItems = 600, kMaxSms = 1024;
   const int sms = std::min(ctx->num_sms, kMaxSms);
   long long heap[kMaxSms];
   long long best = 0;
@@ -1103,11 +1102,16 @@ PrefillPlan plan_prefill(const oomattn_ctx* ctx, int n_new, int L) {
     const int step = 2 * (128 / pack), pairs = (n_new + step - 1) / step, units = ctx->cfg.n_heads / pack;
     auto tiles = [&](int p) { return (L - n_new + std::min(n_new, step * (p + 1)) + 127) / 128; };
     const int most = tiles(pairs - 1);
+    long long work = 0;
+    for (int p = 0; p < pairs; ++p) work += (long long)tiles(p) * units;
+    // chunks to try: equal parts, and the work per SM and up to a quarter more (k < 0)
     int last_chunk = 0;
-    for (int c = 1; c <= std::min(kMaxChunks, most); ++c) {
-      if (c > 1 && (long long)pairs * units * c > kMaxItems) break;
-      const int chunk = (most + c - 1) / c, chunks = (most + chunk - 1) / chunk;
-      if (chunk == last_chunk) continue;
+    for (int k = -5; k < std::min(kMaxChunks, most); ++k) {
+      const long long share = (work + sms - 1) / sms * (11 - k) / 16;
+      const int chunk = k < 0 ? (int)std::min<long long>(most, std::max(1ll, share)) : (most + k) / (k + 1);
+      const int chunks = (most + chunk - 1) / chunk;
+      if (chunk == last_chunk || chunks > kMaxChunks) continue;
+      if (chunks > 1 && (long long)pairs * units * chunks > kMaxItems) continue;
       last_chunk = chunk;
       for (int i = 0; i < sms; ++i) heap[i] = 0;
       long long end = 0;
