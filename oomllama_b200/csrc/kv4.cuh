@@ -155,22 +155,17 @@ __host__ __device__ __forceinline__ int q4_v_meta(int tok) {  // the pair's 4 x 
 }
 
 // ---------------------------------------------------------------- rows read back
-__global__ void iota_kernel(int* p, int n) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < n) p[i] = i;
-}
-
 struct GatherArgs {
   void* k_out;
   void* v_out;
   int layer;
   int n;          // tokens per row: slots sb.len[z] .. sb.len[z] + n - 1
   int pages;      // pages a row's range can touch
-  int paged;      // 1: out as pool pages [page][n_kv][16][128] from slot 0, zeros at and past slot n
+  int head_rows;  // not 0: out as [n_kv][head_rows][128] from slot 0, zeros at and past slot n
   int* status;
 };
 
-enum : int { kOutF32 = 0, kOutBf16 = 1, kOutF16 = 2 };  // f16: paged, of a 4-bit cache only
+enum : int { kOutF32 = 0, kOutBf16 = 1, kOutF16 = 2 };  // f16: by heads, of a 4-bit cache only
 template <int OUT>
 __device__ __forceinline__ void store4(void* p, size_t i, const float* x) {
   if (OUT == kOutBf16) {
@@ -183,7 +178,7 @@ __device__ __forceinline__ void store4(void* p, size_t i, const float* x) {
 // LayerKVCache::get (oomllama_turbo.rs:57-63) on the device: the cached rows as
 // values.  One CTA of 128 threads per (row, page, kv head): 64 threads read the
 // K chunk, 64 the V chunk; a thread's 128-bit load is 32 codes (4-bit cache).
-// A 4-bit page is 2.5 KB read for 8 KB (16-bit) written; for the prefill's pages
+// A 4-bit page is 2.5 KB read for 8 KB (16-bit) written; for the prefill's rows
 // the arithmetic is in f16 pairs (9334 tokens of 8 kv heads 14.8 us in f32).
 template <int KV, int OUT>
 __global__ void __launch_bounds__(128)
@@ -196,7 +191,7 @@ __global__ void __launch_bounds__(128)
   const int first = sb.len[z], last = first + a.n;  // slots wanted
   const int lp = first / kPageSize + (rest - z * a.pages);
   const int s0 = lp * kPageSize;
-  if (!a.paged && s0 >= last) return;
+  if (!a.head_rows && s0 >= last) return;
   const bool held = s0 < last;
   int page = pool.n_pool_pages - 1;
   if (held) {
@@ -211,11 +206,10 @@ __global__ void __launch_bounds__(128)
   void* out = is_v ? a.v_out : a.k_out;
   // element offset of (slot, dim) in the output
   auto at = [&](int slot, int d) -> size_t {
-    return a.paged ? (((size_t)lp * pool.n_kv + g) * kPageSize + (slot - s0)) * kHeadDim + d
-                   : (((size_t)z * a.n + (slot - first)) * pool.n_kv + g) * kHeadDim + d;
+    return a.head_rows ? ((size_t)g * a.head_rows + slot) * kHeadDim + d
+                       : (((size_t)z * a.n + (slot - first)) * pool.n_kv + g) * kHeadDim + d;
   };
   auto wanted = [&](int slot) { return slot >= first && slot < last; };
-  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
   if (KV == kKvQ4) {
     const uint8_t* c = static_cast<const uint8_t*>(is_v ? pool.v : pool.k) + q4_chunk_off(pool, a.layer, page, g);
     const uint4 w4 = *reinterpret_cast<const uint4*>(c + u * 16);
@@ -271,7 +265,7 @@ __global__ void __launch_bounds__(128)
       const int tok = (u & 31) >> 1, t = (u & 1) * 2, slot = s0 + tok;
       const uint32_t o2 = *reinterpret_cast<const uint32_t*>(c + kQ4Meta + tok * 16 + wp * 4);
       const uint32_t s2 = *reinterpret_cast<const uint32_t*>(c + kQ4Meta + tok * 16 + 8 + wp * 4);
-      if (!wanted(slot) && !a.paged) return;
+      if (!wanted(slot)) return;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const float o = __half2float(__ushort_as_half((uint16_t)(o2 >> (16 * q))));
@@ -280,7 +274,7 @@ __global__ void __launch_bounds__(128)
         for (int e = 0; e < 2; ++e) {  // t and t + 1 of this group: 16 dims in a row
           float x[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = wanted(slot) ? q4_value((w[2 * e + q] >> (4 * i)) & 15u, s, o) : 0.f;
+          for (int i = 0; i < 8; ++i) x[i] = q4_value((w[2 * e + q] >> (4 * i)) & 15u, s, o);
           store8<OUT == kOutBf16>(out, at(slot, 32 * (2 * wp + q) + 8 * (t + e)), x);
         }
       }
@@ -294,7 +288,7 @@ __global__ void __launch_bounds__(128)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const int slot = s0 + 8 * h + 2 * t + p;
-          if (!wanted(slot) && !a.paged) continue;
+          if (!wanted(slot)) continue;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const float o = __half2float(__ushort_as_half((uint16_t)((q ? o4.y : o4.x) >> (16 * p))));
@@ -302,7 +296,7 @@ __global__ void __launch_bounds__(128)
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = q4_value((w[2 * tt + q] >> (16 * p + 4 * i)) & 15u, s, o);
-            store4<OUT>(out, at(slot, 32 * (2 * wp + q) + 4 * gg), wanted(slot) ? x : zero);
+            store4<OUT>(out, at(slot, 32 * (2 * wp + q) + 4 * gg), x);
           }
         }
       }

@@ -134,12 +134,10 @@ struct oomattn_ctx {
   // scratch blocks that a larger one replaced: captured graphs may still name them
   void* kept[96] = {};
   int n_kept = 0;
-  // prefill over a 4-bit cache: one sequence's rows of one layer as fp16 pages
-  // [exp_pages + 1][n_kv][16][128] of K, then of V (the last page zero), and the
-  // block table that names them in order
+  // prefill over a 4-bit cache: one sequence's rows of one layer in fp16,
+  // [n_kv][16 exp_pages][128] of K, then of V
   uint8_t* d_exp = nullptr;
   int exp_pages = 0;
-  int* d_exp_table = nullptr;
   PrefillPlan plan{1, 0};  // of the last such prefill: plan_n queries, plan_len tokens
   int plan_n = 0, plan_len = 0;
   // Q8 linear: activation splits and split-K partials, and per-row-tile
@@ -246,13 +244,13 @@ void build_rope_table(float theta, int n_pos, std::vector<float>& c, std::vector
   for (std::thread& t : threads) t.join();
 }
 
-int encode_pool_map(oomattn_ctx* ctx, void* base, uint64_t n_pages, CUtensorMap* map) {
+int encode_pool_map(oomattn_ctx* ctx, void* base, uint64_t n_pages, CUtensorMap* map, int box_rows = kPageSize) {
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) return fail(ctx, OOMATTN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   const uint64_t rows = n_pages * ctx->cfg.n_kv_heads * kPageSize;
   cuuint64_t dims[2] = {(cuuint64_t)kHeadDim, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)kHeadDim * 2};
-  cuuint32_t box[2] = {64, (cuuint32_t)kPageSize};
+  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1028,37 +1026,27 @@ int project(oomattn_ctx* ctx, const float* x, int T, int k, const KfJob* jobs, i
   return OOMATTN_OK;
 }
 
-// Prefill over a 4-bit cache, many tokens: the sequence's rows of one layer as
-// fp16 pages (11 bits of the held values; bf16 would keep 8: 0.0029 to 0.0032
-// off the exact output instead of 0.0017, which is that of its own rounding), in
-// order, which the tensor-core prefill then reads as its pool.
-// It reads 160 and writes 512 bytes per token and kv head once, for the 4 * 128
-// * group * n_new products that each of those tokens takes part in.
+// Prefill over a 4-bit cache, many tokens: the sequence's rows of one layer in
+// fp16 (11 bits of the held values; bf16 would keep 8: 0.0029 to 0.0032 off the
+// exact output instead of 0.0017, which is that of its own rounding), in order,
+// for the tensor-core prefill.  It reads 160 and writes 512 bytes per token and kv
+// head once, for the 4 * 128 * group * n_new products that each of those tokens
+// takes part in.
 int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtensorMap* kmap, CUtensorMap* vmap) {
   const int n_kv = ctx->cfg.n_kv_heads;
   const int pages = ((L + kPageSize - 1) / kPageSize + 7) / 8 * 8;  // the prefill's 128-key tiles: zeros past L
   const size_t page_bytes = (size_t)n_kv * kPageSize * kHeadDim * 2;
   if (pages > ctx->exp_pages) {
     const int cap = pages + pages / 2;  // a growing sequence does not reallocate at every chunk
-    if ((long long)(cap + 1) * n_kv * kPageSize >= (1ll << 31))
+    if ((long long)cap * n_kv * kPageSize >= (1ll << 31))
       return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "prefill over %d tokens of a 4-bit cache", L);
-    // K pages, V pages, table
-    const size_t half_bytes = (size_t)(cap + 1) * page_bytes, bytes = 2 * half_bytes + (size_t)cap * sizeof(int);
     void* p = ctx->d_exp;
-    const int rc = grow_block(ctx, &p, bytes, "the prefill's scratch");
+    const int rc = grow_block(ctx, &p, 2 * (size_t)cap * page_bytes, "the prefill's scratch");
     if (rc) return rc;
     ctx->d_exp = static_cast<uint8_t*>(p);
-    ctx->exp_pages = 0;  // until it is set up
-    uint8_t* b = static_cast<uint8_t*>(p);
-    int* table = reinterpret_cast<int*>(b + 2 * half_bytes);
-    CK(cudaMemsetAsync(b + half_bytes - page_bytes, 0, page_bytes, ctx->stream));  // the null pages
-    CK(cudaMemsetAsync(b + 2 * half_bytes - page_bytes, 0, page_bytes, ctx->stream));
-    iota_kernel<<<(cap + 255) / 256, 256, 0, ctx->stream>>>(table, cap);
-    CKLAUNCH();
-    ctx->d_exp_table = table;
     ctx->exp_pages = cap;
   }
-  const size_t half = (size_t)(ctx->exp_pages + 1) * page_bytes;
+  uint8_t* v_rows = ctx->d_exp + (size_t)ctx->exp_pages * page_bytes;
   SeqBatch sb;
   sb.n = 1;
   sb.seq[0] = seq;
@@ -1066,21 +1054,16 @@ int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtenso
   sb.pos[0] = 0;
   GatherArgs a;
   a.k_out = ctx->d_exp;
-  a.v_out = ctx->d_exp + half;
+  a.v_out = v_rows;
   a.layer = layer;
   a.n = L;
   a.pages = pages;
-  a.paged = 1;
+  a.head_rows = ctx->exp_pages * kPageSize;
   a.status = ctx->d_status;
   int rc = launch_gather(ctx, a, sb, kOutF16);
-  if (!rc) rc = encode_pool_map(ctx, ctx->d_exp, (uint64_t)ctx->exp_pages + 1, kmap);
-  if (!rc) rc = encode_pool_map(ctx, ctx->d_exp + half, (uint64_t)ctx->exp_pages + 1, vmap);
-  pool->k = ctx->d_exp;
-  pool->v = ctx->d_exp + half;
-  pool->block_table = ctx->d_exp_table;
-  pool->max_pages_per_seq = pages;
-  pool->n_pool_pages = ctx->exp_pages + 1;
-  pool->kv_bf16 = 1;
+  if (!rc) rc = encode_pool_map(ctx, ctx->d_exp, ctx->exp_pages, kmap, 128);
+  if (!rc) rc = encode_pool_map(ctx, v_rows, ctx->exp_pages, vmap, 128);
+  pool->n_pool_pages = ctx->exp_pages;  // per kv head
   return rc;
 }
 
@@ -1501,7 +1484,7 @@ int oomattn_kv_gather(oomattn_ctx* ctx, int32_t layer, int32_t n_seqs, const int
     a.layer = layer;
     a.n = n;
     a.pages = (n + kPageSize - 2) / kPageSize + 1;  // the most that n slots can touch
-    a.paged = 0;
+    a.head_rows = 0;
     a.status = ctx->d_status;
     rc = launch_gather(ctx, a, sb, out_dtype == OOMATTN_DTYPE_BF16 ? kOutBf16 : kOutF32);
     if (rc) return rc;
