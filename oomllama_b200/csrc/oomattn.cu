@@ -115,7 +115,7 @@ struct oomattn_ctx {
   int* d_status = nullptr;
   CUtensorMap kmap{}, vmap{};
   bool have_maps = false;
-  int prefill_regs[2] = {0, 0};  // compiled register counts of the prefill kernel (bf16 pages, fp16 pages)
+  int prefill_regs[2] = {0, 0};  // compiled register counts of the prefill kernel (bf16 pages, fp16 rows)
   int kf_q8_regs = 0;    // and of the Q8 tensor-core linear (its register split needs kKfLaunchRegs)
   // host mirrors (authoritative for lengths; updated at enqueue time)
   std::vector<int> h_block_table;  // [max_seqs][max_pages_per_seq]

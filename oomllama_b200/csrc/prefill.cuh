@@ -771,19 +771,43 @@ __global__ void prefill_chunk_merge_kernel(const float* __restrict__ part_o, con
   const int tile_end = min(a.n_new, (row / a.tile_tokens + 1) * a.tile_tokens);
   const int nt = (a.prefix + tile_end + 127) / 128;
   const int nc = (nt + a.key_chunk - 1) / a.key_chunk;
-  float M = -INFINITY;
-  for (int c = 0; c < nc; ++c) M = fmaxf(M, a.part_lse[((size_t)c * a.n_pad + row) * a.n_heads + h]);
+  // four chunks at a time: their loads are in flight together (333 rows of 32 heads in 3 chunks: 2 us less)
+  constexpr int B = 4;
+  auto lse_at = [&](int c) { return a.part_lse[((size_t)c * a.n_pad + row) * a.n_heads + h]; };
+  auto o_at = [&](int c) {
+    return __ldg(reinterpret_cast<const float4*>(part_o + (((size_t)c * a.n_pad + row) * a.n_heads + h) * kHeadDim) + lane);
+  };
+  float ls[B];
+  float4 o[B];
+#pragma unroll
+  for (int k = 0; k < B; ++k) {
+    ls[k] = k < nc ? lse_at(k) : -INFINITY;
+    o[k] = k < nc ? o_at(k) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  float M = fmaxf(fmaxf(ls[0], ls[1]), fmaxf(ls[2], ls[3]));
+#pragma unroll 4
+  for (int c = B; c < nc; ++c) M = fmaxf(M, lse_at(c));
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float wsum = 0.f;
-  for (int c = 0; c < nc; ++c) {
-    const float w = expf(a.part_lse[((size_t)c * a.n_pad + row) * a.n_heads + h] - M);
-    const float4 o = __ldg(reinterpret_cast<const float4*>(part_o + (((size_t)c * a.n_pad + row) * a.n_heads + h) *
-                                                           kHeadDim) + lane);
-    wsum += w;
-    acc.x += w * o.x;
-    acc.y += w * o.y;
-    acc.z += w * o.z;
-    acc.w += w * o.w;
+  for (int c0 = 0; c0 < nc; c0 += B) {
+    if (c0 > 0) {
+#pragma unroll
+      for (int k = 0; k < B; ++k)
+        if (c0 + k < nc) {
+          ls[k] = lse_at(c0 + k);
+          o[k] = o_at(c0 + k);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < B; ++k)
+      if (c0 + k < nc) {
+        const float w = expf(ls[k] - M);
+        wsum += w;
+        acc.x += w * o[k].x;
+        acc.y += w * o[k].y;
+        acc.z += w * o[k].z;
+        acc.w += w * o[k].w;
+      }
   }
   const float inv = 1.f / wsum;
   const size_t o_off = ((size_t)row * a.n_heads + h) * kHeadDim + lane * 4;
