@@ -347,8 +347,8 @@ int oomattn_decode_static_scratch_status(int device, void* stream, int32_t* flag
 
 /* Causal prefill of the n_new newest tokens of `seq` (bf16 or 4-bit cache):
  * query i (absolute slot len-n_new+i) attends to slots 0..len-n_new+i.
- * Over a 4-bit cache few queries (up to 5 + 200000 / (len * n_kv_heads), at most
- * 48) run as decode rows, without limits on values; more take the cached rows and
+ * Over a 4-bit cache few queries (up to 5 + 200000 / (len * n_kv_heads), with
+ * groups of at most four heads 7 + 260000 / (len * n_kv_heads), at most 48) run as decode rows, without limits on values; more take the cached rows and
  * q as fp16, and a q value of magnitude 65536 or more, or a NaN in q or V, gives
  * OOMATTN_ERR_DEVICE_CHECK at oomattn_sync.
  *   q: bf16 [n_new][n_heads][128] rotated; out: [n_new][n_heads][128] in

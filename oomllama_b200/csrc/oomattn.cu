@@ -1118,11 +1118,12 @@ PrefillPlan plan_prefill(const oomattn_ctx* ctx, int n_new, int L) {
 // time grows with queries * tokens * kv heads, the expanded form's hardly with the
 // queries; by rows and expanded (us) 8 queries behind 30000 tokens of 28q/4kv take
 // 46.3 and 44.9, 12 behind 8000 21.9 and 24.5, 20 behind 4000 20.9 and 20.6, 32
-// behind 2000 18.5 and 17.2, 48 behind 1000 15.9 and 16.3; of 32q/8kv 12 behind
-// 9001 31.2 and 29.2, 20 behind 2000 17.6 and 16.8.
+// behind 2000 18.5 and 17.2, 48 behind 1000 15.9 and 16.3; of 32q/8kv (the narrow
+// decode) 8 behind 9001 23.4 and 29.1, 12 31.2 and 29.2, 20 behind 2000 17.6 and 16.8.
 constexpr int kQ4PrefillRows = 48;
 int q4_prefill_max_rows(const oomattn_ctx* ctx, int L) {
-  return std::min<long long>(kQ4PrefillRows, 5 + 200000 / ((long long)L * ctx->cfg.n_kv_heads));
+  const long long keys = (long long)L * ctx->cfg.n_kv_heads;
+  return std::min<long long>(kQ4PrefillRows, q4_wide(ctx->group) ? 5 + 200000 / keys : 7 + 260000 / keys);
 }
 int q4_prefill_rows(oomattn_ctx* ctx, int layer, int seq, int n_new, const void* q, void* out, int out_dtype,
                     float* lse) {
