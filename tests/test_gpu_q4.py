@@ -284,7 +284,7 @@ def test_decode_static_scratch(lib):
 
 
 # ----------------------------------------------------------------------------------------------- prefill
-@pytest.mark.parametrize("heads", [(28, 4), (8, 8), (10, 2), (16, 2), (9, 3)])
+@pytest.mark.parametrize("heads", [(28, 4), (8, 8), (10, 2), (16, 2), (9, 3), (6, 1), (8, 2)])
 @pytest.mark.parametrize("n_new,prefix", [(1, 0), (1, 50), (7, 9), (16, 100), (24, 0), (25, 0), (25, 111), (100, 28), (300, 500),
                                           (24, 3000), (60, 2000)])
 @pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
