@@ -157,7 +157,10 @@ __device__ __forceinline__ void merge_splits_staged(const DecodeArgs& a, int z, 
 // without one (the f32 kernel, which holds no shared ring) the partials are
 // loaded into registers.
 // kLate: the launch may leave the merge to a kernel after it (no counters).
-template <bool OUT16 = false, bool kLate = false>
+// kBias: l and O are 2^kBias times what they are about 2^m (m so much lower); O / l
+// cancels it, the lse takes it out of both before its logarithm, whose last bit it
+// would cost otherwise.
+template <bool OUT16 = false, bool kLate = false, int kBias = 0>
 __device__ __forceinline__ void combine_and_store(const MergeSmem& ms, const DecodeArgs& a, int z, int g, int split,
                                                   int nsplit, int n_kv, int tid, int* s_last, float* stage,
                                                   int stage_floats, float* s_w) {
@@ -188,7 +191,7 @@ __device__ __forceinline__ void combine_and_store(const MergeSmem& ms, const Dec
     const float inv = 1.f / lsum;
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] *= inv;
-    lse2 = M + log2f(lsum);
+    lse2 = kBias ? (M + kBias) + log2f(lsum * (1.f / (1 << kBias))) : M + log2f(lsum);
     if (nsplit == 1) {
       const size_t zh = (size_t)z * a.n_heads + h;
       store_out4<OUT16>(a, zh, da, acc[0], acc[1], acc[2], acc[3]);

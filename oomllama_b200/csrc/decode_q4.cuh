@@ -13,13 +13,17 @@
 //
 // Tiles.  m16n8k16 with keys (K) or dims (V) as the 16 rows and query heads as
 // the 8 columns; a query (or probability) enters as an f16 high part and a low
-// one (x - high), 22 bits of the f32 value together.  A group of up to four
-// heads (WIDE = false) has both parts side by side, column 2 h the high part
-// of head h, column 2 h + 1 the low: one product does both, and the two
-// columns of an accumulator lie in one lane.  A group of five to eight (WIDE)
-// has a column per head and a second product for the low parts.  (Heads as rows,
-// eight high and eight low, would cost a group of four as many products as one
-// of eight: 96.2 instead of 66.7 us for 8 x 32768 tokens of 32q/8kv.)
+// one (x - high), 22 bits of the f32 value together.  Probabilities are held at
+// 2^14 times their size (kQ4PBias): f16 ends at 2^-24, so a weight keeps its 22
+// bits down to 2^-16 of the largest and is off by 2^-39 of it at most below that.
+// (At their own size all below 2^-25 were lost from O but not from the sum l:
+// beside a key 17.5 nats above 8191 others, a quarter of what those carry.)
+// A group of up to four heads (WIDE = false) has both parts side by side, column
+// 2 h the high part of head h, column 2 h + 1 the low: one product does both, and
+// the two columns of an accumulator lie in one lane.  A group of five to eight
+// (WIDE) has a column per head and a second product for the low parts.  (Heads as
+// rows, eight high and eight low, would cost a group of four as many products as
+// one of eight: 96.2 instead of 66.7 us for 8 x 32768 tokens of 32q/8kv.)
 // K codes enter as subnormal halves (code * 2^-24, or 2^-20 for the upper nibble
 // of a byte, whose q is prescaled by 1/16): unpacking is one AND per two codes.
 // q is scaled by a power of two to [2^14, 2^15) per head, and its high part put
@@ -58,6 +62,11 @@ constexpr int kQ4TileBytes = kQ4Pages * kQ4Pair;         // 5 KB
 // stages each, or three of three, per SM -- about 160 and 180 KB in flight.
 __host__ __device__ constexpr int q4_stages(bool wide) { return !wide ? 2 : 3; }
 __host__ __device__ constexpr int q4_ctas_per_sm(bool wide) { return !wide ? 4 : 3; }
+// The running maximum that weights are taken against lies this far (base 2) below
+// the largest logit: weights in (0, 2^14], and so l and O, which cancels in O / l
+// and in the lse.  An f16 high part holds up to 2^15.99, which leaves room for the
+// maximum's own rounding (half a unit of its last place: logits to 2^24).
+constexpr int kQ4PBias = 14;
 __host__ __device__ constexpr int q4_ring_bytes(bool wide) { return kDecWarps * q4_stages(wide) * kQ4TileBytes; }
 __host__ __device__ constexpr int q4_tail_bytes(bool wide) {  // barriers, a flag, merge weights
   return kDecWarps * q4_stages(wide) * 8 + 64 + kMaxGroup * 32 * 4;
@@ -272,7 +281,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
   // O of the lane: dims 32 w + 4 g + 2 i + r.  Wide: [w][2 i + r] of heads (2 t, 2 t + 1);
   // narrow: [w][i] of head t, r = 0 and 1.  oo: sum p * offset of groups 2 (g % 2) and + 1.
   uint64_t o[4][2 * HL];
-  float oo[HL][2], m[HL], l[HL];  // m: the running maximum as a base-2 logit
+  float oo[HL][2], m[HL], l[HL];  // m: the running maximum as a base-2 logit, less kQ4PBias
 #pragma unroll
   for (int w = 0; w < 4; ++w)
 #pragma unroll
@@ -387,7 +396,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, off));
       // the running maximum is rounded: the same number enters every weight, so its rounding cancels
-      const float mf = fmaxf(m[h], mt * f2[h]);
+      const float mf = fmaxf(m[h], fmaf(mt, f2[h], -(float)kQ4PBias));
       alpha[h] = ex2_ftz(m[h] - mf);
       m[h] = mf;
       float ps = 0.f;
@@ -515,7 +524,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
     }
   }
   consumer_bar();
-  combine_and_store<OUT16, true>(ms, a, z, g_kv, item.split, item.nsplit, pool.n_kv, threadIdx.x, s_last,
+  combine_and_store<OUT16, true, kQ4PBias>(ms, a, z, g_kv, item.split, item.nsplit, pool.n_kv, threadIdx.x, s_last,
                           reinterpret_cast<float*>(smem_q4), kRing / 4, s_w);
 }
 
