@@ -48,3 +48,34 @@ def test_decode_weights_below_a_dominant_key(heads, n, rows):
     want_lse = 1.546875 * 128 / math.sqrt(128) + math.log1p((n - 1) * math.exp(-1.546875 * 128 / math.sqrt(128)))
     np.testing.assert_allclose(lse.cpu().numpy(), want_lse, rtol=2e-6)
     eng.close()
+
+
+# ----------------------------------------------------------------------------------------------- the scale
+def _held(x):
+    """The definition that include/oomattn.h gives: the scale is the range times 1/15 in f32, rounded to bf16."""
+    g = x.float().unflatten(-1, (4, 32))
+    lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
+    s = ((hi - lo) * (torch.ones(()) / 15)).bfloat16().half().float()
+    o = (lo + 8 * s).half().float()
+    c = torch.where(s > 0, ((g - o) / s).round().clamp(-8, 7), torch.zeros(()))
+    return (o + c * s).flatten(-2)
+
+
+def test_scale_on_a_border():
+    """Groups whose (max - min) * (1/15) and (max - min) / 15 round to different bf16 numbers: the former is held, and
+    what is held is within the format's bound of the row either way."""
+    r = 1 + 3 * torch.rand(1 << 24, generator=torch.Generator().manual_seed(1))
+    r = r[(r / 15).bfloat16() != (r * (torch.ones(()) / 15)).bfloat16()]
+    n = r.numel() // 8
+    assert n >= 8
+    x = torch.rand(2 * n * 4, 32, generator=torch.Generator().manual_seed(2)) * r[:8 * n, None]
+    x[:, 0], x[:, 31] = 0, r[:8 * n]
+    k, v = x.view(2, n, 1, 128)
+    eng = make_engine(4, 1, [n], kv_dtype="q4")
+    eng.kv_write(0, 0, k.contiguous().cuda(), v.contiguous().cuda())
+    kg, vg = eng.kv_gather(0, [0])
+    eng.sync()
+    np.testing.assert_array_equal(kg.cpu().numpy(), _held(k).numpy())
+    np.testing.assert_array_equal(vg.cpu().numpy(), _held(v).numpy())
+    assert ((kg.cpu().double() - k.double()).abs() <= q4_ref.code_bound(k)).all()
+    eng.close()
