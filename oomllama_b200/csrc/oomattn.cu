@@ -946,6 +946,10 @@ int decode_rows_impl(oomattn_ctx* ctx, int layer, int n_rows, const int32_t* seq
                      const float* q, float* out, float* lse, int o_stride, int lse_stride, DecIo io = DecIo::kF32) {
   int rc = check_layer(ctx, layer);
   if (rc) return rc;
+  // out is written by 16-byte stores; q is read by 8-byte loads from a bf16 cache's decode, by 16-byte ones else
+  const uintptr_t q_mask = ctx->cfg.kv_dtype == OOMATTN_DTYPE_BF16 ? 7 : 15;
+  if ((reinterpret_cast<uintptr_t>(q) & q_mask) || !aligned16(out) || (reinterpret_cast<uintptr_t>(lse) & 3))
+    return fail(ctx, OOMATTN_ERR_INVALID_ARG, "q and out must be %d- and 16-byte aligned, lse 4-byte", (int)q_mask + 1);
   DeviceGuard dg(ctx->device);
   const int hq = ctx->cfg.n_heads;
   for (int r0 = 0; r0 < n_rows; r0 += kMaxBatch) {
@@ -2020,10 +2024,11 @@ extern "C" int oomattn_decode_static_scratch(int device, void* stream, int32_t k
     return static_fail(errbuf, errbuf_len, OOMATTN_ERR_OUT_OF_RANGE, "pool of %d pages unsupported", n_pool_pages);
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u)
     return static_fail(errbuf, errbuf_len, OOMATTN_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
-  if (kv_dtype == OOMATTN_DTYPE_Q4 && ((reinterpret_cast<uintptr_t>(k_pool) & 15u) ||
-                                       static_cast<const uint8_t*>(v_pool) != static_cast<const uint8_t*>(k_pool) + kQ4Chunk))
+  if ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15u)
+    return static_fail(errbuf, errbuf_len, OOMATTN_ERR_INVALID_ARG, "the pools must be 16-byte aligned");
+  if (kv_dtype == OOMATTN_DTYPE_Q4 && static_cast<const uint8_t*>(v_pool) != static_cast<const uint8_t*>(k_pool) + kQ4Chunk)
     return static_fail(errbuf, errbuf_len, OOMATTN_ERR_INVALID_ARG,
-                       "a 4-bit pool must be 16-byte aligned, its V chunks %d bytes behind its K chunks", kQ4Chunk);
+                       "a 4-bit pool's V chunks must lie %d bytes behind its K chunks", kQ4Chunk);
   SeqBatch sb;
   sb.n = n_rows;
   for (int z = 0; z < n_rows; ++z) {
