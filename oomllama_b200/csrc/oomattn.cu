@@ -617,10 +617,9 @@ int launch_rope_append(oomattn_ctx* ctx, const AppendArgs& ap, const SeqBatch& s
 // The append with a norm of the q and k heads and / or into a 4-bit cache: one
 // warp per four heads of a token (qk_norm.cuh).
 int launch_qk_norm_append(oomattn_ctx* ctx, const AppendArgs& ap, const NormArgs& na, const SeqBatch& sb, int T) {
-  const void* ptrs[] = {ap.q, ap.k, ap.v, ap.q_out, ap.bq, ap.bk, ap.bv, na.qw, na.kw};
+  const void* ptrs[] = {ap.q, ap.k, ap.v, ap.q_out, ap.bq, ap.bk, ap.bv};  // na's: check_norm
   for (const void* p : ptrs)
-    if (p && !aligned16(p))
-      return fail(ctx, OOMATTN_ERR_INVALID_ARG, "tensors, biases and norm weights must be 16-byte aligned");
+    if (p && !aligned16(p)) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "tensors and biases must be 16-byte aligned");
   const int hq = ctx->cfg.n_heads, hkv = ctx->cfg.n_kv_heads, kv = ctx->cfg.kv_dtype;
   const long long qw = ap.q ? (hq + 3) / 4 : 0, kw = ap.k ? (hkv + 3) / 4 : 0;
   const bool q4 = kv == OOMATTN_DTYPE_Q4;
@@ -657,9 +656,14 @@ int launch_append(oomattn_ctx* ctx, const AppendArgs& ap, const oomattn_qk_norm*
   return launch_rope_append(ctx, ap, sb, T);
 }
 
-int check_norm(oomattn_ctx* ctx, const oomattn_qk_norm* norm) {
-  if (norm && !(norm->eps >= 0.f && norm->eps <= 3.4e38f))
-    return fail(ctx, OOMATTN_ERR_INVALID_ARG, "the norm's eps must be a finite number >= 0");
+// n norms in a row (norm null: none), before the first launch of the call that takes them.
+int check_norm(oomattn_ctx* ctx, const oomattn_qk_norm* norm, int n = 1) {
+  for (int i = 0; norm && i < n; ++i) {
+    if (!(norm[i].eps >= 0.f && norm[i].eps <= 3.4e38f))
+      return fail(ctx, OOMATTN_ERR_INVALID_ARG, "the norm's eps must be a finite number >= 0");
+    if (!aligned16(norm[i].q) || !aligned16(norm[i].k))
+      return fail(ctx, OOMATTN_ERR_INVALID_ARG, "norm weights must be 16-byte aligned");
+  }
   return OOMATTN_OK;
 }
 
@@ -2729,6 +2733,7 @@ extern "C" int oomattn_decoder_layer_q8_qk_norm(oomattn_ctx* ctx, int32_t layer,
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "decoder_layer_q8 weight shapes do not match the configuration");
   if (!w->input_norm || !w->post_norm) return fail(ctx, OOMATTN_ERR_INVALID_ARG, "null norm weights");
   int rc = check_layer(ctx, layer);
+  if (!rc) rc = check_norm(ctx, norm);
   if (rc) return rc;
   DeviceGuard dg(ctx->device);
   const size_t B = (size_t)n_seqs, inter = (size_t)w->gate.rows;
@@ -2830,6 +2835,8 @@ extern "C" int oomattn_decode_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q8
   const int H = ctx->cfg.hidden_size;
   if (m->embed.cols != H || m->lm_head.cols != H || !m->final_norm)
     return fail(ctx, OOMATTN_ERR_INVALID_ARG, "embedding / LM head width or final norm does not match hidden %d", H);
+  int rc = check_norm(ctx, norms, m->n_layers);
+  if (rc) return rc;
   DeviceGuard dg(ctx->device);
   const size_t B = (size_t)n_seqs, vocab = (size_t)m->lm_head.rows;
   const size_t xf = (B * H + 31) / 32 * 32;
@@ -2850,7 +2857,7 @@ extern "C" int oomattn_decode_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q8
   float* lg = logits ? logits : xb + xf;
   // OomLlamaModel::forward_turbo (src/oomllama.rs:504-553) for one new token per sequence, then the greedy
   // pick of the generation loop (:973-976, :1000-1003)
-  int rc = oomattn_embed_q8(ctx, &m->embed, tokens, n_seqs, xa);
+  rc = oomattn_embed_q8(ctx, &m->embed, tokens, n_seqs, xa);
   if (rc) return rc;
   for (int l = 0; l < m->n_layers; ++l) {
     rc = oomattn_decoder_layer_q8_qk_norm(ctx, l, n_seqs, seq_ids, xa, &m->layers[l], norms ? norms + l : nullptr, xb);
@@ -2891,11 +2898,9 @@ extern "C" int oomattn_prefill_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q
         w->up.rows != w->gate.rows || w->down.rows != H || w->down.cols != w->gate.rows || !w->input_norm ||
         !w->post_norm)
       return fail(ctx, OOMATTN_ERR_INVALID_ARG, "layer %d: weight shapes do not match the configuration", l);
-    if (norms) {
-      const int nrc = check_norm(ctx, norms + l);
-      if (nrc) return nrc;
-    }
   }
+  int rc = check_norm(ctx, norms, m->n_layers);
+  if (rc) return rc;
   DeviceGuard dg(ctx->device);
   const size_t T = (size_t)n_seqs * n_new, B = (size_t)n_seqs, vocab = (size_t)m->lm_head.rows;
   const size_t inter = (size_t)m->layers[0].gate.rows;
@@ -2918,7 +2923,6 @@ extern "C" int oomattn_prefill_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q
   float* xlast = xb + up32(T * H);
   float* lg = logits ? logits : xlast + up32(B * H);
   // layer scratch: q, k, v, rotated q (bf16), attention output, h, gate, up
-  int rc;
   float* sb = layer_scratch(ctx, up32(T * nq) * 3 + up32(T * nkv) * 2 + up32(T * nq / 2) + up32(T * H) +
                                      2 * up32(T * inter) + 64, &rc);
   if (rc) return rc;
