@@ -15,7 +15,8 @@
  *  - Every function returns an oomattn_status (0 = OK).  Nothing aborts or
  *    throws across the ABI; oomattn_last_error() holds the message of the last
  *    failure on a context.  Invalid shapes, indices and positions are rejected
- *    on the host before any GPU work is queued.
+ *    on the host before any GPU work is queued.  A call that returns an error
+ *    leaves the sequences' lengths as they were, in every layer of a model step.
  *  - Device pointers are raw CUDA device addresses owned by the caller;
  *    host pointers are marked "host".  All GPU work is queued on the context's
  *    stream (oomattn_set_stream); nothing synchronises the host except

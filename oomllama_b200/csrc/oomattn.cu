@@ -12,6 +12,8 @@
 #include <string.h>
 
 #include <algorithm>
+#include <memory>
+#include <new>
 #include <string>
 #include <system_error>
 #include <thread>
@@ -547,6 +549,46 @@ void commit_append(oomattn_ctx* ctx, int layer, const SeqBatch& sb, int n_new) {
   for (int z = 0; z < sb.n; ++z) ctx->h_len[(size_t)layer * ctx->cfg.max_seqs + sb.seq[z]] = sb.len[z] + n_new;
 }
 
+// What a step of several calls has appended, layers [first, first + layers): taken back (the host lengths are what
+// they were) where a later call of the step fails, so that a refused step leaves the cache as it found it.
+struct AppendGuard {
+  oomattn_ctx* ctx;
+  int first, layers, n_seqs;
+  const int32_t* seq_ids;
+  int n_new;
+  int done(int rc) {  // the step's own result
+    if (!rc) layers = 0;
+    return rc;
+  }
+  ~AppendGuard() {
+    for (int l = first; l < first + layers; ++l)
+      for (int z = 0; z < n_seqs; ++z) ctx->h_len[(size_t)l * ctx->cfg.max_seqs + seq_ids[z]] -= n_new;
+  }
+};
+
+// An append of more sequences than one launch carries: all of them are looked at before the first launch, since
+// that one's rows may replace others (starts).  A sequence of two launches is appended to twice.
+int check_append(oomattn_ctx* ctx, int layer, int n_seqs, const int32_t* seq_ids, int n_new, const int32_t* starts) {
+  if (n_seqs <= kMaxBatch) return OOMATTN_OK;  // its only launch plans it
+  std::unique_ptr<int[]> was(new (std::nothrow) int[n_seqs]);
+  if (!was) return fail(ctx, OOMATTN_ERR_NO_MEMORY, "no host memory for %d sequences", n_seqs);
+  int* len = ctx->h_len.data() + (size_t)layer * ctx->cfg.max_seqs;
+  int rc = OOMATTN_OK, done = 0;
+  for (int r0 = 0; r0 < n_seqs && !rc; r0 += kMaxBatch) {
+    const int n = std::min(kMaxBatch, n_seqs - r0);
+    SeqBatch sb;
+    rc = plan_append(ctx, layer, n, seq_ids + r0, n_new, sb, starts ? starts + r0 : nullptr);
+    if (rc) break;
+    for (int z = 0; z < n; ++z) was[done++] = len[sb.seq[z]];
+    commit_append(ctx, layer, sb, n_new);
+  }
+  while (done > 0) {
+    --done;
+    len[seq_ids[done]] = was[done];
+  }
+  return rc;
+}
+
 AppendArgs base_append_args(oomattn_ctx* ctx, int layer, int n_new) {
   AppendArgs ap;
   memset(&ap, 0, sizeof(ap));
@@ -677,6 +719,7 @@ int rope_append_impl(oomattn_ctx* ctx, int layer, int n_seqs, const int32_t* seq
   if (!rc) rc = validate_dtype(ctx, in_dtype, "rope_append input");
   if (!rc) rc = validate_dtype(ctx, q_out_dtype, "rope_append q_out");
   if (!rc) rc = check_norm(ctx, norm);
+  if (!rc) rc = check_append(ctx, layer, n_seqs, seq_ids, n_new, starts);
   if (rc) return rc;
   DeviceGuard dg(ctx->device);
   const int in_es = in_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4, out_es = q_out_dtype == OOMATTN_DTYPE_BF16 ? 2 : 4;
@@ -1923,6 +1966,7 @@ int oomattn_attention_forward_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t b
                           norm, use_prefill ? qb16 : (void*)qbuf, use_prefill ? OOMATTN_DTYPE_BF16 : OOMATTN_DTYPE_F32);
   }
   if (rc) return rc;
+  AppendGuard appended{ctx, layer, 1, batch, seqs.data(), seq_len};
   // attention
   if (use_prefill) {
     for (int b = 0; b < batch; ++b) {
@@ -1943,9 +1987,9 @@ int oomattn_attention_forward_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t b
   }
   // o_proj: out = attn . Wo^T   (src/oomllama_turbo.rs:715-720): a GEMV for decode-sized
   // token counts, the tensor-core linear above that
-  if (T <= kGemvMaxT) return f32_gemv(ctx, abuf, wo, (int)T, o_out, qo, nullptr, nullptr, out);
+  if (T <= kGemvMaxT) return appended.done(f32_gemv(ctx, abuf, wo, (int)T, o_out, qo, nullptr, nullptr, out));
   const KfJob oj{wo, 0, o_out, nullptr, nullptr, out};
-  return kf_linear_f32(ctx, abuf, (int)T, qo, &oj, 1);
+  return appended.done(kf_linear_f32(ctx, abuf, (int)T, qo, &oj, 1));
 }
 
 }  // extern "C"
@@ -2762,6 +2806,7 @@ extern "C" int oomattn_decoder_layer_q8_qk_norm(oomattn_ctx* ctx, int32_t layer,
   rc = rope_append_impl(ctx, layer, n_seqs, seq_ids, nullptr, 1, q, k, v, OOMATTN_DTYPE_F32, nullptr, nullptr, nullptr,
                         norm, qr, OOMATTN_DTYPE_F32);
   if (rc) return rc;
+  AppendGuard appended{ctx, layer, 1, n_seqs, seq_ids, 1};
   rc = oomattn_decode(ctx, layer, n_seqs, seq_ids, nullptr, qr, att, nullptr);
   if (rc) return rc;
   const Q8Job o{&w->o, nullptr, x, h};
@@ -2771,7 +2816,7 @@ extern "C" int oomattn_decoder_layer_q8_qk_norm(oomattn_ctx* ctx, int32_t layer,
   rc = q8_run(ctx, gu, 2, h, nullptr, n_seqs, w->post_norm, w->eps);
   if (rc) return rc;
   const Q8Job dn{&w->down, nullptr, h, out};
-  return q8_run(ctx, &dn, 1, g, u, n_seqs);
+  return appended.done(q8_run(ctx, &dn, 1, g, u, n_seqs));
 }
 
 extern "C" int oomattn_embed_q8(oomattn_ctx* ctx, const oomattn_q8_matrix* emb, const int32_t* token_ids,
@@ -2859,15 +2904,17 @@ extern "C" int oomattn_decode_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q8
   // pick of the generation loop (:973-976, :1000-1003)
   rc = oomattn_embed_q8(ctx, &m->embed, tokens, n_seqs, xa);
   if (rc) return rc;
+  AppendGuard appended{ctx, 0, 0, n_seqs, seq_ids, 1};
   for (int l = 0; l < m->n_layers; ++l) {
     rc = oomattn_decoder_layer_q8_qk_norm(ctx, l, n_seqs, seq_ids, xa, &m->layers[l], norms ? norms + l : nullptr, xb);
     if (rc) return rc;
+    appended.layers = l + 1;
     std::swap(xa, xb);
   }
   const Q8Job head{&m->lm_head, nullptr, nullptr, lg};
   rc = q8_run(ctx, &head, 1, xa, nullptr, n_seqs, m->final_norm, m->eps);
   if (rc) return rc;
-  return oomattn_argmax(ctx, lg, n_seqs, (int)vocab, next);
+  return appended.done(oomattn_argmax(ctx, lg, n_seqs, (int)vocab, next));
 }
 
 extern "C" int oomattn_prefill_step_q8(oomattn_ctx* ctx, const oomattn_q8_model* m, int32_t n_seqs,
@@ -2944,6 +2991,7 @@ extern "C" int oomattn_prefill_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q
   // last token's logits give the first greedy pick (src/oomllama.rs:969-976)
   rc = oomattn_embed_q8(ctx, &m->embed, tokens, (int32_t)T, xa);
   if (rc) return rc;
+  AppendGuard appended{ctx, 0, 0, n_seqs, seq_ids, n_new};
   for (int l = 0; l < m->n_layers; ++l) {
     const oomattn_q8_layer* w = &m->layers[l];
     const Q8Job qkv[3] = {{&w->q, w->bq, nullptr, q}, {&w->k, w->bk, nullptr, k}, {&w->v, w->bv, nullptr, v}};
@@ -2952,6 +3000,7 @@ extern "C" int oomattn_prefill_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q
     rc = rope_append_impl(ctx, l, n_seqs, seq_ids, nullptr, n_new, q, k, v, OOMATTN_DTYPE_F32, nullptr, nullptr,
                           nullptr, norms ? norms + l : nullptr, qr, OOMATTN_DTYPE_BF16);
     if (rc) return rc;
+    appended.layers = l + 1;
     for (int b = 0; b < n_seqs; ++b) {
       rc = oomattn_prefill(ctx, l, seq_ids[b], n_new, qr + (size_t)b * n_new * nq, att + (size_t)b * n_new * nq,
                            OOMATTN_DTYPE_F32, nullptr);
@@ -2974,7 +3023,7 @@ extern "C" int oomattn_prefill_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q
   const Q8Job head{&m->lm_head, nullptr, nullptr, lg};
   rc = q8_run(ctx, &head, 1, xlast, nullptr, n_seqs, m->final_norm, m->eps);
   if (rc) return rc;
-  return oomattn_argmax(ctx, lg, n_seqs, (int)vocab, next);
+  return appended.done(oomattn_argmax(ctx, lg, n_seqs, (int)vocab, next));
 }
 
 // ------------------------------------------------------------------ .oom files
