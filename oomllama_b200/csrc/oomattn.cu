@@ -131,15 +131,16 @@ struct oomattn_ctx {
   uint8_t* d_kf = nullptr;
   size_t kf_bytes = 0;
   // key-split prefill: the chunks' partial O and lse
-  uint8_t* d_pf_part = nullptr;
+  void* d_pf_part = nullptr;
   size_t pf_part_bytes = 0;
-  // scratch blocks that a larger one replaced: captured graphs may still name them
+  // scratch that grew while captured graphs may name the old block (see grow_block)
+  bool graphs = false;  // a call that uses scratch has been captured
   void* kept[96] = {};
   int n_kept = 0;
   // prefill over a 4-bit cache: one sequence's rows of one layer in fp16,
-  // [n_kv][16 exp_pages][128] of K, then of V
-  uint8_t* d_exp = nullptr;
-  int exp_pages = 0;
+  // [n_kv][16 pages][128] of K, then of V
+  void* d_exp = nullptr;
+  size_t exp_bytes = 0;
   PrefillPlan plan{1, 0};  // of the last such prefill: plan_n queries, plan_len tokens
   int plan_n = 0, plan_len = 0;
   // Q8 linear: activation splits and split-K partials, and per-row-tile
@@ -338,36 +339,57 @@ int validate_dtype(oomattn_ctx* ctx, int dt, const char* what) {
   return OOMATTN_OK;
 }
 
-// A larger block in place of *p (null: the first).  The old one stays until the
-// context is destroyed, since a captured graph may name it; each is half as large
-// again as what was asked for, so that few are kept.  Not during a capture: the
-// block would be new to the graph alone.
-int grow_block(oomattn_ctx* ctx, void** p, size_t bytes, const char* what) {
+// Whether the context's stream is being captured; remembered, since the graph will name the scratch of that time.
+int note_capture(oomattn_ctx* ctx, bool* capturing) {
   cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-  CK(cudaStreamIsCapturing(ctx->stream, &st));
-  if (st != cudaStreamCaptureStatusNone)
-    return fail(ctx, OOMATTN_ERR_UNSUPPORTED, "%s has to grow: run a call of this size once before the capture", what);
-  if (*p && ctx->n_kept == (int)(sizeof(ctx->kept) / sizeof(ctx->kept[0])))
-    return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "%s has grown too often", what);
-  void* q = nullptr;
-  if (cudaMalloc(&q, bytes) != cudaSuccess) {
+  const cudaError_t e = cudaStreamIsCapturing(ctx->stream, &st);
+  if (e != cudaSuccess) {
     cudaGetLastError();
-    return fail(ctx, OOMATTN_ERR_NO_MEMORY, "%s of %zu bytes failed", what, bytes);
+    return fail(ctx, OOMATTN_ERR_CUDA, "cudaStreamIsCapturing: %s", cudaGetErrorString(e));
   }
-  if (*p) ctx->kept[ctx->n_kept++] = *p;
-  *p = q;
+  *capturing = st != cudaStreamCaptureStatusNone;
+  ctx->graphs |= *capturing;
   return OOMATTN_OK;
 }
 
-int ensure_scratch(oomattn_ctx* ctx, size_t bytes) {
-  if (bytes <= ctx->scratch_bytes) return OOMATTN_OK;
-  const size_t want = ctx->d_scratch ? bytes + bytes / 2 : bytes;
-  void* p = ctx->d_scratch;
-  const int rc = grow_block(ctx, &p, want, "the scratch");
+// *p, of *have bytes, made to hold `need` bytes; called by every user of the block.  One that is too small is freed
+// for a larger one, but where a graph may name it, it stays until the context is destroyed; then, and where the caller
+// says that it grows step by step (ahead), the new block is half as large again where the memory is there, so that few
+// are made.  Not during a capture: the block would be new to the graph alone.
+int grow_block(oomattn_ctx* ctx, void** p, size_t* have, size_t need, const char* what, bool ahead = false) {
+  bool capturing;
+  const int rc = note_capture(ctx, &capturing);
   if (rc) return rc;
+  if (need <= *have) return OOMATTN_OK;
+  if (capturing)
+    return fail(ctx, OOMATTN_ERR_UNSUPPORTED, "%s has to grow: run a call of this size once before the capture", what);
+  const bool more = *p && (ahead || ctx->graphs);
+  if (*p && !ctx->graphs) {
+    cudaStreamSynchronize(ctx->stream);
+    cudaFree(*p);
+    *p = nullptr;
+    *have = 0;
+  }
+  if (*p && ctx->n_kept == (int)(sizeof(ctx->kept) / sizeof(ctx->kept[0])))
+    return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "%s has grown too often", what);
+  void* q = nullptr;
+  for (const size_t bytes : {more ? need + need / 2 : need, need}) {
+    if (cudaMalloc(&q, bytes) == cudaSuccess) {
+      if (*p) ctx->kept[ctx->n_kept++] = *p;
+      *p = q;
+      *have = bytes;
+      return OOMATTN_OK;
+    }
+    cudaGetLastError();
+  }
+  return fail(ctx, OOMATTN_ERR_NO_MEMORY, "%s of %zu bytes failed", what, need);
+}
+
+int ensure_scratch(oomattn_ctx* ctx, size_t bytes) {
+  void* p = ctx->d_scratch;
+  const int rc = grow_block(ctx, &p, &ctx->scratch_bytes, bytes, "the scratch");
   ctx->d_scratch = static_cast<float*>(p);
-  ctx->scratch_bytes = want;
-  return OOMATTN_OK;
+  return rc;
 }
 
 // ------------------------------------------------------------------ K-F host side
@@ -1086,35 +1108,32 @@ int project(oomattn_ctx* ctx, const float* x, int T, int k, const KfJob* jobs, i
 int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtensorMap* kmap, CUtensorMap* vmap) {
   const int n_kv = ctx->cfg.n_kv_heads;
   const int pages = ((L + kPageSize - 1) / kPageSize + 7) / 8 * 8;  // the prefill's 128-key tiles: zeros past L
-  const size_t page_bytes = (size_t)n_kv * kPageSize * kHeadDim * 2;
-  if (pages > ctx->exp_pages) {
-    const int cap = pages + pages / 2;  // a growing sequence does not reallocate at every chunk
-    if ((long long)cap * n_kv * kPageSize >= (1ll << 31))
-      return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "prefill over %d tokens of a 4-bit cache", L);
-    void* p = ctx->d_exp;
-    const int rc = grow_block(ctx, &p, 2 * (size_t)cap * page_bytes, "the prefill's scratch");
-    if (rc) return rc;
-    ctx->d_exp = static_cast<uint8_t*>(p);
-    ctx->exp_pages = cap;
-  }
-  uint8_t* v_rows = ctx->d_exp + (size_t)ctx->exp_pages * page_bytes;
+  const size_t page_bytes = (size_t)n_kv * kPageSize * kHeadDim * 2;  // of K, or of V
+  const int most = ((1ll << 31) - 1) / ((long long)n_kv * kPageSize);  // 32-bit rows
+  if (pages > most) return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "prefill over %d tokens of a 4-bit cache", L);
+  // ahead: a growing sequence does not allocate at every chunk
+  int rc = grow_block(ctx, &ctx->d_exp, &ctx->exp_bytes, 2 * (size_t)pages * page_bytes, "the prefill's scratch", true);
+  if (rc) return rc;
+  const int cap = (int)std::min<size_t>(most, ctx->exp_bytes / (2 * page_bytes));
+  uint8_t* k_rows = static_cast<uint8_t*>(ctx->d_exp);
+  uint8_t* v_rows = k_rows + (size_t)cap * page_bytes;
   SeqBatch sb;
   sb.n = 1;
   sb.seq[0] = seq;
   sb.len[0] = 0;
   sb.pos[0] = 0;
   GatherArgs a;
-  a.k_out = ctx->d_exp;
+  a.k_out = k_rows;
   a.v_out = v_rows;
   a.layer = layer;
   a.n = L;
   a.pages = pages;
-  a.head_rows = ctx->exp_pages * kPageSize;
+  a.head_rows = cap * kPageSize;
   a.status = ctx->d_status;
-  int rc = launch_gather(ctx, a, sb, kOutF16);
-  if (!rc) rc = encode_pool_map(ctx, ctx->d_exp, ctx->exp_pages, kmap, 128);
-  if (!rc) rc = encode_pool_map(ctx, v_rows, ctx->exp_pages, vmap, 128);
-  pool->n_pool_pages = ctx->exp_pages;  // per kv head
+  rc = launch_gather(ctx, a, sb, kOutF16);
+  if (!rc) rc = encode_pool_map(ctx, k_rows, cap, kmap, 128);
+  if (!rc) rc = encode_pool_map(ctx, v_rows, cap, vmap, 128);
+  pool->n_pool_pages = cap;  // per kv head
   return rc;
 }
 
@@ -1315,10 +1334,9 @@ int oomattn_destroy(oomattn_ctx* ctx) {
   void* ptrs[] = {ctx->kpool,     ctx->vpool,      ctx->d_block_table, ctx->d_cos,    ctx->d_sin,
                   ctx->d_part_o,  ctx->d_part_lse, ctx->d_counters,    ctx->d_status, ctx->d_scratch,
                   ctx->d_q8_scratch, ctx->d_q8_counters, ctx->d_layer_scratch, ctx->d_model_scratch,
-                  ctx->d_argmax_part, ctx->d_kf, ctx->d_pf_part};
+                  ctx->d_argmax_part, ctx->d_kf, ctx->d_pf_part, ctx->d_exp};
   for (void* p : ptrs)
     if (p) cudaFree(p);
-  if (ctx->d_exp) cudaFree(ctx->d_exp);
   for (int i = 0; i < ctx->n_kept; ++i) cudaFree(ctx->kept[i]);
   delete ctx;
   return OOMATTN_OK;
@@ -1829,16 +1847,10 @@ static int prefill_impl(oomattn_ctx* ctx, int32_t layer, int32_t seq, int32_t n_
   if (n_chunks > 1) {
     const size_t rows_all = (size_t)n_chunks * a.n_pad;
     const size_t ob = rows_all * ctx->cfg.n_heads * kHeadDim * 4, lb = rows_all * ctx->cfg.n_heads * 4;
-    if (ob + lb > ctx->pf_part_bytes) {
-      const size_t want = ctx->d_pf_part ? (ob + lb) + (ob + lb) / 2 : ob + lb;
-      void* p = ctx->d_pf_part;
-      rc = grow_block(ctx, &p, want, "the prefill's partials");
-      if (rc) return rc;
-      ctx->d_pf_part = static_cast<uint8_t*>(p);
-      ctx->pf_part_bytes = want;
-    }
-    part_o = reinterpret_cast<float*>(ctx->d_pf_part);
-    a.part_lse = reinterpret_cast<float*>(ctx->d_pf_part + ob);
+    rc = grow_block(ctx, &ctx->d_pf_part, &ctx->pf_part_bytes, ob + lb, "the prefill's partials");
+    if (rc) return rc;
+    part_o = static_cast<float*>(ctx->d_pf_part);
+    a.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(ctx->d_pf_part) + ob);
     rc = encode_out_map(ctx, part_o, (int)rows_all, false, pack, &pmap);
     if (rc) return rc;
   }
