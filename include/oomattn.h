@@ -22,11 +22,11 @@
  *    stream (oomattn_set_stream); nothing synchronises the host except
  *    oomattn_sync and oomattn_kv_read.
  *  - Calls may be captured into CUDA graphs once the same calls have run (their
- *    scratch is allocated by the first one of a size; attention and prefill
- *    refuse a capture in which it would grow).  Graphs of one context share its
- *    scratch: they do not run at the same time as one another, nor as the
- *    context's other calls.  Where a linear, MLP, layer or model step later needs
- *    more scratch than any before it, capture its earlier graphs again.
+ *    scratch is allocated by the first one of a size; a capture in which it would
+ *    grow is refused).  Scratch that a captured call used stays for its graph when
+ *    a later call needs more, until the context is destroyed.  Graphs of one
+ *    context share its scratch: they do not run at the same time as one another,
+ *    nor as the context's other calls.
  *  - A context owns the paged K/V pools of all layers, the block tables, the
  *    RoPE table and the split-KV scratch.  One context per device per host
  *    thread; calls on one context are not thread-safe (the reference engine

@@ -128,7 +128,7 @@ struct oomattn_ctx {
   float* d_scratch = nullptr;
   size_t scratch_bytes = 0;
   // K-F (tensor-core linear): the split / converted operand planes
-  uint8_t* d_kf = nullptr;
+  void* d_kf = nullptr;
   size_t kf_bytes = 0;
   // key-split prefill: the chunks' partial O and lse
   void* d_pf_part = nullptr;
@@ -145,15 +145,17 @@ struct oomattn_ctx {
   int plan_n = 0, plan_len = 0;
   // Q8 linear: activation splits and split-K partials, and per-row-tile
   // arrival counters (zero between launches)
-  uint8_t* d_q8_scratch = nullptr;
+  void* d_q8_scratch = nullptr;
   size_t q8_scratch_bytes = 0;
-  unsigned* d_q8_counters = nullptr;
-  int q8_counters_n = 0;
+  void* d_q8_counters = nullptr;
+  size_t q8_counter_bytes = 0;
+  struct { void* p; size_t bytes; } kept_counters[16] = {};  // of those, the blocks that a failed wait clears
+  int n_kept_counters = 0;
   // decoder-layer step: normalised activations, projections, MLP intermediates
-  float* d_layer_scratch = nullptr;
+  void* d_layer_scratch = nullptr;
   size_t layer_scratch_bytes = 0;
   // model step: the residual stream between layers and the logits
-  float* d_model_scratch = nullptr;
+  void* d_model_scratch = nullptr;
   size_t model_scratch_bytes = 0;
   // argmax: per-(row, chunk) (value, index) partials
   void* d_argmax_part = nullptr;
@@ -411,21 +413,8 @@ int encode_2d(oomattn_ctx* ctx, const void* base, CUtensorMapDataType dt, int es
 }
 
 uint8_t* kf_scratch(oomattn_ctx* ctx, size_t bytes, int* rc) {
-  *rc = OOMATTN_OK;
-  if (bytes > ctx->kf_bytes) {
-    if (ctx->d_kf) {
-      cudaStreamSynchronize(ctx->stream);
-      cudaFree(ctx->d_kf);
-      ctx->d_kf = nullptr;
-      ctx->kf_bytes = 0;
-    }
-    if (cudaMalloc(&ctx->d_kf, bytes) != cudaSuccess) {
-      *rc = fail(ctx, OOMATTN_ERR_NO_MEMORY, "linear operand scratch of %zu bytes failed", bytes);
-      return nullptr;
-    }
-    ctx->kf_bytes = bytes;
-  }
-  return ctx->d_kf;
+  *rc = grow_block(ctx, &ctx->d_kf, &ctx->kf_bytes, bytes, "linear operand scratch");
+  return static_cast<uint8_t*>(ctx->d_kf);
 }
 
 size_t align256(size_t b) { return (b + 255) & ~size_t(255); }
@@ -1357,7 +1346,8 @@ int oomattn_sync(oomattn_ctx* ctx) {
   if (st) {
     CK(cudaMemset(ctx->d_status, 0, sizeof(int)));
     // a linear that gave up on a wait may have left cut-tile arrivals behind
-    if (ctx->d_q8_counters) CK(cudaMemset(ctx->d_q8_counters, 0, sizeof(unsigned) * ctx->q8_counters_n));
+    if (ctx->d_q8_counters) CK(cudaMemset(ctx->d_q8_counters, 0, ctx->q8_counter_bytes));
+    for (int i = 0; i < ctx->n_kept_counters; ++i) CK(cudaMemset(ctx->kept_counters[i].p, 0, ctx->kept_counters[i].bytes));
     if (st & kDevErrTimeout) return fail(ctx, OOMATTN_ERR_TIMEOUT, "a device-side wait timed out (status %d)", st);
     if (st & kDevErrRange)
       return fail(ctx, OOMATTN_ERR_DEVICE_CHECK,
@@ -2276,29 +2266,16 @@ extern "C" int oomattn_q8_unpack(const uint8_t* stream, uint64_t stream_bytes, i
 namespace {
 
 int ensure_q8_scratch(oomattn_ctx* ctx, size_t bytes, int row_tiles) {
-  if (bytes > ctx->q8_scratch_bytes) {
-    if (ctx->d_q8_scratch) {
-      cudaStreamSynchronize(ctx->stream);
-      cudaFree(ctx->d_q8_scratch);
-      ctx->d_q8_scratch = nullptr;
-      ctx->q8_scratch_bytes = 0;
-    }
-    if (cudaMalloc(&ctx->d_q8_scratch, bytes) != cudaSuccess)
-      return fail(ctx, OOMATTN_ERR_NO_MEMORY, "q8 scratch allocation of %zu bytes failed", bytes);
-    ctx->q8_scratch_bytes = bytes;
-  }
-  if (row_tiles > ctx->q8_counters_n) {
-    if (ctx->d_q8_counters) {
-      cudaStreamSynchronize(ctx->stream);
-      cudaFree(ctx->d_q8_counters);
-      ctx->d_q8_counters = nullptr;
-      ctx->q8_counters_n = 0;
-    }
-    if (cudaMalloc(&ctx->d_q8_counters, sizeof(unsigned) * row_tiles) != cudaSuccess)
-      return fail(ctx, OOMATTN_ERR_NO_MEMORY, "q8 counter allocation failed");
-    CK(cudaMemsetAsync(ctx->d_q8_counters, 0, sizeof(unsigned) * row_tiles, ctx->stream));
-    ctx->q8_counters_n = row_tiles;
-  }
+  int rc = grow_block(ctx, &ctx->d_q8_scratch, &ctx->q8_scratch_bytes, bytes, "q8 scratch");
+  if (rc) return rc;
+  void* const old = ctx->d_q8_counters;
+  const size_t old_bytes = ctx->q8_counter_bytes, need = sizeof(unsigned) * row_tiles;
+  if (need > old_bytes && ctx->graphs && ctx->n_kept_counters == 16)
+    return fail(ctx, OOMATTN_ERR_OUT_OF_RANGE, "q8 counters have grown too often");
+  rc = grow_block(ctx, &ctx->d_q8_counters, &ctx->q8_counter_bytes, need, "q8 counters");
+  if (rc || ctx->q8_counter_bytes == old_bytes) return rc;
+  if (old && ctx->graphs) ctx->kept_counters[ctx->n_kept_counters++] = {old, old_bytes};
+  CK(cudaMemsetAsync(ctx->d_q8_counters, 0, ctx->q8_counter_bytes, ctx->stream));
   return OOMATTN_OK;
 }
 
@@ -2477,7 +2454,7 @@ int launch_q8_tc(oomattn_ctx* ctx, const Q8Job* jobs, int n_jobs, int cols, int 
   a.n_tokens = nt;
   a.units = p.units;
   a.part = part;
-  a.counters = ctx->d_q8_counters;
+  a.counters = static_cast<unsigned*>(ctx->d_q8_counters);
   a.status = ctx->d_status;
   a.timeout_ns = ctx->timeout_ns;
   a.test_flags = ctx->test_flags;
@@ -2617,7 +2594,7 @@ int q8_run(oomattn_ctx* ctx, const Q8Job* jobs, int n_jobs, const float* x, cons
                        part_floats * 4 + 256;
   int rc = ensure_q8_scratch(ctx, bytes, max_blocks);
   if (rc) return rc;
-  uint32_t* xh = reinterpret_cast<uint32_t*>(ctx->d_q8_scratch);
+  uint32_t* xh = static_cast<uint32_t*>(ctx->d_q8_scratch);
   uint32_t* xl = xh + xw;
   float* xsum = reinterpret_cast<float*>(xl + xw);
   float* sx = xsum + (size_t)group * nchunks;  // [16][cols / 256], the integer form's digit scales
@@ -2664,7 +2641,7 @@ int q8_run(oomattn_ctx* ctx, const Q8Job* jobs, int n_jobs, const float* x, cons
     a.xl = xl;
     a.xsum = xsum;
     a.n_tokens = nt;
-    a.counters = ctx->d_q8_counters;
+    a.counters = static_cast<unsigned*>(ctx->d_q8_counters);
     a.splits = xp.splits;
     a.chunks_per_split = xp.cps;
     a.status = ctx->d_status;
@@ -2703,21 +2680,8 @@ int q8_run(oomattn_ctx* ctx, const Q8Job* jobs, int n_jobs, const float* x, cons
 
 // Per-context buffers of the layer step (grown on demand).
 float* layer_scratch(oomattn_ctx* ctx, size_t floats, int* rc) {
-  if (floats * 4 > ctx->layer_scratch_bytes) {
-    if (ctx->d_layer_scratch) {
-      cudaStreamSynchronize(ctx->stream);
-      cudaFree(ctx->d_layer_scratch);
-      ctx->d_layer_scratch = nullptr;
-      ctx->layer_scratch_bytes = 0;
-    }
-    if (cudaMalloc(&ctx->d_layer_scratch, floats * 4) != cudaSuccess) {
-      *rc = fail(ctx, OOMATTN_ERR_NO_MEMORY, "layer scratch allocation of %zu bytes failed", floats * 4);
-      return nullptr;
-    }
-    ctx->layer_scratch_bytes = floats * 4;
-  }
-  *rc = OOMATTN_OK;
-  return ctx->d_layer_scratch;
+  *rc = grow_block(ctx, &ctx->d_layer_scratch, &ctx->layer_scratch_bytes, floats * 4, "layer scratch");
+  return static_cast<float*>(ctx->d_layer_scratch);
 }
 
 int run_rmsnorm(oomattn_ctx* ctx, const float* x, const float* w, float eps, int n_tokens, int hidden, float* out) {
@@ -2856,17 +2820,8 @@ extern "C" int oomattn_argmax(oomattn_ctx* ctx, const float* logits, int32_t n_r
   const int chunk = (n + chunks - 1) / chunks;
   const int n_chunks = (n + chunk - 1) / chunk;
   const size_t need = (size_t)n_rows * n_chunks * 8;
-  if (need > ctx->argmax_part_bytes) {
-    if (ctx->d_argmax_part) {
-      cudaStreamSynchronize(ctx->stream);
-      cudaFree(ctx->d_argmax_part);
-      ctx->d_argmax_part = nullptr;
-      ctx->argmax_part_bytes = 0;
-    }
-    if (cudaMalloc(&ctx->d_argmax_part, need) != cudaSuccess)
-      return fail(ctx, OOMATTN_ERR_NO_MEMORY, "argmax scratch allocation of %zu bytes failed", need);
-    ctx->argmax_part_bytes = need;
-  }
+  const int rc = grow_block(ctx, &ctx->d_argmax_part, &ctx->argmax_part_bytes, need, "argmax scratch");
+  if (rc) return rc;
   float* pv = static_cast<float*>(ctx->d_argmax_part);
   int* pi = reinterpret_cast<int*>(pv + (size_t)n_rows * n_chunks);
   argmax_partial_kernel<<<dim3(n_chunks, n_rows), kArgmaxThreads, 0, ctx->stream>>>(logits, n, chunk, pv, pi);
@@ -2898,18 +2853,9 @@ extern "C" int oomattn_decode_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q8
   const size_t B = (size_t)n_seqs, vocab = (size_t)m->lm_head.rows;
   const size_t xf = (B * H + 31) / 32 * 32;
   const size_t need = (2 * xf + (logits ? 0 : B * vocab) + 64) * 4;
-  if (need > ctx->model_scratch_bytes) {
-    if (ctx->d_model_scratch) {
-      cudaStreamSynchronize(ctx->stream);
-      cudaFree(ctx->d_model_scratch);
-      ctx->d_model_scratch = nullptr;
-      ctx->model_scratch_bytes = 0;
-    }
-    if (cudaMalloc(&ctx->d_model_scratch, need) != cudaSuccess)
-      return fail(ctx, OOMATTN_ERR_NO_MEMORY, "model scratch allocation of %zu bytes failed", need);
-    ctx->model_scratch_bytes = need;
-  }
-  float* xa = ctx->d_model_scratch;
+  rc = grow_block(ctx, &ctx->d_model_scratch, &ctx->model_scratch_bytes, need, "model scratch");
+  if (rc) return rc;
+  float* xa = static_cast<float*>(ctx->d_model_scratch);
   float* xb = xa + xf;
   float* lg = logits ? logits : xb + xf;
   // OomLlamaModel::forward_turbo (src/oomllama.rs:504-553) for one new token per sequence, then the greedy
@@ -2966,18 +2912,9 @@ extern "C" int oomattn_prefill_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q
   auto up32 = [](size_t n) { return (n + 31) / 32 * 32; };  // 128-byte aligned pieces
   // model scratch: the residual stream (two buffers), the last token of each sequence, the logits
   const size_t need_m = (2 * up32(T * H) + up32(B * H) + (logits ? 0 : up32(B * vocab)) + 64) * 4;
-  if (need_m > ctx->model_scratch_bytes) {
-    if (ctx->d_model_scratch) {
-      cudaStreamSynchronize(ctx->stream);
-      cudaFree(ctx->d_model_scratch);
-      ctx->d_model_scratch = nullptr;
-      ctx->model_scratch_bytes = 0;
-    }
-    if (cudaMalloc(&ctx->d_model_scratch, need_m) != cudaSuccess)
-      return fail(ctx, OOMATTN_ERR_NO_MEMORY, "model scratch allocation of %zu bytes failed", need_m);
-    ctx->model_scratch_bytes = need_m;
-  }
-  float* xa = ctx->d_model_scratch;
+  rc = grow_block(ctx, &ctx->d_model_scratch, &ctx->model_scratch_bytes, need_m, "model scratch");
+  if (rc) return rc;
+  float* xa = static_cast<float*>(ctx->d_model_scratch);
   float* xb = xa + up32(T * H);
   float* xlast = xb + up32(T * H);
   float* lg = logits ? logits : xlast + up32(B * H);

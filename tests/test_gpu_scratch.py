@@ -55,3 +55,77 @@ def test_growth_with_little_memory_left():
         torch.cuda.empty_cache()
     assert (out == 0).all()  # of a cache that holds zeros
     eng.close()
+
+
+def _captured(f):
+    f()  # the scratch of this size
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        f()
+    return graph
+
+
+def test_graphs_outlive_larger_calls(oracle):
+    """A linear, a Q8 linear, an argmax, an MLP and a decode step in graphs; then each kind of scratch grows; the replays
+    give what they gave."""
+    from test_gpu_model_q8 import _model
+    model, _ = _model(oracle, 2, 4, 2, 512, 320, 5)
+    eng = make_engine(4, 2, [64, 400, 400], kv_dtype="bf16", hidden=512, n_layers=2)
+    x, w = randn((40, 512), 1).cuda(), randn((256, 512), 2).cuda()
+    lay = model.layers[0]
+    outs = {"linear": torch.empty(40, 256, device="cuda"), "q8": torch.empty(5, lay.gate.rows, device="cuda"),
+            "mlp": torch.empty(3, 512, device="cuda"), "logits": torch.empty(1, 320, device="cuda")}
+    tokens = torch.tensor([7], dtype=torch.int32, device="cuda")
+    nxt = torch.empty(1, dtype=torch.int32, device="cuda")
+
+    def step():
+        for layer in range(2):
+            eng.set_seq_len(layer, 0, 20)
+        eng.decode_step_q8(model, [0], tokens, next_tokens=nxt, logits=outs["logits"])
+
+    calls = [lambda: eng.linear(x, w, out=outs["linear"]), lambda: eng.q8_linear(lay.gate, x[:5], out=outs["q8"]),
+             lambda: eng.q8_mlp(lay.gate, lay.up, lay.down, x[:3], out=outs["mlp"]), step]
+    graphs = [_captured(f) for f in calls]
+    eng.sync()
+    first = {k: t.clone() for k, t in outs.items()}
+    # larger ones of every kind
+    big = randn((700, 512), 3).cuda()
+    eng.linear(big, w)
+    eng.q8_linear(lay.gate, big)
+    eng.q8_linear(lay.gate, big[:16])
+    eng.q8_mlp(lay.gate, lay.up, lay.down, big)
+    eng.prefill_step_q8(model, [1, 2], torch.ones(2, 300, dtype=torch.int32, device="cuda"))
+    eng.decode_step_q8(model, [1, 2], torch.ones(2, dtype=torch.int32, device="cuda"))
+    fill = torch.full((64 << 20,), 0xFF, dtype=torch.uint8, device="cuda")  # what freed blocks would have become
+    for t in outs.values():
+        t.fill_(-1)
+    for g in graphs:
+        g.replay()
+    eng.sync()
+    for k, t in outs.items():
+        assert torch.equal(t, first[k]), k
+    del fill, graphs
+    eng.close()
+
+
+def test_a_capture_that_would_grow_is_refused(oracle):
+    from test_gpu_model_q8 import _model
+    from oomllama_b200._lib import OomAttnError
+    model, _ = _model(oracle, 1, 4, 2, 512, 320, 5)
+    eng = make_engine(4, 2, [64], kv_dtype="bf16", hidden=512)
+    lay, x, w = model.layers[0], randn((100, 512), 1).cuda(), randn((64, 512), 2).cuda()
+    graph = torch.cuda.CUDAGraph()
+    y = torch.zeros(4, device="cuda")
+    with torch.cuda.graph(graph):
+        for f in (lambda: eng.linear(x, w), lambda: eng.q8_linear(lay.gate, x[:2]),
+                  lambda: eng.q8_mlp(lay.gate, lay.up, lay.down, x), lambda: eng.argmax(x)):
+            with pytest.raises(OomAttnError) as e:
+                f()
+            assert e.value.code == 8
+        y.add_(1)
+    graph.replay()
+    eng.q8_linear(lay.gate, x[:2])
+    eng.sync()
+    assert (y == 1).all()
+    eng.close()
