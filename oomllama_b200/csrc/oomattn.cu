@@ -2908,7 +2908,8 @@ extern "C" int oomattn_prefill_step_q8_qk_norm(oomattn_ctx* ctx, const oomattn_q
   if (rc) return rc;
   DeviceGuard dg(ctx->device);
   const size_t T = (size_t)n_seqs * n_new, B = (size_t)n_seqs, vocab = (size_t)m->lm_head.rows;
-  const size_t inter = (size_t)m->layers[0].gate.rows;
+  size_t inter = 0;  // of the widest MLP
+  for (int l = 0; l < m->n_layers; ++l) inter = std::max(inter, (size_t)m->layers[l].gate.rows);
   auto up32 = [](size_t n) { return (n + 31) / 32 * 32; };  // 128-byte aligned pieces
   // model scratch: the residual stream (two buffers), the last token of each sequence, the logits
   const size_t need_m = (2 * up32(T * H) + up32(B * H) + (logits ? 0 : up32(B * vocab)) + 64) * 4;
