@@ -732,11 +732,12 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         const int tok = F16 ? rr / a.pack : rr, hr = F16 ? h + rr - tok * a.pack : h;
         const int row_in_chunk = q0 + tpt * i + tok;
         const bool valid = tok < (i ? rows_valid[1] : rows_valid[0]);
+        // a NaN key's row has l = NaN, and so its lse
+        const float lse = l == 0.f ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
         if (valid && split_pair)
-          a.part_lse[((size_t)blockIdx.y * a.n_pad + row_in_chunk) * a.n_heads + hr] =
-              (l > 0.f ? (m_used + log2f(l)) * 0.69314718055994531f : -INFINITY);
+          a.part_lse[((size_t)blockIdx.y * a.n_pad + row_in_chunk) * a.n_heads + hr] = lse;
         else if (valid && a.lse)
-          a.lse[(size_t)row_in_chunk * a.n_heads + hr] = (l > 0.f ? (m_used + log2f(l)) * 0.69314718055994531f : -INFINITY);
+          a.lse[(size_t)row_in_chunk * a.n_heads + hr] = lse;
       }
     }
   }

@@ -79,3 +79,21 @@ def test_scale_on_a_border():
     np.testing.assert_array_equal(vg.cpu().numpy(), _held(v).numpy())
     assert ((kg.cpu().double() - k.double()).abs() <= q4_ref.code_bound(k)).all()
     eng.close()
+
+
+@pytest.mark.parametrize("kv_dtype", ["q4", "bf16"])
+@pytest.mark.parametrize("n_new,prefix", [(20, 0), (100, 100), (64, 4000)])
+def test_prefill_nan_key(n_new, prefix, kv_dtype):
+    """A NaN of K reaches the queries that see its token, in out and lse both, and no other."""
+    n, at = n_new + prefix, prefix + n_new // 2
+    k, v = randn((n, 2, 128), 1), randn((n, 2, 128), 2)
+    k[at, 1, 100] = math.nan
+    eng = make_engine(8, 2, [n], kv_dtype=kv_dtype)
+    eng.kv_write(0, 0, k.cuda(), v.cuda())
+    q = randn((n_new, 8, 128), 3, torch.bfloat16)
+    out, lse = eng.prefill(0, 0, q.cuda(), with_lse=True)
+    eng.sync()
+    sees = torch.arange(n_new) >= n_new // 2
+    for x in (out.cpu().isnan().all(-1), out.cpu().isnan().any(-1), lse.cpu().isnan()):
+        assert not x[:, :4].any() and torch.equal(x[:, 4:], sees[:, None].expand(-1, 4))
+    eng.close()
