@@ -40,6 +40,14 @@ constexpr int kPfVStages = 2;                     // V ring: a stage frees once 
 constexpr int kTileBytes = 128 * kHeadDim * 2;    // 32 KB: one 128 x 128 bf16 operand tile
 constexpr int kHalfTileBytes = kTileBytes / 2;    // one 64-column half
 constexpr int kPfSmemBytes = (2 + kPfKStages + kPfVStages) * kTileBytes + 1024 + 256;
+// Over fp16 rows the maximum that weights are taken against lies this far (base 2)
+// below the row's: weights up to 2^(8 + 6), so that f16 (which ends at 2^-24) holds
+// small ones too: each is off by 2^-31 of the largest at most besides its 11 bits,
+// where at their own size those below 2^-25 were lost from O but not from the sum
+// (60 queries behind a key 17.5 nats above 8131 others: 6 % of what these carry).
+// It cancels in O / l and is taken out of the lse.  The room above, 2^1.99, is the
+// maximum's own rounding: logits to 2^24.
+constexpr int kPfPBias = 6;
 constexpr float kRescaleThreshold = 8.0f;         // log2 units: rescale O only when the max grows by > 256x
 constexpr int kPfLaunchRegs = 168;                // 65536 / 384, rounded down to a multiple of 8
 constexpr int kPfProducerRegs = 88;
@@ -598,7 +606,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         for (int k = 0; k < 8; ++k)
           mv[k] = max3f(mv[k], __uint_as_float(sr[c + 2 * k]), __uint_as_float(sr[c + 2 * k + 1]));
       const float mx = max3f(max3f(mv[0], mv[1], mv[2]), max3f(mv[3], mv[4], mv[5]), fmaxf(mv[6], mv[7]));
-      const float mxs = mx * cl;
+      const float mxs = F16 ? fmaf(mx, cl, -(float)kPfPBias) : mx * cl;
       bool need = false;
       float alpha = 1.f;
       if (j == 0) {
@@ -623,7 +631,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
       }
       // P in fp16 (11 significant bits, 8x finer than bf16; p <= 2^8 after the
-      // lazy rescale, far inside fp16 range) packed in place over the scores
+      // lazy rescale, 2^14 with kPfPBias, inside fp16 range) packed in place over the scores
       // (step c reads sr[2c], sr[2c+1] and writes sr[c], c <= 2c) and stored
       // into S columns [0,64) in two halves of 64 keys.  Each half is released
       // to the MMA thread on its own barrier, so the P.V of keys 0..63 runs
@@ -733,7 +741,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         const int row_in_chunk = q0 + tpt * i + tok;
         const bool valid = tok < (i ? rows_valid[1] : rows_valid[0]);
         // a NaN key's row has l = NaN, and so its lse
-        const float lse = l == 0.f ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
+        const float lse2 = F16 ? (m_used + kPfPBias) + log2f(l * (1.f / (1 << kPfPBias))) : m_used + log2f(l);
+        const float lse = l == 0.f ? -INFINITY : lse2 * 0.69314718055994531f;
         if (valid && split_pair)
           a.part_lse[((size_t)blockIdx.y * a.n_pad + row_in_chunk) * a.n_heads + hr] = lse;
         else if (valid && a.lse)

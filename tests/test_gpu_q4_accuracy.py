@@ -50,6 +50,26 @@ def test_decode_weights_below_a_dominant_key(heads, n, rows):
     eng.close()
 
 
+@pytest.mark.parametrize("heads", [(28, 4), (16, 8)])
+def test_prefill_weights_below_a_dominant_key(heads):
+    """The expanded form's weights are f16 at 2^6 times their size: each is off by at most 2^-31 of the largest besides
+    its 11 bits; the values are fp16 too."""
+    n_heads, n_kv = heads
+    n, n_new = 8192, 60
+    k, v = _dominated(n, n_kv, 4)
+    eng = make_engine(n_heads, n_kv, [n], kv_dtype="q4")
+    eng.kv_write(0, 0, k.cuda(), v.cuda())
+    q = torch.ones(n_new, n_heads, 128, device="cuda", dtype=torch.bfloat16)
+    out = eng.prefill(0, 0, q).cpu().double().numpy()
+    eng.sync()
+    for i in (0, n_new - 1):
+        seen = n - n_new + i + 1
+        want = np.repeat(_dominated_want(v, seen), n_heads // n_kv, 0)
+        err = np.abs(out[i] - want)
+        assert (err <= seen * 2.0 ** -31 * 2.5 + 2.0 ** -9 * np.abs(want)).all(), (err.max(), np.abs(want).max())
+    eng.close()
+
+
 # ----------------------------------------------------------------------------------------------- the scale
 def _held(x):
     """The definition that include/oomattn.h gives: the scale is the range times 1/15 in f32, rounded to bf16."""
