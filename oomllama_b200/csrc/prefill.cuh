@@ -765,7 +765,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 // holds key 0, is never empty).  One warp per (row,
 // head), 4 dimensions per lane; rows of unsplit pairs, or outside the
 // launch's block ranges, were written by the prefill kernel itself.
-__global__ void prefill_chunk_merge_kernel(const float* __restrict__ part_o, const PrefillArgs a) {
+// As a programmatic dependent it is resident while the prefill still writes the
+// partials: they are not read-only memory to it (no __ldg, no __restrict__).
+__global__ void prefill_chunk_merge_kernel(const float* part_o, const PrefillArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // a programmatic dependent of the prefill
   const long long item = (blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
@@ -783,9 +785,9 @@ __global__ void prefill_chunk_merge_kernel(const float* __restrict__ part_o, con
   const int nc = (nt + a.key_chunk - 1) / a.key_chunk;
   // four chunks at a time: their loads are in flight together (333 rows of 32 heads in 3 chunks: 2 us less)
   constexpr int B = 4;
-  auto lse_at = [&](int c) { return a.part_lse[((size_t)c * a.n_pad + row) * a.n_heads + h]; };
+  auto lse_at = [&](int c) { return __ldcg(a.part_lse + ((size_t)c * a.n_pad + row) * a.n_heads + h); };
   auto o_at = [&](int c) {
-    return __ldg(reinterpret_cast<const float4*>(part_o + (((size_t)c * a.n_pad + row) * a.n_heads + h) * kHeadDim) + lane);
+    return __ldcg(reinterpret_cast<const float4*>(part_o + (((size_t)c * a.n_pad + row) * a.n_heads + h) * kHeadDim) + lane);
   };
   float ls[B];
   float4 o[B];
