@@ -68,9 +68,9 @@ enum { OOMATTN_DTYPE_F32 = 0, OOMATTN_DTYPE_BF16 = 1, OOMATTN_DTYPE_Q4 = 2 };
  *   s = f16(bf16((max x - min x) * (1/15))), o = f16(min x + 8 s),
  *   c = clamp(rint((x - o) / s) + 8, 0, 15)   (8 where s = 0)
  * and the row stands for o + (c - 8) s: 80 bytes instead of 256 in bf16, each
- * value off by at most 0.53 s + 2^-12 |o|.  Values saturate at +-60000; a
- * group that holds a NaN reads back as NaN; groups whose values differ by less
- * than about 1e-5 keep only their middle.
+ * value off by at most 0.53 s + 2^-11 |o| + 5e-7.  Values saturate at +-60000; a
+ * group that holds a NaN reads back as NaN; of groups whose values differ by less
+ * than 4.4e-7 only the least value is kept (s is 0).
  * A page of 16 tokens of one kv head is a chunk of OOMATTN_Q4_CHUNK bytes of K
  * and, right behind it, one of V: one pool, whose chunk of K (layer, page, kv)
  * lies at ((layer*(n_pages+1) + page)*n_kv + kv) * 2 * OOMATTN_Q4_CHUNK.

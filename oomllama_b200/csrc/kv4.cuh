@@ -7,13 +7,17 @@
 //   s = f16(bf16((max x - min x) * (1/15)))  (f32; 8 significant bits)
 //   o = f16(min x + 8 s)
 //   c = clamp(rint((x - o) / s) + 8, 0, 15)  (8 where s = 0)
-// and the group stands for o + (c - 8) s.  The roundings: a code is off by at
-// most half a step s; s rounded to 8 bits moves the end of a group's range by
-// at most 15 s 2^-9 < 0.03 s; o is off by at most 2^-12 |o|.  s has 8 bits so
-// that (c - 8) s, a 4-bit number times an 8-bit one, is exact in f16.  A group
-// that holds a NaN reads back as NaN; values saturate at +-60000, which keeps
-// s <= 8000 and (c - 8) s <= 64000 finite in f16.  5 bits per value, against
-// 16: 160 bytes instead of 512 for a token's K and V of one kv head.
+// and the group stands for o + (c - 8) s.  The roundings: codes are taken against
+// the rounded o and s, so a value in their range is off by at most half a step s.
+// s is off by 2^-8 of itself (bf16) or 2^-25 (where it is an f16 subnormal), which
+// moves the range's end by 15 times that, o by 2^-11 |o|: the least and greatest
+// value may lie outside by 0.06 s + 2^-11 |o| + 15 * 2^-25.  Together at most
+// 0.53 s + 2^-11 |o| + 5e-7.  s has 8 bits so that (c - 8) s, a 4-bit number times
+// an 8-bit one, is exact in f16.  A group that holds a NaN reads back as NaN;
+// values saturate at +-60000, which keeps s <= 8000 and (c - 8) s <= 64000 finite
+// in f16; s rounds to 0 below a range of 15 * 2^-25, and the group reads back as
+// its least value.  5 bits per value, against 16: 160 bytes instead of 512 for a
+// token's K and V of one kv head.
 //
 // The codes lie in the order in which the decode kernel's lanes want them as
 // tensor-core operands, so that a lane's 64-bit load is its operand and no
