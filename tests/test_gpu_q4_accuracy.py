@@ -101,6 +101,68 @@ def test_scale_on_a_border():
     eng.close()
 
 
+# ----------------------------------------------------------------------------------------------- the prefill's two forms
+def _filled(n_heads, n_kv, n, seed, cap):
+    eng = make_engine(n_heads, n_kv, [cap], kv_dtype="q4", shuffle_seed=seed)
+    for pool in eng.kv_pool():
+        pool.fill_(0xFF)  # NaN in every slot that is not written
+    k, v = (randn((n, n_kv, 128), seed + i, torch.bfloat16) for i in (1, 2))
+    eng.kv_write(0, 0, k.cuda(), v.cuda())
+    return eng, q4_ref.held(k).transpose(0, 1).double(), q4_ref.held(v).transpose(0, 1).double()
+
+
+def _by_rows(n_heads, n_kv, n_new, n):
+    """Whether the queries run as decode rows (include/oomattn.h)."""
+    most = 5 + 200000 // (n * n_kv) if n_heads // n_kv > 4 else 7 + 260000 // (n * n_kv)
+    return n_new <= min(48, most)
+
+
+def _expanded_bounds(q, k, v, seen):
+    """want, lse and how far the expanded form's may be off, for one query [Hq, 128] that sees `seen` keys.
+    K, V and the weights are rounded to 11 bits (2^-11 relative, q enters exactly): independent roundings c_i, of which
+    the sum stays within 7 sqrt(sum c_i^2) but for one in 10^10 (Hoeffding).  A score's are 2^-11 |q_d k_d| scale, and
+    reach the lse times w_j and the output times w_j (v - out).  The tensor core truncates a running sum once per 16
+    keys by 2^-23 of it; f32 does the rest."""
+    group = q.shape[0] // k.shape[0]
+    kk, vv = (t[:, :seen].repeat_interleave(group, 0) for t in (k, v))
+    scale, u = 1 / math.sqrt(128), 2.0 ** -11
+    s = torch.einsum("hd,hld->hl", q, kk) * scale
+    w = torch.softmax(s, -1)
+    want, lse = torch.einsum("hl,hld->hd", w, vv), torch.logsumexp(s, -1)
+    ds2 = torch.einsum("hd,hld->hl", q ** 2, kk ** 2) * (scale * u) ** 2
+    dlse = 7 * torch.sqrt((w ** 2 * ds2).sum(-1)) + 1e-5 + ds2.amax(-1) * 7
+    var = torch.einsum("hl,hld->hd", w ** 2 * ds2, (vv - want[:, None]) ** 2)
+    var = var + 2 * u * u * torch.einsum("hl,hld->hd", w ** 2, vv ** 2)
+    dout = 7 * torch.sqrt(var) + (seen * 2.0 ** -26 + ds2.amax() * 7) * vv.abs().amax()
+    return want, lse, dout, dlse
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(28, 4), (8, 8), (10, 2), (9, 3), (8, 2), (16, 2)])
+@pytest.mark.parametrize("n_new,prefix,rows", [(1, 0, True), (1, 50, True), (7, 9, True), (16, 100, True), (25, 111, True),
+                                               (24, 1200, True), (60, 0, False), (100, 28, False), (300, 500, False),
+                                               (60, 2000, False)])
+def test_prefill_within_its_form(heads, n_new, prefix, rows, out_dtype):
+    n = n_new + prefix
+    assert _by_rows(*heads, n_new, n) == rows
+    eng, k, v = _filled(*heads, n, 30, n + 100)
+    q = randn((n_new, heads[0], 128), 33, torch.bfloat16)
+    out, lse = eng.prefill(0, 0, q.cuda(), out_dtype=out_dtype, with_lse=True)
+    eng.sync()
+    out, lse = torch.from_numpy(as_f32_np(out)).double(), lse.cpu().double()
+    half = 2.0 ** -8 if out_dtype == torch.bfloat16 else 0.0
+    for i in sorted({*range(0, n_new, max(1, n_new // 16)), n_new - 1}):
+        want, want_lse, dout, dlse = _expanded_bounds(q[i].double(), k, v, prefix + i + 1)
+        if rows:  # q and p in 22 bits: the decode's bounds
+            dout, dlse = torch.full_like(dout, 1.5e-4), 1e-5 + 2e-6 * want_lse.abs()
+        err = (out[i] - want).abs() - half * want.abs()
+        assert (err <= dout * (1 + half)).all(), (i, float(err.max()))
+        assert ((lse[i] - want_lse).abs() <= dlse).all(), (i, float((lse[i] - want_lse).abs().max()))
+        if rows and not half:
+            assert (out[i] - want).norm() <= 1e-5 * want.norm()
+    eng.close()
+
+
 @pytest.mark.parametrize("kv_dtype", ["q4", "bf16"])
 @pytest.mark.parametrize("n_new,prefix", [(20, 0), (100, 100), (64, 4000)])
 def test_prefill_nan_key(n_new, prefix, kv_dtype):
