@@ -1930,6 +1930,7 @@ int oomattn_attention_forward_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t b
   int rc = check_layer(ctx, layer);
   if (!rc) rc = check_norm(ctx, norm);
   if (rc) return rc;
+  if (ctx->cfg.hidden_size <= 0) return fail(ctx, OOMATTN_ERR_BAD_CONFIG, "the context has no hidden_size");
   DeviceGuard dg(ctx->device);
   const long long T = (long long)batch * seq_len;
   const int hq = ctx->cfg.n_heads, qo = hq * kHeadDim;
