@@ -1622,6 +1622,8 @@ int oomattn_qkv_rope_append_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t n_s
   const long long T = (long long)n_seqs * n_new;
   const int nq = ctx->cfg.n_heads * kHeadDim, nk = ctx->cfg.n_kv_heads * kHeadDim;
   if (T <= kGemvMaxT && !rows_apart(ctx, norm)) {
+    if (!aligned16(x) || !aligned16(wq) || !aligned16(wk) || !aligned16(wv))
+      return fail(ctx, OOMATTN_ERR_INVALID_ARG, "x and the weights must be 16-byte aligned");
     SeqBatch sb;
     rc = plan_append(ctx, layer, n_seqs, seq_ids, n_new, sb);
     if (rc) return rc;

@@ -66,3 +66,20 @@ def test_static_scratch_pools(lib, kv_dtype):
                 0, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream), code, p(pool, k_off), p(pool, v_off), 4, p(bt), 4,
                 4, 1, ctypes.c_float(0.0), 1, arr([0]), arr([20]), p(q), p(out), None, err, 256) == 1, err.value
     torch.cuda.synchronize()
+
+
+def test_fused_projection():
+    from oomllama_b200._lib import OomAttnError
+    H = 256
+    eng = make_engine(2, 1, [40, 40], kv_dtype="bf16", hidden=H)
+    x, wq, wk = randn((3, H), 1).cuda(), randn((256, H), 2).cuda(), randn((128, H), 3).cuda()
+    odd = lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)  # noqa: E731
+    for args in ((odd(x), wq, wk, wk), (x, odd(wq), wk, wk), (x, wq, odd(wk), wk), (x, wq, wk, odd(wk))):
+        with pytest.raises(OomAttnError) as e:
+            eng.qkv_rope_append(0, [0], *args)
+        assert e.value.code == 1
+    assert eng.seq_len(0, 0) == 0
+    eng.qkv_rope_append(0, [0], x, wq, wk, wk)
+    eng.sync()
+    assert eng.seq_len(0, 0) == 3
+    eng.close()
