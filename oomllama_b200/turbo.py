@@ -65,6 +65,22 @@ def _dev(t: torch.Tensor, name: str, device: int, dtype=None, numel=None):
     return t
 
 
+def _ids(seq_ids, rows: int):
+    """The C array of a call's sequences, one for each of its rows."""
+    seq_ids = list(seq_ids)
+    if len(seq_ids) != rows:
+        raise ValueError(f"{len(seq_ids)} sequences for {rows} rows")
+    return int_array(seq_ids)
+
+
+def _room(t: torch.Tensor, name: str, device: int, numel: int, dtype=None):
+    """A buffer of the caller's that a kernel writes numel elements of."""
+    _dev(t, name, device, dtype=dtype)
+    if t.numel() < numel:
+        raise ValueError(f"{name} has {t.numel()} elements, {numel} are written")
+    return t
+
+
 @dataclass
 class TurboConfig:
     """TurboConfig (src/oomllama_turbo.rs:474-497) plus the settings the
@@ -310,10 +326,12 @@ class TurboEngine:
             _dev(bq, "bq", self.device, dtype=torch.float32, numel=c.n_heads * HEAD_DIM)
         if out is None:
             out = torch.empty(R, c.n_heads, HEAD_DIM, dtype=q_out_dtype, device=q.device)
+        else:
+            _room(out, "out", self.device, R * c.n_heads * HEAD_DIM)
         norm = self._qk_norm(q_norm, None, eps)
         self._bind_stream()
         check(self._ctx, self._L.oomattn_rope_q_qk_norm(self._ctx, R, int_array(positions), _ptr(q), _dtype_code(q),
-                                                        _ptr(bq), norm, _ptr(out), _DT[out.dtype]))
+                                                        _ptr(bq), norm, _ptr(out), _dtype_code(out)))
         return out
 
     def qkv_rope_append(self, layer: int, seq_ids, x, wq, wk, wv, bq=None, bk=None, bv=None,
@@ -323,12 +341,17 @@ class TurboEngine:
         seq_ids = list(seq_ids)
         c = self.config
         T = x.shape[0]
+        if not seq_ids or T % len(seq_ids):
+            raise ValueError("token count is not a multiple of the number of sequences")
         n_new = T // len(seq_ids)
         H = c.hidden_size
         _dev(x, "x", self.device, dtype=torch.float32, numel=T * H)
         _dev(wq, "wq", self.device, numel=c.n_heads * HEAD_DIM * H)
         _dev(wk, "wk", self.device, dtype=wq.dtype, numel=c.n_kv_heads * HEAD_DIM * H)
         _dev(wv, "wv", self.device, dtype=wq.dtype, numel=c.n_kv_heads * HEAD_DIM * H)
+        for name, b, n in (("bq", bq, c.n_heads), ("bk", bk, c.n_kv_heads), ("bv", bv, c.n_kv_heads)):
+            if b is not None:
+                _dev(b, name, self.device, dtype=torch.float32, numel=n * HEAD_DIM)
         q_out = torch.empty(T, c.n_heads, HEAD_DIM, dtype=q_out_dtype, device=x.device)
         norm = self._qk_norm(q_norm, k_norm, eps)
         self._bind_stream()
@@ -344,11 +367,17 @@ class TurboEngine:
         seq_ids = list(seq_ids)
         c = self.config
         rows = len(seq_ids)
+        lens = None if lens is None else list(lens)
+        _same_count(lens, seq_ids, "lens")
         _dev(q, "q", self.device, dtype=torch.float32, numel=rows * c.n_heads * HEAD_DIM)
         if out is None:
             out = torch.empty(rows, c.n_heads, HEAD_DIM, dtype=torch.float32, device=q.device)
+        else:
+            _room(out, "out", self.device, rows * c.n_heads * HEAD_DIM, dtype=torch.float32)
         if with_lse and lse is None:
             lse = torch.empty(rows, c.n_heads, dtype=torch.float32, device=q.device)
+        elif with_lse:
+            _room(lse, "lse", self.device, rows * c.n_heads, dtype=torch.float32)
         self._bind_stream()
         check(self._ctx, self._L.oomattn_decode(
             self._ctx, layer, rows, int_array(seq_ids), None if lens is None else int_array(lens), _ptr(q),
@@ -361,6 +390,8 @@ class TurboEngine:
         seq_ids = list(seq_ids)
         c = self.config
         rows = len(seq_ids)
+        lens = None if lens is None else list(lens)
+        _same_count(lens, seq_ids, "lens")
         _dev(q, "q", self.device, dtype=torch.float32, numel=rows * c.n_heads * HEAD_DIM)
         if out is None:
             out = torch.empty(rows, c.n_heads, _lib.PACKED_STRIDE, dtype=torch.float32, device=q.device)
@@ -392,15 +423,17 @@ class TurboEngine:
         _dev(q, "q", self.device, dtype=torch.bfloat16, numel=n_new * c.n_heads * HEAD_DIM)
         if out is None:
             out = torch.empty(n_new, c.n_heads, HEAD_DIM, dtype=out_dtype, device=q.device)
+        else:
+            _room(out, "out", self.device, n_new * c.n_heads * HEAD_DIM)
         lse = torch.empty(n_new, c.n_heads, dtype=torch.float32, device=q.device) if with_lse else None
         self._bind_stream()
         if blocks is None:
             check(self._ctx, self._L.oomattn_prefill(self._ctx, layer, seq, n_new, _ptr(q), _ptr(out),
-                                                     _DT[out.dtype], _ptr(lse)))
+                                                     _dtype_code(out), _ptr(lse)))
         else:
             flat = [int(x) for lo_hi in blocks for x in lo_hi]
             check(self._ctx, self._L.oomattn_prefill_blocks(self._ctx, layer, seq, n_new, _ptr(q), _ptr(out),
-                                                            _DT[out.dtype], _ptr(lse), len(blocks),
+                                                            _dtype_code(out), _ptr(lse), len(blocks),
                                                             int_array(flat)))
         return (out, lse) if with_lse else out
 
@@ -497,7 +530,8 @@ class TurboEngine:
         _dev(x, "x", self.device, dtype=torch.float32)
         if residual is not None:
             _dev(residual, "residual", self.device, dtype=torch.float32, numel=T * down.rows)
-        out = torch.empty(T, down.rows, dtype=torch.float32, device=x.device) if out is None else out
+        out = (torch.empty(T, down.rows, dtype=torch.float32, device=x.device) if out is None
+               else _room(out, "out", self.device, T * down.rows, dtype=torch.float32))
         self._bind_stream()
         check(self._ctx, self._L.oomattn_q8_mlp(self._ctx, ctypes.byref(gate.c_struct()), ctypes.byref(up.c_struct()),
                                                 ctypes.byref(down.c_struct()), _ptr(x), T, _ptr(residual), _ptr(out)))
@@ -510,7 +544,7 @@ class TurboEngine:
         _dev(x, "x", self.device, dtype=torch.float32)
         out = torch.empty_like(x) if out is None else _dev(out, "out", self.device, dtype=torch.float32, numel=B * H)
         self._bind_stream()
-        ids = int_array(seq_ids)
+        ids = _ids(seq_ids, B)
         norm = self._qk_norm(w.q_norm, w.k_norm, w.eps)
         check(self._ctx, self._L.oomattn_decoder_layer_q8_qk_norm(self._ctx, layer, B, ids, _ptr(x),
                                                                   ctypes.byref(w.c_struct()), norm, _ptr(out)))
@@ -562,7 +596,7 @@ class TurboEngine:
         if logits is not None:
             _dev(logits, "logits", self.device, dtype=torch.float32, numel=B * model.lm_head.rows)
         self._bind_stream()
-        ids = int_array(seq_ids)
+        ids = _ids(seq_ids, B)
         check(self._ctx, self._L.oomattn_decode_step_q8_qk_norm(self._ctx, ctypes.byref(model.c_struct()),
                                                                 model.c_norms(self), B, ids, _ptr(tokens), _ptr(nxt),
                                                                 None if logits is None else _ptr(logits)))
@@ -580,7 +614,7 @@ class TurboEngine:
             _dev(logits, "logits", self.device, dtype=torch.float32, numel=B * model.lm_head.rows)
         self._bind_stream()
         check(self._ctx, self._L.oomattn_prefill_step_q8_qk_norm(self._ctx, ctypes.byref(model.c_struct()),
-                                                                 model.c_norms(self), B, int_array(seq_ids), n_new,
+                                                                 model.c_norms(self), B, _ids(seq_ids, B), n_new,
                                                                  _ptr(tokens), _ptr(nxt),
                                                                  None if logits is None else _ptr(logits)))
         return nxt
