@@ -23,7 +23,9 @@
  *    oomattn_sync and oomattn_kv_read.
  *  - Calls may be captured into CUDA graphs once the same calls have run (their
  *    scratch is allocated by the first one of a size; a capture in which it would
- *    grow is refused).  Scratch that a captured call used stays for its graph when
+ *    grow is refused).  Lengths, positions and the decode's schedule are fixed at
+ *    capture: a replay works at the lengths of that time, so a generation loop of
+ *    growing sequences calls.  Scratch that a captured call used stays for its graph when
  *    a later call needs more, until the context is destroyed.  Graphs of one
  *    context share its scratch: they do not run at the same time as one another,
  *    nor as the context's other calls.
@@ -350,8 +352,10 @@ int oomattn_decode_static_scratch_status(int device, void* stream, int32_t* flag
 /* Causal prefill of the n_new newest tokens of `seq` (bf16 or 4-bit cache):
  * query i (absolute slot len-n_new+i) attends to slots 0..len-n_new+i.
  * Over a 4-bit cache few queries (up to 5 + 200000 / (len * n_kv_heads), with
- * groups of at most four heads 7 + 260000 / (len * n_kv_heads), at most 48) run as decode rows, without limits on values; more take the cached rows and
- * q as fp16, and a q value of magnitude 65536 or more, or a NaN in q or V, gives
+ * groups of at most four heads 7 + 260000 / (len * n_kv_heads), at most 48) run as
+ * decode rows, without limits on values, an f32 out within 1e-5 in norm; more take
+ * the cached rows, q and the weights as fp16 (an f32 out about 2e-4 off in norm),
+ * and a q value of magnitude 65536 or more, or a NaN in q or V, gives
  * OOMATTN_ERR_DEVICE_CHECK at oomattn_sync.
  *   q: bf16 [n_new][n_heads][128] rotated; out: [n_new][n_heads][128] in
  *   out_dtype; lse: f32 [n_new][n_heads] or NULL. */

@@ -58,8 +58,8 @@ namespace oomattn {
 constexpr int kQ4Pages = 2;                              // pages per tile
 constexpr int kQ4Tile = kQ4Pages * kPageSize;            // tokens per tile
 constexpr int kQ4TileBytes = kQ4Pages * kQ4Pair;         // 5 KB
-// The narrow form fits 128 registers and the wide one 168: four CTAs of two
-// stages each, or three of three, per SM -- about 160 and 180 KB in flight.
+// The narrow form has 128 registers (8 bytes spilled) and the wide one 168: four
+// CTAs of two stages each, or three of three, per SM -- about 160 and 180 KB in flight.
 __host__ __device__ constexpr int q4_stages(bool wide) { return !wide ? 2 : 3; }
 __host__ __device__ constexpr int q4_ctas_per_sm(bool wide) { return !wide ? 4 : 3; }
 // The running maximum that weights are taken against lies this far (base 2) below

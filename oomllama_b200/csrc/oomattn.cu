@@ -1132,8 +1132,10 @@ int q4_expand(oomattn_ctx* ctx, int layer, int seq, int L, KVPool* pool, CUtenso
 // tiles and kUnit more, and the chunks' partials are written and read once.
 // Against the rule of prefill_impl (chunks of the work per SM): 700 queries behind
 // 9001 tokens of 32q/8kv 140 instead of 150 us, 32 behind 2000 17 instead of 19,
-// 1024 behind 9001 of 40q/8kv 251 instead of 299.  Making a plan takes 20 to 60 us
-// of the host.
+// 1024 behind 9001 of 40q/8kv 251 instead of 299.  Making a plan takes 10 us of the
+// host (4096 queries) to 83 (333 behind 9001) and 117 (100 behind 30000 of 40q/8kv);
+// the last one is kept, so the layers of a step over one sequence share it, and
+// sequences of unlike lengths in one step plan again at every layer.
 PrefillPlan plan_prefill(const oomattn_ctx* ctx, int n_new, int L) {
   constexpr int kScale = 16, kUnit = 2 * kScale, kMaxChunks = 32, kMaxItems = 600, kMaxSms = 1024;
   const int sms = std::min(ctx->num_sms, kMaxSms);
@@ -1175,10 +1177,13 @@ PrefillPlan plan_prefill(const oomattn_ctx* ctx, int n_new, int L) {
 // Prefill over a 4-bit cache, few tokens (drafts to verify, a short tail of a
 // prompt): each as one decode row that sees the slots up to its own.  The rows'
 // time grows with queries * tokens * kv heads, the expanded form's hardly with the
-// queries; by rows and expanded (us) 8 queries behind 30000 tokens of 28q/4kv take
-// 46.3 and 44.9, 12 behind 8000 21.9 and 24.5, 20 behind 4000 20.9 and 20.6, 32
-// behind 2000 18.5 and 17.2, 48 behind 1000 15.9 and 16.3; of 32q/8kv (the narrow
-// decode) 8 behind 9001 23.4 and 29.1, 12 31.2 and 29.2, 20 behind 2000 17.6 and 16.8.
+// queries; by rows and expanded (us, L2 flushed, launch gaps and events included) 8
+// queries behind 30000 tokens of 28q/4kv take 53.2 and 54.3, 12 behind 8000 28.6 and
+// 33.8, 20 behind 4000 26.6 and 27.6, 32 behind 2000 24.5 and 23.5, 48 behind 1000
+// 22.4 and 21.5; of 32q/8kv (the narrow decode) 8 behind 9001 28.7 and 37.9, 12 36.8
+// and 37.9, 20 behind 2000 22.5 and 23.5.  (The rule was set with the cache in L2,
+// where the forms meet a little earlier: 12 behind 8000 21.9 and 24.5, 20 behind 4000
+// 20.9 and 20.6.)
 constexpr int kQ4PrefillRows = 48;
 int q4_prefill_max_rows(const oomattn_ctx* ctx, int L) {
   const long long keys = (long long)L * ctx->cfg.n_kv_heads;

@@ -9,8 +9,8 @@
 // Measured on that prompt (70 MB, floor 10.6 us): 23.2 us into the 4-bit cache,
 // 18.0 us into a bf16 one (76 MB, 11.5); without a norm rope_append_kernel takes
 // 14.0.  Bound by the latency of its loads (ncu: long scoreboard 3.5 of 9 stall
-// cycles, issue 2.6 of 4, DRAM 17 %): four CTAs per SM at 64 registers were the
-// best of three to six.  64 tokens of 32q/8kv take 7.3 us with the gather of
+// cycles, issue 2.6 of 4, DRAM 17 %): four CTAs per SM at 64 registers (4 bytes
+// spilled into a 4-bit cache) were the best of three to six.  64 tokens of 32q/8kv take 7.3 us with the gather of
 // their rows, launch latency.
 #pragma once
 #include "common.cuh"
