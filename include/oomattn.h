@@ -276,7 +276,8 @@ int oomattn_qkv_rope_append_qk_norm(oomattn_ctx* ctx, int32_t layer, int32_t n_s
  * slots of sequence seq_ids[z] (lens NULL: the whole current length).
  *   q: f32 [n_rows][n_heads][128] rotated; out: f32 [n_rows][n_heads][128];
  *   lse: f32 [n_rows][n_heads] natural-log LSE of the scaled scores, or NULL.
- *   q (8-byte over a bf16 cache) and out must be 16-byte aligned. */
+ *   q (8-byte over a bf16 cache) and out must be 16-byte aligned.  Over a 4-bit
+ *   cache scores are to stay within +-1e8. */
 int oomattn_decode(oomattn_ctx* ctx, int32_t layer, int32_t n_rows, const int32_t* seq_ids /* host */,
                    const int32_t* lens /* host, may be NULL */, const float* q, float* out, float* lse);
 

@@ -64,8 +64,8 @@ __host__ __device__ constexpr int q4_stages(bool wide) { return !wide ? 2 : 3; }
 __host__ __device__ constexpr int q4_ctas_per_sm(bool wide) { return !wide ? 4 : 3; }
 // The running maximum that weights are taken against lies this far (base 2) below
 // the largest logit: weights in (0, 2^14], and so l and O, which cancels in O / l
-// and in the lse.  An f16 high part holds up to 2^15.99, which leaves room for the
-// maximum's own rounding (half a unit of its last place: logits to 2^24).
+// and in the lse.  It is rounded up, so that no weight passes 2^14 where a unit of
+// its last place is large (logits of 2^25 and more), which f16 would not hold.
 constexpr int kQ4PBias = 14;
 __host__ __device__ constexpr int q4_ring_bytes(bool wide) { return kDecWarps * q4_stages(wide) * kQ4TileBytes; }
 __host__ __device__ constexpr int q4_tail_bytes(bool wide) {  // barriers, a flag, merge weights
@@ -395,8 +395,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, q4_ctas_per_sm(WIDE))
       float mt = fmaxf(max3f(sc[h][0], sc[h][1], sc[h][2]), sc[h][3]);
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, off));
-      // the running maximum is rounded: the same number enters every weight, so its rounding cancels
-      const float mf = fmaxf(m[h], fmaf(mt, f2[h], -(float)kQ4PBias));
+      // the running maximum is rounded (up): the same number enters every weight, so its rounding cancels
+      const float mf = fmaxf(m[h], __fmaf_ru(mt, f2[h], -(float)kQ4PBias));
       alpha[h] = ex2_ftz(m[h] - mf);
       m[h] = mf;
       float ps = 0.f;

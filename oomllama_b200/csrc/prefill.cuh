@@ -45,8 +45,8 @@ constexpr int kPfSmemBytes = (2 + kPfKStages + kPfVStages) * kTileBytes + 1024 +
 // small ones too: each is off by 2^-31 of the largest at most besides its 11 bits,
 // where at their own size those below 2^-25 were lost from O but not from the sum
 // (60 queries behind a key 17.5 nats above 8131 others: 6 % of what these carry).
-// It cancels in O / l and is taken out of the lse.  The room above, 2^1.99, is the
-// maximum's own rounding: logits to 2^24.
+// It cancels in O / l and is taken out of the lse.  The maximum is rounded up, so
+// that no weight passes 2^14 where a unit of its last place is large.
 constexpr int kPfPBias = 6;
 constexpr float kRescaleThreshold = 8.0f;         // log2 units: rescale O only when the max grows by > 256x
 constexpr int kPfLaunchRegs = 168;                // 65536 / 384, rounded down to a multiple of 8
@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         for (int k = 0; k < 8; ++k)
           mv[k] = max3f(mv[k], __uint_as_float(sr[c + 2 * k]), __uint_as_float(sr[c + 2 * k + 1]));
       const float mx = max3f(max3f(mv[0], mv[1], mv[2]), max3f(mv[3], mv[4], mv[5]), fmaxf(mv[6], mv[7]));
-      const float mxs = F16 ? fmaf(mx, cl, -(float)kPfPBias) : mx * cl;
+      const float mxs = F16 ? __fmaf_ru(mx, cl, -(float)kPfPBias) : mx * cl;
       bool need = false;
       float alpha = 1.f;
       if (j == 0) {

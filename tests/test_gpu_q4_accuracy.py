@@ -70,6 +70,44 @@ def test_prefill_weights_below_a_dominant_key(heads):
     eng.close()
 
 
+@pytest.mark.parametrize("heads", [(4, 2), (16, 2)])
+@pytest.mark.parametrize("qscale", [1e2, 1e3])
+def test_scores_of_a_hundred_million(heads, qscale):
+    """Keys at the edge of the format and large queries: scores (base 2) around 2^23 and 2^26.7, of which a unit in the
+    last place is 1 and 8.  The running maximum is rounded up, so that no weight passes 2^14, whatever that rounding is,
+    and f16 holds it: the greatest score takes all, as in 64 bits, where the next is a million behind.  What a value is
+    then off by: decode, the weight's 22 bits on its offset and its code's share, |o| + |8 s| <= 3 max |v|, each; prefill,
+    the 11 bits of the weight and of the value."""
+    n_heads, n_kv = heads
+    n, n_new = 500, 70
+    k = (2e4 * randn((n, n_kv, 128), 1)).clamp(-59000, 59000)
+    v = randn((n, n_kv, 128), 2, torch.bfloat16).float()
+    eng = make_engine(n_heads, n_kv, [n], kv_dtype="q4")
+    eng.kv_write(0, 0, k.cuda(), v.cuda())
+    kh, vh = q4_ref.held(k).transpose(0, 1).double(), q4_ref.held(v).transpose(0, 1).double()
+    q = qscale * randn((n_new, n_heads, 128), 3, torch.bfloat16)
+    lens = [n - n_new + i + 1 for i in range(n_new)]
+    want, want_lse = q4_ref.attend(q, kh, vh, lens)
+    # a score is off by 2^-20 (decode), or 2^-11 for the keys' own rounding, of sum |q_d k_d| / sqrt(128) at most: rows
+    # whose two greatest scores lie twice that apart are one value's alone
+    s = torch.einsum("thd,hld->thl", q.double(), kh.repeat_interleave(n_heads // n_kv, 0)) / 128 ** 0.5
+    seen = torch.arange(n)[None, None] < torch.tensor(lens)[:, None, None]
+    top = s.masked_fill(~seen, -math.inf).topk(2, -1).values
+    size = (q.double().abs().sum(-1) * kh.abs().amax() / 128 ** 0.5).numpy()
+    vmax = float(vh.abs().max())
+    for form, got, lse in (("decode", *eng.decode(0, [0] * n_new, q.float().cuda(), lens=lens, with_lse=True)),
+                           ("prefill", *eng.prefill(0, 0, q.cuda(), with_lse=True))):
+        got, lse = got.cpu().double().numpy(), lse.cpu().double().numpy()
+        off = 2.0 ** -20 if form == "decode" else 2.0 ** -11
+        clear = (top[..., 0] - top[..., 1]).numpy() > 2 * off * size
+        assert np.isfinite(got).all() and clear.mean() > 0.5, form
+        bound = 6 * 2.0 ** -22 * vmax if form == "decode" else 2.0 ** -10 * np.abs(want) + 2.0 ** -22 * vmax
+        assert (np.abs(got - want) <= bound)[clear].all(), form
+        assert (np.abs(lse - want_lse) <= off * size).all(), form
+    eng.sync()
+    eng.close()
+
+
 # ----------------------------------------------------------------------------------------------- the scale
 def _held(x):
     """The definition that include/oomattn.h gives: the scale is the range times 1/15 in f32, rounded to bf16."""
